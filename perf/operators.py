@@ -162,7 +162,7 @@ def _prepare_plan(c, seed):
     table = torch.full((n, stride), -1, dtype=torch.int32, device=DEV)
     at = torch.arange(stride, device=DEV)[None, :] < _ints(pages)[:, None]
     table[at] = perm[: sum(pages)]
-    cap = sum(add) + 3                              # rows behind the last token stay as they are
+    cap = sum(add) + 3                              # rows behind the last token have no slot
     return {"c": c, "held": _ints(held), "add": _ints(add), "free": perm[sum(pages):].contiguous(), "table": table,
             "taken_in": _ints([5]), "taken": _ints([0]), "q_start": _ints([0] * (n + 1)), "kv_len": _ints([0] * n),
             "slot": torch.full((cap,), -7, dtype=torch.int32, device=DEV),
@@ -267,8 +267,8 @@ def _plain_plan(st):
     slot = torch.where(pg >= 0, pg * page + p % page, -1).int()
     live = t < end[-1]
     lost = add.sum() - ((slot >= 0) & live).sum()
-    return {"table": table, "q_start": start.int(), "kv_len": kv.int(), "slot": torch.where(live, slot, st["slot"]),
-            "pos": torch.where(live, p.int(), st["pos"]), "taken": (st["taken_in"] + need.sum()).int(),
+    return {"table": table, "q_start": start.int(), "kv_len": kv.int(), "slot": torch.where(live, slot, -1),
+            "pos": torch.where(live, p, 0).int(), "taken": (st["taken_in"] + need.sum()).int(),
             "info": torch.stack([end[-1], lost]).int()}
 
 

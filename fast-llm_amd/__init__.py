@@ -137,6 +137,56 @@ class WeightInfo(C.Structure):
                 ("estride", C.c_uint64), ("host", C.c_void_p), ("tensor", C.c_uint64)]
 
 
+class Dtype(enum.IntEnum):
+    """FLH_DT_*: element types of activations and of the key/value cache."""
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+
+
+class RopeLayout(enum.IntEnum):
+    """FLH_ROPE_*: pair i is elements (i, i + n_rot/2) or (2i, 2i + 1)."""
+    HALVES = 0
+    PAIRS = 1
+
+
+KV_NONE = 0xFFFFFFFF
+
+
+class _KvCacheC(C.Structure):
+    """flh_kv_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_uint32), ("n_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_kv_head", C.c_uint32), ("d_k", C.c_uint32), ("d_v", C.c_uint32),
+                ("k_page", C.c_uint64), ("k_tok", C.c_uint64), ("k_head", C.c_uint64), ("v_page", C.c_uint64),
+                ("v_tok", C.c_uint64), ("v_head", C.c_uint64)]
+
+
+class KvPlanP(C.Structure):
+    """flh_kv_plan_p (pointers are device addresses)."""
+    _fields_ = [("held", C.c_void_p), ("add", C.c_void_p), ("free_pages", C.c_void_p), ("taken_in", C.c_void_p),
+                ("taken", C.c_void_p), ("table", C.c_void_p), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("slot", C.c_void_p), ("pos", C.c_void_p), ("info", C.c_void_p), ("n_seq", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_free", C.c_uint32), ("table_stride", C.c_uint32), ("max_tok", C.c_uint32)]
+
+
+class RopeKvP(C.Structure):
+    """flh_rope_kv_p (pointers are device addresses, strides in elements)."""
+    _fields_ = [("q", C.c_void_p), ("q_out", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("pos", C.c_void_p),
+                ("slot", C.c_void_p), ("q_tok", C.c_uint64), ("q_head", C.c_uint64), ("qo_tok", C.c_uint64),
+                ("qo_head", C.c_uint64), ("k_tok", C.c_uint64), ("k_head", C.c_uint64), ("v_tok", C.c_uint64),
+                ("v_head", C.c_uint64), ("dtype", C.c_uint32), ("n_tok", C.c_uint32), ("n_head", C.c_uint32),
+                ("pos_stride", C.c_uint32)]
+
+
+class AttnP(C.Structure):
+    """flh_attn_p (pointers are device addresses, strides in elements)."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("table", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t), ("q_tok", C.c_uint64),
+                ("q_head", C.c_uint64), ("o_tok", C.c_uint64), ("o_head", C.c_uint64), ("dtype", C.c_uint32),
+                ("n_head", C.c_uint32), ("n_seq", C.c_uint32), ("n_tok", C.c_uint32), ("max_q", C.c_uint32),
+                ("table_stride", C.c_uint32), ("causal", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float)]
+
+
 class FlhError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"fastllm_hip error {code}: {msg}")
@@ -194,6 +244,13 @@ _SIGS = {
     "flh_rmsnorm_act_q8": (_I, [_P, _P, _P, _U32, C.c_float, _I, _P]),
     "flh_rmsnorm_stream_dot": (_I, [_I, _P, _U64, _U32, _U32, _P, _P, C.c_float, _P, _P, _I, _U32, _U32, _P]),
     "flh_wmerge": (_I, [_P, _P, _P, _P, _P, _F, _U32, _U32, _U32, _U32, _U32, _U32, _P]),
+    "flh_kv_plan": (_I, [_P, _P]),
+    "flh_rope_table_create": (_I, [_U32, _U32, _I, C.c_double, _P, _U32, _P, C.POINTER(_P)]),
+    "flh_rope_table_destroy": (_I, [_P]),
+    "flh_rope": (_I, [_P, _U32, _P, _U64, _U64, _P, _U64, _U64, _U32, _U32, _U32, _P, _U32, _P]),
+    "flh_rope_kv_append": (_I, [_P, _P, _P, _P]),
+    "flh_paged_attn_ws_bytes": (_SZ, [_P, _P]),
+    "flh_paged_attn": (_I, [_P, _P, _P]),
     "flh_fill_normal": (_I, [_P, _SZ, _U64, _F, _F, _F, _F, _P]),
     "flh_quantize": (_I, [_I, _P, _U32, _U32, _P, _P]),
     "flh_quantize_host": (_I, [_I, _P, _U32, _U32, _P]),
@@ -281,6 +338,14 @@ class Stream:
         h = C.c_void_p()
         check(lib().flh_stream_create(C.byref(h)))
         self.handle = h.value
+
+    @classmethod
+    def wrap(cls, handle: int) -> "Stream":
+        """Another program's stream (a hipStream_t; 0: the default stream) for
+        the calls here.  It stays that program's: do not close() it."""
+        s = cls.__new__(cls)
+        s.handle = handle
+        return s
 
     def sync(self):
         check(lib().flh_stream_sync(self.handle))
@@ -509,6 +574,73 @@ def wmerge(parts, gates, add1, add2, y, scale, n_parts, n, n_full, ncol, pstride
            stream: Stream):
     check(lib().flh_wmerge(_p(parts), _p(gates), _p(add1), _p(add2), _p(y), scale, n_parts, n,
                            n_full, ncol, pstride, ystride, stream.handle))
+
+
+# ------------------------------------------- paged cache and attention --
+class KvCache:
+    """A paged key/value cache of one layer (flh_kv_cache).  k_strides and
+    v_strides: elements between pages, tokens of a page, kv heads."""
+
+    def __init__(self, k, v, dtype: int, n_pages: int, page_size: int, n_kv_head: int, d_k: int, d_v: int, k_strides,
+                 v_strides):
+        self.c = _KvCacheC(_p(k), _p(v), int(dtype), n_pages, page_size, n_kv_head, d_k, d_v, *k_strides, *v_strides)
+
+
+class RopeTable:
+    """Rotary frequencies (flh_rope_table_create): n_rot elements of a head from
+    `first` on; freq: radians per position of each pair (default base^(-2i /
+    n_rot)); axis: the position axis of each pair (default 0)."""
+
+    def __init__(self, n_rot: int, base: float = 10000.0, freq=None, axis=None, n_axis: int = 1, first: int = 0,
+                 layout: int = RopeLayout.HALVES):
+        self.handle = None
+        f = None if freq is None else np.ascontiguousarray(freq, dtype=np.float64)
+        a = None if axis is None else np.ascontiguousarray(axis, dtype=np.uint8)
+        for v in (f, a):
+            if v is not None and v.size != n_rot // 2:
+                raise ValueError("freq and axis have one entry per pair")
+        h = C.c_void_p()
+        check(lib().flh_rope_table_create(n_rot, first, int(layout), base, None if f is None else f.ctypes.data, n_axis,
+                                          None if a is None else a.ctypes.data, C.byref(h)))
+        self.handle = h.value
+
+    def close(self):
+        if self.handle and lib():
+            lib().flh_rope_table_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def kv_plan(p: KvPlanP, stream: Stream) -> None:
+    """Pages for the tokens that requests add, their slots and positions."""
+    check(lib().flh_kv_plan(C.byref(p), stream.handle))
+
+
+def rope(table: RopeTable, dtype: int, x, x_tok: int, x_head: int, y, y_tok: int, y_head: int, n_tok: int, n_head: int,
+         d: int, pos, pos_stride: int, stream: Stream) -> None:
+    """Rotary positions on n_head heads of n_tok tokens, x -> y (may be x)."""
+    check(lib().flh_rope(table.handle, int(dtype), _p(x), x_tok, x_head, _p(y), y_tok, y_head, n_tok, n_head, d, _p(pos),
+                         pos_stride, stream.handle))
+
+
+def rope_kv_append(table: RopeTable | None, cache: KvCache, p: RopeKvP, stream: Stream) -> None:
+    """Rotary positions on queries and keys, keys and values into the cache."""
+    check(lib().flh_rope_kv_append(table.handle if table else None, C.byref(cache.c), C.byref(p), stream.handle))
+
+
+def paged_attn_ws_bytes(cache: KvCache, p: AttnP) -> int:
+    """Workspace bytes of paged_attn with these arguments."""
+    return lib().flh_paged_attn_ws_bytes(C.byref(cache.c), C.byref(p))
+
+
+def paged_attn(cache: KvCache, p: AttnP, stream: Stream) -> None:
+    """Attention of new tokens over the paged cache."""
+    check(lib().flh_paged_attn(C.byref(cache.c), C.byref(p), stream.handle))
 
 
 def fill_normal(dst, n: int, seed: int, stream: Stream, mean: float = 0.0, std: float = 1.0,

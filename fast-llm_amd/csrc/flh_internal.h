@@ -8,6 +8,7 @@
 #include <memory>
 #include <mutex>
 #include <shared_mutex>
+#include "../../include/fastllm_hip.h"
 
 namespace flh {
 
@@ -195,6 +196,34 @@ int launch_merge(const float * x, float * y, uint32_t rows, uint32_t nparts,
                  hipStream_t s);
 int launch_quantize_weights(int fmt, const float * src, uint32_t rows,
                             uint32_t cols, uint8_t * dst, hipStream_t s);
+// The paged cache (flh_kv.hip) and attention over it (flh_attn.hip).
+struct RopePair {
+    uint64_t frac;                      // turns per position, in 2^-64
+    uint32_t axis, pad;
+};
+// q (rotated) -> qo, and with kc the keys (rotated) and values into the cache;
+// strides in elements; rot null: nothing is rotated
+struct RopeArgs {
+    const void * q; void * qo; const void * k; const void * v;
+    void * kc; void * vc;
+    const RopePair * rot;
+    const int32_t * pos; const uint32_t * slot;
+    uint64_t q_tok, q_head, qo_tok, qo_head, k_tok, k_head, v_tok, v_head;
+    uint64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head;
+    uint32_t n_tok, n_head, n_kv, d, dv, n_rot, first, halves, pos_stride, n_slot, sh;
+};
+struct AttnArgs {
+    const void * q; void * out; const void * k; const void * v;
+    const uint32_t * q_start; const uint32_t * kv_len; const uint32_t * table;
+    void * ws;
+    uint64_t q_tok, q_head, o_tok, o_head, k_page, k_tok, k_head, v_page, v_tok, v_head;
+    uint32_t n_pages, sh, n_kv, dk, dv, group, n_seq, n_tok, max_q, table_stride, causal, window;
+    float scale;
+};
+int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s);
+int launch_rope(const RopeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
+size_t attn_ws_bytes(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype);
+int launch_attn(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 int launch_fill_normal(float * dst, size_t n, uint64_t seed, float mean,
                        float stddev, float outlier_frac, float outlier_scale,
                        hipStream_t s);

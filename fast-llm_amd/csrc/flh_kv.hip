@@ -1,0 +1,239 @@
+// flh_kv.hip -- the paged key/value cache's book-keeping and writes: block
+// tables and slot maps from request lengths, rotary positions, and the append
+// of keys and values.
+#include "flh_common.h"
+#include "flh_internal.h"
+#include "flh_status.h"
+
+namespace flh {
+
+// ------------------------------------------------------------------- plan --
+// One workgroup walks the requests 1024 at a time (thread per request): an
+// exclusive scan of the new rows and of the pages needed, carried from batch to
+// batch, gives every request its first row and its first entry of the free list;
+// then the batch's new pages and (rows <= PLAN_ROWS) rows are dealt to the
+// threads flat, each finding its request by a binary search over the scan in
+// LDS.  More rows go to k_kv_slots, a launch over all CUs behind this one.  One
+// workgroup, so taken and kv_len may be updated in place: nobody else reads
+// them.  Sums are 64-bit (a garbage length costs its own rows only).
+constexpr uint32_t PLAN_T = 1024;
+
+__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, uint32_t d) {
+    const uint32_t lo = __shfl_up((uint32_t)v, d), hi = __shfl_up((uint32_t)(v >> 32), d);
+    return ((uint64_t)hi << 32) | lo;
+}
+// inclusive scan of v over the workgroup (ws: 16 wave sums); total in *sum
+__device__ __forceinline__ uint64_t scan_wg(uint64_t v, uint64_t * ws, uint64_t * sum) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint64_t o = shfl_up64(v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();                                              // ws may hold the scan before
+    if (lane == 63) ws[wave] = v;
+    __syncthreads();
+    uint64_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < PLAN_T / 64; ++w) {
+        if (w < wave) before += ws[w];
+        all += ws[w];
+    }
+    *sum = all;
+    return v + before;
+}
+__device__ __forceinline__ uint32_t sat32(uint64_t v) { return v > 0xFFFFFFFFull ? 0xFFFFFFFFu : (uint32_t)v; }
+
+// the last of n requests (n >= 1) whose entry of the ascending at is <= i
+template <typename T>
+__device__ __forceinline__ uint32_t owner(const T * at, uint32_t n, T i) {
+    uint32_t lo = 0;
+    while (n > 1) {
+        const uint32_t h = n >> 1;
+        if (at[lo + h] <= i) { lo += h; n -= h; }
+        else n = h;
+    }
+    return lo;
+}
+__device__ __forceinline__ uint32_t slot_of(uint32_t page, uint32_t at, uint32_t sh) {
+    return page > (0xFFFFFFFEu >> sh) ? FLH_KV_NONE : (page << sh) | (at & ((1u << sh) - 1u));
+}
+
+__global__ __launch_bounds__(PLAN_T) void k_kv_plan(flh_kv_plan_p p, uint32_t sh, int rows_too) {
+    __shared__ uint64_t ws[PLAN_T / 64], l_page[PLAN_T];
+    __shared__ uint32_t l_row[PLAN_T], l_held[PLAN_T], l_before[PLAN_T];
+    const uint32_t tid = threadIdx.x;
+    const uint64_t ps = 1ull << sh;
+    uint64_t row0 = 0, page0 = p.taken_in ? *p.taken_in : 0, lost = 0;
+    for (uint32_t base = 0; base < p.n_seq; base += PLAN_T) {
+        const uint32_t s = base + tid, nb = min(PLAN_T, p.n_seq - base);
+        const bool in = tid < nb;
+        const uint64_t held = in ? p.held[s] : 0, add = in ? p.add[s] : 0;
+        uint64_t sum;
+        const uint64_t end = row0 + scan_wg(add, ws, &sum);
+        const uint32_t r0 = (uint32_t)min(end - add, (uint64_t)p.max_tok), r1 = (uint32_t)min(end, (uint64_t)p.max_tok);
+        row0 += sum;
+        const uint64_t kv = held + (r1 - r0);
+        const uint64_t before = min((held + ps - 1) >> sh, (uint64_t)p.table_stride);
+        const uint64_t need = min((kv + ps - 1) >> sh, (uint64_t)p.table_stride) - before;
+        const uint64_t first = page0 + scan_wg(need, ws, &sum) - need;
+        const uint64_t pages = sum;
+        l_row[tid] = r0;
+        l_held[tid] = (uint32_t)held;
+        l_before[tid] = (uint32_t)before;
+        l_page[tid] = first - page0;
+        if (in) {
+            // rows with a slot: in the page begun before (if the table holds one), and
+            // in the new pages that the free list had
+            uint64_t ok = 0;
+            if (held < before << sh) {
+                const uint32_t g = p.table[(uint64_t)s * p.table_stride + before - 1];
+                if (slot_of(g, 0, sh) != FLH_KV_NONE) ok = min(kv, before << sh) - held;
+            }
+            const uint64_t got = first >= p.n_free ? 0 : min(need, p.n_free - first);
+            if (need) ok += min(kv, (before + got) << sh) - min(kv, before << sh);
+            lost += add - ok;
+            p.q_start[s] = r0;
+            p.kv_len[s] = sat32(kv);
+        }
+        __syncthreads();
+        for (uint64_t i = tid; i < pages; i += PLAN_T) {
+            const uint32_t q = owner(l_page, nb, i);
+            const uint64_t at = page0 + i;
+            p.table[(uint64_t)(base + q) * p.table_stride + l_before[q] + (i - l_page[q])] =
+                at < p.n_free ? p.free_pages[at] : FLH_KV_NONE;
+        }
+        if (rows_too) {
+            const uint32_t e = (uint32_t)min(row0, (uint64_t)p.max_tok);
+            for (uint32_t i = l_row[0] + tid; i < e; i += PLAN_T) {
+                const uint32_t q = owner(l_row, nb, i);
+                const uint64_t at = (uint64_t)l_held[q] + (i - l_row[q]), pg = at >> sh;
+                uint32_t g = FLH_KV_NONE;
+                if (pg < l_before[q]) g = p.table[(uint64_t)(base + q) * p.table_stride + pg];
+                else if (pg < p.table_stride) {
+                    const uint64_t f = page0 + l_page[q] + (pg - l_before[q]);
+                    if (f < p.n_free) g = p.free_pages[f];
+                }
+                p.slot[i] = slot_of(g, (uint32_t)at, sh);
+                if (p.pos) p.pos[i] = (int32_t)(uint32_t)at;
+            }
+        }
+        page0 += pages;
+        __syncthreads();                                          // the tables in LDS are the next batch's
+    }
+    const uint32_t rows = (uint32_t)min(row0, (uint64_t)p.max_tok);
+    if (rows_too)
+        for (uint32_t i = rows + tid; i < p.max_tok; i += PLAN_T) {
+            p.slot[i] = FLH_KV_NONE;
+            if (p.pos) p.pos[i] = 0;
+        }
+    uint64_t all;
+    (void)scan_wg(lost, ws, &all);
+    if (tid == 0) {
+        p.q_start[p.n_seq] = rows;
+        *p.taken = sat32(page0);
+        if (p.info) {
+            p.info[0] = rows;
+            p.info[1] = sat32(all);
+        }
+    }
+}
+
+// Slots and positions of many rows, a thread each, from the finished table.
+__global__ __launch_bounds__(256) void k_kv_slots(flh_kv_plan_p p, uint32_t sh) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.max_tok) return;
+    if (i >= p.q_start[p.n_seq]) {
+        p.slot[i] = FLH_KV_NONE;
+        if (p.pos) p.pos[i] = 0;
+        return;
+    }
+    const uint32_t s = owner(p.q_start, p.n_seq, i);
+    const uint32_t r0 = p.q_start[s], n = p.q_start[s + 1] - r0;
+    const uint64_t at = (uint64_t)(p.kv_len[s] - n) + (i - r0), pg = at >> sh;
+    const uint32_t g = pg < p.table_stride ? p.table[(uint64_t)s * p.table_stride + pg] : FLH_KV_NONE;
+    p.slot[i] = slot_of(g, (uint32_t)at, sh);
+    if (p.pos) p.pos[i] = (int32_t)(uint32_t)at;
+}
+
+int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s) {
+    constexpr uint32_t PLAN_ROWS = 16384;
+    const uint32_t sh = (uint32_t)__builtin_ctz(p.page_size);
+    const bool one = p.max_tok <= PLAN_ROWS;
+    hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(PLAN_T), 0, s, p, sh, one ? 1 : 0);
+    if (int rc = hip_check(hipGetLastError(), "k_kv_plan launch")) return rc;
+    if (one) return FLH_OK;
+    hipLaunchKernelGGL(k_kv_slots, dim3((uint32_t)(((uint64_t)p.max_tok + 255) / 256)), dim3(256), 0, s, p, sh);
+    return hip_check(hipGetLastError(), "k_kv_slots launch");
+}
+
+// ------------------------------------------------------------------- rope --
+// cos and sin of pair `t` at its position: turn = pos * frac mod 2^64 is the
+// angle as a fraction of a turn, exact to 2^-33 of a turn for every 32-bit
+// position (frac is rounded once, to 2^-65).  The nearest quarter turn comes off in
+// integers, so the rest, at most an eighth of a turn, keeps 24 bits as a float.
+__device__ __forceinline__ void rope_cs(const RopePair & t, const int32_t * pos, uint32_t pos_stride, uint32_t tok,
+                                        float & c, float & s) {
+    const uint64_t turn = (uint64_t)(int64_t)pos[(size_t)t.axis * pos_stride + tok] * t.frac;
+    const uint32_t hi = (uint32_t)(turn >> 32), q = (hi + 0x20000000u) >> 30;
+    const float r = (float)(int32_t)(hi - (q << 30)) * 0x1p-31f;  // half turns
+    float s0, c0;
+    sincospif(r, &s0, &c0);
+    const float a = q & 1 ? s0 : c0, b = q & 1 ? c0 : s0;
+    c = (q + 1) & 2 ? -a : a;
+    s = q & 2 ? -b : b;
+}
+
+template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+
+// One thread per pair or element: token blockIdx.x, the heads of q, k and v one
+// after the other.
+template <typename AT, typename CT>
+__global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
+    const uint32_t tok = blockIdx.x, nk = a.kc ? a.n_kv : 0, P = a.rot ? a.n_rot / 2 : 0;
+    const uint32_t slot = nk ? a.slot[tok] : 0;
+    const bool live = nk && slot < a.n_slot;
+    const uint64_t page = slot >> a.sh, off = slot & ((1u << a.sh) - 1u);
+    const uint32_t rest = a.d - 2 * P, per = P + rest;            // units of a head: pairs, then single elements
+    for (uint32_t u = threadIdx.x; u < per * (a.n_head + nk); u += 256) {
+        const uint32_t h = u / per, e = u % per;
+        const bool isq = h < a.n_head;
+        if (!isq && !live) continue;
+        const AT * x = isq ? (const AT *)a.q + tok * a.q_tok + h * a.q_head : (const AT *)a.k + tok * a.k_tok + (h - a.n_head) * a.k_head;
+        AT * yq = (AT *)a.qo + tok * a.qo_tok + h * a.qo_head;
+        CT * yk = (CT *)a.kc + page * a.kc_page + off * a.kc_tok + (h - a.n_head) * a.kc_head;
+        if (e < P) {
+            const uint32_t i = a.first + (a.halves ? e : 2 * e), j = i + (a.halves ? P : 1);
+            float c, s;
+            rope_cs(a.rot[e], a.pos, a.pos_stride, tok, c, s);
+            const float v = to_f(x[i]), w = to_f(x[j]);
+            const float ya = v * c - w * s, yb = v * s + w * c;
+            if (isq) { yq[i] = (AT)ya; yq[j] = (AT)yb; }
+            else { yk[i] = (CT)ya; yk[j] = (CT)yb; }
+        } else {
+            const uint32_t k = e - P, i = k < a.first || !P ? k : k + 2 * P;
+            if (isq) yq[i] = x[i];
+            else yk[i] = (CT)to_f(x[i]);
+        }
+    }
+    if (!live) return;
+    for (uint32_t u = threadIdx.x; u < nk * a.dv; u += 256) {
+        const uint32_t h = u / a.dv, i = u % a.dv;
+        ((CT *)a.vc)[page * a.vc_page + off * a.vc_tok + h * a.vc_head + i] =
+            (CT)to_f(((const AT *)a.v)[tok * a.v_tok + h * a.v_head + i]);
+    }
+}
+
+template <typename AT>
+static int rope_go(const RopeArgs & a, uint32_t cdt, hipStream_t s) {
+    if (cdt == FLH_DT_BF16) hipLaunchKernelGGL((k_rope<AT, __bf16>), dim3(a.n_tok), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rope<AT, _Float16>), dim3(a.n_tok), dim3(256), 0, s, a);
+    return hip_check(hipGetLastError(), "k_rope launch");
+}
+int launch_rope(const RopeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s) {
+    if (dtype == FLH_DT_F32) return rope_go<float>(a, cache_dtype, s);
+    if (dtype == FLH_DT_F16) return rope_go<_Float16>(a, cache_dtype, s);
+    return rope_go<__bf16>(a, cache_dtype, s);
+}
+
+}  // namespace flh

@@ -357,6 +357,131 @@ int flh_wmerge(const float * parts, const float * gates, const float * add1,
                uint32_t n, uint32_t n_full, uint32_t ncol, uint32_t pstride,
                uint32_t ystride, void * stream);
 
+/* ------------------------------------------- paged cache and attention -- */
+/* What a decoder layer runs between its QKV dots and its O dot: pages for
+ * the tokens that requests add, rotary positions, the key/value cache, and
+ * attention over it.  The reference has a flat fp32 cache and per-head tasks
+ * for this (ROPE_DS2, KV_APPEND, ATTN_HEAD, src/runtime/decode_params.h:48-55,
+ * 118-160, 183-232; CPU only); these entry points are this backend's own form for many
+ * requests at once, so flh_exec_tasks goes on refusing those task kinds.
+ * Lengths, tables and slots are read on the device, so a captured step can be
+ * replayed while requests grow. */
+
+/* Element types of activations and of the cache. */
+enum { FLH_DT_F32 = 0, FLH_DT_F16 = 1, FLH_DT_BF16 = 2 };
+
+/* "no page" / "no slot" */
+#define FLH_KV_NONE 0xFFFFFFFFu
+
+/* A paged key/value cache of one layer: n_pages pages of page_size tokens (a
+ * power of two up to 65536).  Token t of a page, kv head h: d_k keys at
+ * k + page*k_page + t*k_tok + h*k_head and d_v values at v + ... (strides in
+ * elements, so heads may lie inside tokens or tokens inside heads, and k and v
+ * may share an allocation).  dtype is F16 or BF16; d_k and d_v are multiples of
+ * 8 up to 256; k and v are 16-byte aligned, strides multiples of 8.  A token's
+ * slot is page*page_size + t; n_pages*page_size < 2^32 - 1. */
+typedef struct flh_kv_cache {
+    void * k, * v;
+    uint32_t dtype, n_pages, page_size, n_kv_head, d_k, d_v;
+    uint64_t k_page, k_tok, k_head, v_page, v_tok, v_head;
+} flh_kv_cache;
+
+/* Block tables and slot maps from request lengths.  Request s holds held[s]
+ * tokens and adds add[s]; its row of table (table_stride entries) holds the
+ * pages of the held ones.  Rows (new tokens) are packed: request s has rows
+ * q_start[s] .. q_start[s+1], cut off at max_tok, and kv_len[s] = held[s] +
+ * its rows.  Pages that a request now reaches are taken off free_pages
+ * (n_free entries, in order, requests in order), from entry *taken_in on (NULL:
+ * 0), and written into the table; *taken = *taken_in + the pages needed; other
+ * table entries stay as they are.  slot[r] and pos[r] of row r: its cache slot
+ * and its position in its request; behind the last row, up to max_tok, they are
+ * FLH_KV_NONE and 0 (a captured step of max_tok rows may have fewer).
+ * A row has slot FLH_KV_NONE when free_pages ran out (its table
+ * entry is FLH_KV_NONE, and *taken > n_free), when its page lies behind
+ * the table's row, or when its table entry is no page.  info[0]: rows;
+ * info[1]: new tokens without a slot (0: all is well; those cut off at max_tok
+ * count).  page_size: a power of two up to 65536.  pos and info may be NULL.
+ * kv_len may be held and taken may be taken_in (a captured step then advances
+ * its requests by itself); nothing else may overlap.  free_pages and table
+ * hold the page numbers of a flh_kv_cache. */
+typedef struct flh_kv_plan_p {
+    const uint32_t * held, * add, * free_pages, * taken_in;
+    uint32_t * taken, * table, * q_start, * kv_len, * slot;
+    int32_t * pos;
+    uint32_t * info;
+    uint32_t n_seq, page_size, n_free, table_stride, max_tok;
+} flh_kv_plan_p;
+int flh_kv_plan(const flh_kv_plan_p * p, void * stream);
+
+/* Rotary frequencies of the elements first .. first + n_rot - 1 of a head.
+ * Pair i (of n_rot / 2) is elements (i, i + n_rot/2) of that range with
+ * FLH_ROPE_HALVES, (2i, 2i + 1) with FLH_ROPE_PAIRS; its angle is the token's
+ * position on axis axis[i] (NULL: 0; axis[i] < n_axis <= 8) times freq[i]
+ * (host doubles, radians per position; NULL: base^(-2i/n_rot)).  Several axes are
+ * the time, height and width of image and video tokens.  n_rot: even, 2..1024.
+ * Angles are kept as 64-bit fractions of a turn, so positions up to
+ * 2^31 - 1 (and negative ones) lose nothing.  The table lives on the device of
+ * flh_init; create waits for its upload. */
+enum { FLH_ROPE_HALVES = 0, FLH_ROPE_PAIRS = 1 };
+typedef struct flh_rope_table flh_rope_table;
+int flh_rope_table_create(uint32_t n_rot, uint32_t first, int layout, double base, const double * freq,
+                          uint32_t n_axis, const uint8_t * axis, flh_rope_table ** out);
+int flh_rope_table_destroy(flh_rope_table * r);
+
+/* (a, b) -> (a cos - b sin, a sin + b cos) over the pairs of n_head heads of
+ * n_tok tokens, x -> y, d elements a head (first + n_rot <= d; the others are
+ * copied); strides in elements.  pos[axis*pos_stride + token].  y may be x with
+ * the same strides, else the two must not overlap.  The arithmetic is fp32 in
+ * every dtype. */
+int flh_rope(const flh_rope_table * r, uint32_t dtype, const void * x, uint64_t x_tok, uint64_t x_head, void * y,
+             uint64_t y_tok, uint64_t y_head, uint32_t n_tok, uint32_t n_head, uint32_t d, const int32_t * pos,
+             uint32_t pos_stride, void * stream);
+
+/* The same for the queries of n_tok tokens (q -> q_out; n_head = 0: none) and
+ * their keys, and the keys and values into the cache at slot[token], rounded
+ * to its dtype; one launch.  Tokens whose slot is not in the cache (FLH_KV_NONE)
+ * write nothing there.  Slots of one call must differ.  r = NULL: nothing is
+ * rotated (pos is not read).  q, k and v may be columns of one product's rows
+ * (any element strides); q_out as y of flh_rope; the cache must not overlap
+ * them. */
+typedef struct flh_rope_kv_p {
+    const void * q; void * q_out; const void * k; const void * v;
+    const int32_t * pos; const uint32_t * slot;
+    uint64_t q_tok, q_head, qo_tok, qo_head, k_tok, k_head, v_tok, v_head;
+    uint32_t dtype, n_tok, n_head, pos_stride;
+} flh_rope_kv_p;
+int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, const flh_rope_kv_p * p, void * stream);
+
+/* Attention of new tokens over the paged cache.  Request s has query rows
+ * q_start[s] .. q_start[s+1] (cut off at n_tok; rows of no request are left as
+ * they are in out) and keys 0 .. kv_len[s] - 1, key j at token j % page_size of page
+ * table[s*table_stride + j / page_size].  causal: the rows are the last
+ * tokens, row i of n at position p = kv_len - n + i, and see the keys
+ * j <= p, with window > 0 also j > p - window; else every row sees every
+ * key (an encoder's states as the cache) and window must be 0.  Query head h
+ * reads kv head h / (n_head / n_kv_head).
+ *   out[row][head] = sum_j softmax_j(scale q.k_j) v_j   over the keys seen,
+ * 0 for a row that sees none; keys not seen have no part in it, whatever the cache
+ * holds there.  Keys whose table entry is no page of the cache, or lies
+ * behind the table's row, are not seen.  dtype of q and out: F32 over either
+ * cache (products as accurate as fp32 ones), or the cache's own.  Sums, maxima
+ * and the softmax are fp32.  scale: finite, >= 0.  q and out: any element strides,
+ * aligned to an element; out must not overlap q.  max_q: the most rows of a
+ * request that the caller expects (it chooses the kernel, the results hold for
+ * any).  ws: flh_paged_attn_ws_bytes of the same arguments (pointers and lengths
+ * are not looked at), 16-byte aligned; its contents need not be kept or
+ * cleared, but calls that may run at the same time need one each. */
+typedef struct flh_attn_p {
+    const void * q; void * out;
+    const uint32_t * q_start, * kv_len, * table;
+    void * ws; size_t ws_bytes;
+    uint64_t q_tok, q_head, o_tok, o_head;
+    uint32_t dtype, n_head, n_seq, n_tok, max_q, table_stride, causal, window;
+    float scale;
+} flh_attn_p;
+size_t flh_paged_attn_ws_bytes(const flh_kv_cache * cache, const flh_attn_p * p);
+int flh_paged_attn(const flh_kv_cache * cache, const flh_attn_p * p, void * stream);
+
 /* ---------------------------------------------------------------- GGUF -- */
 /* GGUF v2/v3 reader (replaces fastllm::Gguf, src/model/gguf.h:28-79,
  * src/model/gguf.cpp:133-303).  The file is mmapped read-only; metadata and

@@ -217,7 +217,8 @@ struct AttnArgs {
     const uint32_t * q_start; const uint32_t * kv_len; const uint32_t * table;
     void * ws;
     uint64_t q_tok, q_head, o_tok, o_head, k_page, k_tok, k_head, v_page, v_tok, v_head;
-    uint32_t n_pages, sh, n_kv, dk, dv, group, n_seq, n_tok, max_q, table_stride, causal, window;
+    uint32_t n_pages, sh, n_kv, dk, dv, group, n_seq, n_tok, max_q, table_stride, causal, window, pmask;
+    uint32_t grid, min_units;           // the launch's (flh_attn.h)
     float scale;
 };
 int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s);

@@ -78,11 +78,14 @@ int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
         return set_error(FLH_ERR_UNSUPPORTED, "attention: q must be F32 or of the cache's dtype");
     if (p->n_head == 0 || p->n_head % c->n_kv_head) return set_error(FLH_ERR_ARG, "attention: n_head must be a multiple of n_kv_head");
     const uint32_t group = p->n_head / c->n_kv_head;
-    if ((uint64_t)p->n_tok * group >= (1ull << 31)) return set_error(FLH_ERR_UNSUPPORTED, "attention: n_tok * (n_head / n_kv_head) must be below 2^31");
+    if ((uint64_t)p->n_tok * group >= (1ull << 30)) return set_error(FLH_ERR_UNSUPPORTED, "attention: n_tok * (n_head / n_kv_head) must be below 2^30");
     if (!(p->scale >= 0.f) || !isfinite(p->scale)) return set_error(FLH_ERR_ARG, "attention: scale must be finite and >= 0");
     if (p->window && !p->causal) return set_error(FLH_ERR_ARG, "attention: a window needs causal");
-    if ((uint64_t)p->table_stride * c->page_size > (1ull << 31))
-        return set_error(FLH_ERR_UNSUPPORTED, "attention: table_stride * page_size must be at most 2^31");
+    const uint64_t keys = (uint64_t)p->table_stride * c->page_size;
+    if (keys > (1ull << 30)) return set_error(FLH_ERR_UNSUPPORTED, "attention: table_stride * page_size must be at most 2^30");
+    // units of work are counted in 32 bits (strips of 16 rows or more, tiles of 64 keys or more)
+    if ((double)c->n_kv_head * ((double)p->n_tok * group / 16 + 2.0 * p->n_seq) * ((double)keys / 64 + 2) >= 4.0e9)
+        return set_error(FLH_ERR_UNSUPPORTED, "attention: too much work for one call (rows times table length)");
     a = AttnArgs{};
     a.q = p->q; a.out = p->out; a.q_start = p->q_start; a.kv_len = p->kv_len; a.table = p->table; a.ws = p->ws;
     a.k = c->k; a.v = c->v;
@@ -92,7 +95,7 @@ int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
     a.n_pages = c->n_pages; a.sh = (uint32_t)__builtin_ctz(c->page_size); a.n_kv = c->n_kv_head;
     a.dk = c->d_k; a.dv = c->d_v; a.group = group;
     a.n_seq = p->n_seq; a.n_tok = p->n_tok; a.max_q = p->max_q; a.table_stride = p->table_stride;
-    a.causal = p->causal != 0; a.window = p->window; a.scale = p->scale;
+    a.causal = p->causal != 0; a.window = p->window; a.pmask = c->page_size - 1; a.scale = p->scale;
     return FLH_OK;
 }
 

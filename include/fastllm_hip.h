@@ -463,7 +463,8 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, con
  *   out[row][head] = sum_j softmax_j(scale q.k_j) v_j   over the keys seen,
  * 0 for a row that sees none; keys not seen have no part in it, whatever the cache
  * holds there.  Keys whose table entry is no page of the cache, or lies
- * behind the table's row, are not seen.  dtype of q and out: F32 over either
+ * behind the table's row, are not seen (kv_len and a table's row: at most 2^30
+ * tokens).  dtype of q and out: F32 over either
  * cache (products as accurate as fp32 ones), or the cache's own.  Sums, maxima
  * and the softmax are fp32.  scale: finite, >= 0.  q and out: any element strides,
  * aligned to an element; out must not overlap q.  max_q: the most rows of a

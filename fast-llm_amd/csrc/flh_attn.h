@@ -200,10 +200,10 @@ __device__ __forceinline__ uint32_t attn_border(uint32_t w, uint32_t U, uint32_t
 // them before every LDS read.  Whoever reads the data waits itself (wait_vm); the
 // compiler's own loads beside them are waited for too long at worst.  (m0, the
 // LDS base, is set each time; nothing else in these kernels uses it.)
-__device__ __forceinline__ void dma16(const void * src, uint32_t lds) {
+__device__ __forceinline__ void dma16(uint64_t src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
-__device__ __forceinline__ void dma4(const void * src, uint32_t lds) {
+__device__ __forceinline__ void dma4(uint64_t src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_vm() {
@@ -214,12 +214,46 @@ __device__ __forceinline__ uint32_t lds_at(const void * p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
 
+// A value that the compiler takes for a new one: what is computed from it is
+// computed where it stands (a few instructions a tile), not kept in registers
+// around the loop over the tiles.
+__device__ __forceinline__ uint32_t fresh(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// base + page * stride + tok * tok_stride, in bytes (strides below 2^32)
+__device__ __forceinline__ uint64_t row_at(uint64_t base, uint32_t page, uint32_t stride, uint32_t tok, uint32_t tok_stride) {
+    return base + (uint64_t)page * stride + (uint64_t)tok * tok_stride;
+}
+
 // what a DMA reads in the place of keys that are not there
 static __device__ __attribute__((aligned(16))) uint32_t g_attn_zero[4];
 
-// 16-byte pieces of a row lie in LDS at piece ^ swz(row), so that a column of
-// pieces (what a matrix-core operand reads of 16 or 32 rows) spreads over the banks
-template <int D> __device__ __forceinline__ uint32_t swz(uint32_t row) { return row & (D % 128 == 0 ? 15u : 7u); }
+// A 16-byte piece of a row lies in LDS at piece ^ swz(row), so that what a
+// matrix-core operand reads at once spreads over the 64 banks: for K one
+// piece of 16 rows, for V (transposing reads) two or four pieces of 4 and 4 rows.
+template <int D> __device__ __forceinline__ uint32_t swz_k(uint32_t row) { return D % 128 == 0 ? row & 15 : (row >> 1) & 7; }
+template <int D> __device__ __forceinline__ uint32_t swz_v(uint32_t row) {
+    static_assert(D == 64 || D % 128 == 0, "rows of 128 or n * 256 bytes");
+    return D == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
+// Address of piece `at` (a constant whose low bits, the lane's, are 0) of the
+// row and lane that `a` = row address + (lane's piece ^ swz) * 16 stands for: the
+// swizzle works inside groups of 16 (8) pieces, to which rows are aligned.
+template <int D> __device__ __forceinline__ uint32_t piece(uint32_t a, uint32_t at) {
+    constexpr uint32_t G = D % 128 == 0 ? 16 : 8;
+    return (a ^ (at % G * 16)) + at / G * (G * 16);
+}
+#define FLH_LDS(T, at) ((const __attribute__((address_space(3))) T *)(uintptr_t)(uint32_t)(at))
+template <typename T> __device__ __forceinline__ typename VecOf<T>::v8 ld_row(uint32_t at) {
+    return *FLH_LDS(typename VecOf<T>::v8, at);
+}
+// Four values of one column each, of four rows (keys): the 16 lanes of a group
+// give the addresses of 4 rows x 4 pieces of 8 bytes, lane i gets column i.
+template <typename T> __device__ __forceinline__ typename VecOf<T>::v4 ld_tr(uint32_t at) {
+    return __builtin_bit_cast(typename VecOf<T>::v4,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)at));
+}
 
 template <typename T> __device__ __forceinline__ float load_f(const T * p) {
     T v;
@@ -233,31 +267,22 @@ template <typename AT> __device__ __forceinline__ void store4(AT * p, float a, f
 }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
-// Values that are no numbers.  0 * inf is NaN, so a weight of 0 (a key that a
-// row does not see, or the vanished low term of a split weight) would carry an
-// infinite value into the row.  The kernels do not look at the values; a piece
-// whose sums come out not finite is done once more with this: the finite
-// values go through the product, and for the others (1 where the class holds, 0
-// elsewhere) a product with the row's visible keys (1 or 0) tells whether the
-// row gets one.
-template <typename T> struct ValueClass {
-    u16x8 fin, pos, neg, nan;
-    __device__ explicit ValueClass(typename VecOf<T>::v8 v) {
-        const u16x8 b = __builtin_bit_cast(u16x8, v);
-        const uint16_t E = __is_same(T, _Float16) ? 0x7C00 : 0x7F80, one = __is_same(T, _Float16) ? 0x3C00 : 0x3F80;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint16_t m = b[i] & 0x7FFF;
-            fin[i] = m < E ? b[i] : (uint16_t)0;
-            pos[i] = b[i] == E ? one : (uint16_t)0;
-            neg[i] = m == E && b[i] != E ? one : (uint16_t)0;
-            nan[i] = m > E ? one : (uint16_t)0;
-        }
-    }
-};
-__device__ __forceinline__ float odd_value(float pos, float neg, float nan) {
-    const float p = pos > 0.f ? INFINITY : 0.f, q = neg > 0.f ? -INFINITY : 0.f;
-    return nan > 0.f ? NAN : p + q;
+// x where bit `at` of m is set, else -infinity
+__device__ __forceinline__ float seen(float x, uint32_t m, uint32_t at) {
+    const uint32_t k = (uint32_t)__builtin_amdgcn_sbfe((int)m, at, 1);
+    return __uint_as_float((k & __float_as_uint(x)) | (~k & 0xFF800000u));
+}
+// bits [lo, hi) of 64 (any lo, hi)
+__device__ __forceinline__ uint64_t bits_of(int32_t lo, int32_t hi) {
+    const uint64_t a = hi >= 64 ? ~0ull : hi <= 0 ? 0ull : (1ull << hi) - 1;
+    return lo <= 0 ? a : lo >= 64 ? 0ull : a & (~0ull << lo);
+}
+// 8 elements as they are in memory, at any element alignment
+template <typename AT> struct Eight { AT v[8]; };
+template <typename AT> __device__ __forceinline__ Eight<AT> load8(const AT * p) {
+    Eight<AT> x;
+    __builtin_memcpy(&x, p, sizeof x);
+    return x;
 }
 
 // The plan of a launch, from host-known arguments.
@@ -275,53 +300,122 @@ AttnPlan attn_pre_plan(const AttnArgs & a);
 int launch_attn_dec(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 
-// Sums of the workgroups that share an item, added up: block (w, y) looks whether
-// the border between workgroups w - 1 and w is the first one inside an item; a
-// wave takes every fourth row of the blocks' share and adds the parts in order.
-// Parts: [2 * workgroup + (1: the item begins in it)][M][DV] sums, then [M] maxima,
-// [M] weights.
-template <typename AT, int M, int KT, int DV>
+// One row by one wave, a key a lane, in fp32: for items whose sums are not
+// finite.  0 * inf is NaN, so in a matrix product a key that a row does not see
+// (weight 0), or the vanished low term of a split weight, carries an infinite or NaN
+// value into the row.  Here only the keys seen are looked at.
+template <typename AT, typename T, int M> __device__ __forceinline__ void attn_row(const AttnArgs & a, const AttnItem & it, uint32_t r) {
+    const uint32_t lane = threadIdx.x & 63, row = it.strip * M + r, tok = row / a.group, head = it.kvh * a.group + row % a.group;
+    const AT * q = (const AT *)a.q + (it.r0 + tok) * a.q_tok + head * a.q_head;
+    const int32_t hi = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
+    const int32_t lo = a.window ? max(0, it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30)) : 0;
+    const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
+    const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int32_t j0 = lo; j0 < hi; j0 += 64) {
+        const int32_t j = j0 + (int32_t)lane;
+        const uint32_t pg = j < hi ? tab[(uint32_t)j >> a.sh] : FLH_KV_NONE;
+        const bool in = pg < a.n_pages;
+        float t = -INFINITY;
+        if (in) {
+            const T * k = (const T *)(uintptr_t)row_at(kb, pg, a.k_page, (uint32_t)j & a.pmask, a.k_tok);
+            t = 0.f;
+            for (uint32_t i = 0; i < a.dk; i += 8) {
+                const Eight<T> x = load8(k + i);
+                for (int e = 0; e < 8; ++e) t = fmaf((float)q[i + e], (float)x.v[e], t);
+            }
+            t *= a.scale;
+        }
+        float top = t;
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn, al = expf(m - base), p = expf(t - base);
+        float sum = p;
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        l = fmaf(l, al, sum);
+        m = mn;
+        for (int c = 0; c < 4; ++c) o[c] *= al;
+        uint64_t left = __ballot(in);
+        while (left) {
+            const int k = __builtin_ctzll(left);
+            left &= left - 1;
+            const float w = __shfl(p, k);
+            const T * v = (const T *)(uintptr_t)row_at(vb, __shfl(pg, k), a.v_page, (uint32_t)(j0 + k) & a.pmask, a.v_tok);
+            for (uint32_t c = 0; c < 4; ++c)
+                if (64 * c + lane < a.dv) o[c] = fmaf(w, (float)v[64 * c + lane], o[c]);
+        }
+    }
+    AT * out = (AT *)a.out + (it.r0 + tok) * a.o_tok + head * a.o_head;
+    for (uint32_t c = 0; c < 4; ++c)
+        if (64 * c + lane < a.dv) out[64 * c + lane] = (AT)(l == 0.f ? 0.f : o[c] / l);
+}
+
+// What a launch leaves in the workspace: the parts of items that lie across a
+// border, [2 * workgroup + (1: the item begins in it)][M][DV] sums, then [M]
+// maxima, [M] weights; then a flag for each workgroup: a sum of it is not finite.
+template <int M, int DV> __device__ __forceinline__ float * attn_part(const AttnArgs & a, uint32_t w, bool begins) {
+    return (float *)a.ws + (size_t)M * (DV + 2) * (2 * w + (begins ? 1 : 0));
+}
+template <int M, int DV> __device__ __forceinline__ uint32_t * attn_flags(const AttnArgs & a) {
+    return (uint32_t *)((float *)a.ws + (size_t)M * (DV + 2) * 2 * a.grid);
+}
+inline size_t attn_ws(uint32_t grid, uint32_t m, uint32_t dv) { return (size_t)grid * (2 * m * (dv + 2) + 1) * 4; }
+
+// Behind the main kernel.  Workgroups (w, y): if the border between main
+// workgroups w - 1 and w is the first one inside an item, the item's parts are
+// added up in order, a wave a row.  Rows of items with sums that are not
+// finite are done by attn_row instead.
+template <typename AT, typename T, int M, int KT, int DV>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
-    const uint32_t lane = threadIdx.x & 63, w = blockIdx.x + 1;
+    const uint32_t lane = threadIdx.x & 63, w = blockIdx.x, r0 = blockIdx.y * 4 + (threadIdx.x >> 6), rs = 4 * gridDim.y;
     AttnWalk<M, KT> walk(a, lane);
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     if (w >= Ge) return;
-    const uint32_t u = attn_border(w, U, Ge);
+    const uint32_t * flags = attn_flags<M, DV>(a);
+    const uint32_t u = attn_border(w, U, Ge), end = attn_border(w + 1, U, Ge);
     AttnItem it;
-    walk.find(u, it);
-    if (u == it.u0 || attn_border(w - 1, U, Ge) > it.u0) return;
-    uint32_t last = w;                                                // the last workgroup with a part
-    while (last + 1 < Ge && attn_border(last + 1, U, Ge) < it.u0 + it.tiles) ++last;
-    const uint32_t parts = last - w + 2, rows = min((uint32_t)M, it.n * a.group - it.strip * M);
-    constexpr size_t PART = (size_t)M * (DV + 2);
-    const float * ws = (const float *)a.ws;
-    auto part = [&](uint32_t i) { return ws + PART * (i == 0 ? 2 * (w - 1) + 1 : 2 * (w - 1 + i)); };
-    constexpr int V = DV / 64;                                        // values a lane
-    for (uint32_t r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += 4 * gridDim.y) {
-        float top = -INFINITY;
-        for (uint32_t i = lane; i < parts; i += 64) top = fmaxf(top, part(i)[(size_t)M * DV + r]);
+    if (w) {
+        walk.find(u, it);
+        if (u != it.u0 && attn_border(w - 1, U, Ge) <= it.u0) {
+            uint32_t last = w, odd = flags[w - 1] | flags[w];         // the last workgroup with a part
+            while (last + 1 < Ge && attn_border(last + 1, U, Ge) < it.u0 + it.tiles) odd |= flags[++last];
+            const uint32_t parts = last - w + 2, rows = min((uint32_t)M, it.n * a.group - it.strip * M);
+            auto part = [&](uint32_t i) { return (const float *)(i == 0 ? attn_part<M, DV>(a, w - 1, true) : attn_part<M, DV>(a, w - 1 + i, false)); };
+            constexpr int V = DV / 64;                                // values a lane
+            for (uint32_t r = r0; r < rows; r += rs) {
+                if (odd) {
+                    attn_row<AT, T, M>(a, it, r);
+                    continue;
+                }
+                float top = -INFINITY;
+                for (uint32_t i = lane; i < parts; i += 64) top = fmaxf(top, part(i)[(size_t)M * DV + r]);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, xor_lane(top, d, lane));
-        const float base = top == -INFINITY ? 0.f : top;
-        float l = 0.f, o[V];
+                for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, xor_lane(top, d, lane));
+                const float base = top == -INFINITY ? 0.f : top;
+                float l = 0.f, o[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = 0.f;
+                for (int k = 0; k < V; ++k) o[k] = 0.f;
 #pragma unroll 4
-        for (uint32_t i = 0; i < parts; ++i) {
-            const float * p = part(i);
-            const float f = __builtin_amdgcn_exp2f(p[(size_t)M * DV + r] - base);
-            l = fmaf(f, p[(size_t)M * (DV + 1) + r], l);
+                for (uint32_t i = 0; i < parts; ++i) {
+                    const float * p = part(i);
+                    const float f = __builtin_amdgcn_exp2f(p[(size_t)M * DV + r] - base);
+                    l = fmaf(f, p[(size_t)M * (DV + 1) + r], l);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float v = p[(size_t)r * DV + lane * V + k];
-                o[k] = f == 0.f ? o[k] : fmaf(f, v, o[k]);            // (a part that sees nothing)
+                    for (int k = 0; k < V; ++k) o[k] = fmaf(f, p[(size_t)r * DV + lane * V + k], o[k]);
+                }
+                const uint32_t row = it.strip * M + r, tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
+                AT * out = (AT *)a.out + tok * a.o_tok + head * a.o_head;
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (lane * V + k < a.dv) out[lane * V + k] = (AT)(l == 0.f ? 0.f : o[k] / l);
             }
         }
-        const uint32_t row = it.strip * M + r, tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
-        AT * out = (AT *)a.out + tok * a.o_tok + head * a.o_head;
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-            if (lane * V + k < a.dv) out[lane * V + k] = (AT)(l == 0.f ? 0.f : o[k] / l);
+    }
+    if (!flags[w]) return;
+    for (uint32_t x = u; x < end;) {                                  // items of workgroup w alone
+        walk.find(x, it);
+        if (it.u0 >= u && it.u0 + it.tiles <= end)
+            for (uint32_t r = r0; r < min((uint32_t)M, it.n * a.group - it.strip * M); r += rs) attn_row<AT, T, M>(a, it, r);
+        x = it.u0 + it.tiles;
     }
 }
 

@@ -38,11 +38,17 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     static_assert((2 * W * M + W) * 4 <= 1088, "shared tail");
     static_assert((size_t)M * DV * 4 <= (size_t)NST * P::STAGE, "a wave's sums lie in its stages");
 
+    // the lane's addresses in a stage: K rows l16 (+ 16 kt), pieces q4 (+ 4 d); V
+    // rows 4 q4 + l16 / 4 (+ 16 kt), pieces of 16 columns (+ 2 d)
+    const uint32_t k_lane = l16 * (DK * 2) + (q4 ^ swz_k<DK>(l16)) * 16;
+    const uint32_t v_row = 4 * q4 + (l16 >> 2);
+    const uint32_t v_lane = 32 * DK * 2 + v_row * (DV * 2) + (((l16 >> 1) & 1) ^ swz_v<DV>(v_row)) * 16 + (l16 & 1) * 8;
     AttnWalk<M, KT> walk(a, lane);
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units), w = blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
     const uint32_t end = attn_border(w + 1, U, Ge);
+    bool odd = false;                                                 // a sum is not finite
     while (u < end) {
         AttnItem it;
         walk.find(u, it);
@@ -66,55 +72,49 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             rhi[mt] = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
             rlo[mt] = a.window ? it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30) : 0;
             c[mt] = a.scale == 0.f ? 1.f : a.scale * 1.4426950408889634f;
-            if constexpr (NS == 1) {
+            Eight<AT> x[DK / 32];
 #pragma unroll
-                for (int s = 0; s < DK / 32; ++s) {
-                    const uint32_t e = 32 * s + 8 * q4;
-                    v8 x = {};
-                    if (real && e < a.dk) __builtin_memcpy(&x, q + e, 16);
-                    qf[0][mt][s] = x;
-                }
-            } else {
-                float x[DK / 32][8], top = 0.f;
+            for (int s = 0; s < DK / 32; ++s) {
 #pragma unroll
-                for (int s = 0; s < DK / 32; ++s) {
-                    const uint32_t e = 32 * s + 8 * q4;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        x[s][j] = real && e < a.dk ? load_f(q + e + j) : 0.f;
-                        top = fmaxf(top, fabsf(x[s][j]));
-                    }
-                }
-                if constexpr (NS == 2) {
-                    // f16 terms: the row's largest element to [2^13, 2^14), and back in c
-                    top = fmaxf(top, xor_lane(top, 16, lane));
-                    top = fmaxf(top, xor_lane(top, 32, lane));
-                    const int ex = top > 0.f && finite(top) ? 14 - (ilogbf(top) + 1) : 0;
-                    c[mt] = fmaxf(ldexpf(c[mt], -ex), 0x1p-126f);     // (c * -inf below)
-#pragma unroll
-                    for (int s = 0; s < DK / 32; ++s)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[s][j] = ldexpf(x[s][j], ex);
-                }
+                for (int j = 0; j < 8; ++j) x[s].v[j] = (AT)0.f;
+                if (real && 32 * s + 8 * q4 < a.dk) x[s] = load8(q + 32 * s + 8 * q4);
+            }
+            int ex = 0;
+            if constexpr (NS == 2) {
+                // f16 terms: the row's largest element to [2^13, 2^14), and back in c
+                float top = 0.f;
 #pragma unroll
                 for (int s = 0; s < DK / 32; ++s)
 #pragma unroll
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)x[s].v[j]));
+                top = fmaxf(top, xor_lane(top, 16, lane));
+                top = fmaxf(top, xor_lane(top, 32, lane));
+                ex = top > 0.f && finite(top) ? 13 - ilogbf(top) : 0;
+                c[mt] = fmaxf(ldexpf(c[mt], -ex), 0x1p-126f);         // (c * -inf below)
+            }
+#pragma unroll
+            for (int s = 0; s < DK / 32; ++s)
+                if constexpr (NS == 1) {
+                    qf[0][mt][s] = __builtin_bit_cast(v8, x[s]);
+                } else {
+#pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         T o[NS];
-                        split<T, NS>(x[s][j], o);
+                        split<T, NS>(NS == 2 ? ldexpf(x[s].v[j], ex) : (float)x[s].v[j], o);
 #pragma unroll
                         for (int t = 0; t < NS; ++t) qf[t][mt][s][j] = o[t];
                     }
-            }
+                }
         }
 
-        const T * kb = (const T *)a.k + it.kvh * a.k_head, * vb = (const T *)a.v + it.kvh * a.v_head;
+        const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
+        const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
         const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
         // page numbers of this wave's keys of tile t: one DMA, lane l's key (lanes from 32 on repeat)
         auto issue_tab = [&](uint32_t t) {
             const int32_t key = key0 + (int32_t)(t * KT + (lane & 31));
             const uint32_t pg = (uint32_t)min(key, max(it.cap - 1, 0)) >> a.sh;
-            dma4(it.cap > 0 ? tab + pg : g_attn_zero, tab_at + (t & 1) * 256);
+            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (t & 1) * 256);
         };
         // keys that a row of the strip sees and that have a page: bit per key
         auto issue_kv = [&](uint32_t t, uint32_t stage) -> uint32_t {
@@ -123,28 +123,89 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             const uint32_t own = pgs[lane & 31];
             const int32_t key = k0 + (int32_t)(lane & 31);
             const uint32_t vm = (uint32_t)__ballot(key >= it.lo && key < it.hi && own < a.n_pages);
-            const uint32_t at = mine_at + stage * P::STAGE;
+            const uint32_t at = mine_at + stage * P::STAGE, ln = fresh(lane);
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
-                const uint32_t o = i * 64 + lane, row = o / (DK / 8), e = ((o % (DK / 8)) ^ swz<DK>(row)) * 8;
-                const uint64_t off = (uint64_t)pgs[row] * a.k_page + ((uint32_t)(k0 + (int32_t)row) & a.pmask) * a.k_tok;
-                const bool ok = ((vm >> row) & 1) && e < a.dk;
-                dma16(ok ? (const void *)(kb + off + e) : (const void *)g_attn_zero, at + 1024 * i);
+                const uint32_t o = i * 64 + ln, r = o / (DK / 8), e = ((o % (DK / 8)) ^ swz_k<DK>(r)) * 8;
+                const uint64_t from = row_at(kb, pgs[r], a.k_page, (uint32_t)(k0 + (int32_t)r) & a.pmask, a.k_tok) + 2 * e;
+                dma16((vm >> r) & 1 && e < a.dk ? from : zero, at + 1024 * i);
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const uint32_t o = i * 64 + lane, row = o / (DV / 8), e = ((o % (DV / 8)) ^ swz<DV>(row)) * 8;
-                const uint64_t off = (uint64_t)pgs[row] * a.v_page + ((uint32_t)(k0 + (int32_t)row) & a.pmask) * a.v_tok;
-                const bool ok = ((vm >> row) & 1) && e < a.dv;
-                dma16(ok ? (const void *)(vb + off + e) : (const void *)g_attn_zero, at + 32 * DK * 2 + 1024 * i);
+                const uint32_t o = i * 64 + ln, r = o / (DV / 8), e = ((o % (DV / 8)) ^ swz_v<DV>(r)) * 8;
+                const uint64_t from = row_at(vb, pgs[r], a.v_page, (uint32_t)(k0 + (int32_t)r) & a.pmask, a.v_tok) + 2 * e;
+                dma16((vm >> r) & 1 && e < a.dv ? from : zero, at + 32 * DK * 2 + 1024 * i);
             }
             return vm;
         };
 
         float m[MT], l[MT];
         f32x4 o[MT][DV / 16];
-        bool careful = false;
-        for (;;) {
+        auto tile = [&](int32_t k0, uint32_t vm, uint32_t at) {
+            f32x4 s[MT][2];
+            const uint32_t ka = fresh(at + k_lane), va = fresh(at + v_lane);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < DK / 32; ++d)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const v8 kf = ld_row<T>(piece<DK>(ka, 4 * d) + 16 * kt * DK * 2);
+#pragma unroll
+                    for (int t2 = NS - 1; t2 >= 0; --t2)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mma16(kf, qf[t2][mt][d], s[mt][kt]);
+                }
+            const bool whole = vm == 0xFFFFFFFFu && k0 >= all_lo && k0 + 32 <= all_hi;
+            v8 pf[NS][MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float x[8], top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = s[mt][j >> 2][j & 3];
+                if (!whole) {
+                    const uint32_t see = (vm & (uint32_t)bits_of(rlo[mt] - k0, rhi[mt] - k0)) >> (4 * q4);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = seen(x[j], see, 16 * (j >> 2) + (j & 3));
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+                top = fmaxf(top, xor_lane(top, 16, lane));
+                top = fmaxf(top, xor_lane(top, 32, lane));
+                const float mn = fmaxf(m[mt], top * c[mt]), base = mn == -INFINITY ? 0.f : mn;
+                const float al = __builtin_amdgcn_exp2f(m[mt] - base);
+                m[mt] = mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(x[j], c[mt], -base)) * weight_unit<T>();
+                    sum += p;
+                    T h[NS];
+                    split<T, NS>(p, h);
+#pragma unroll
+                    for (int t2 = 0; t2 < NS; ++t2) pf[t2][mt][j] = h[t2];
+                }
+                l[mt] = fmaf(l[mt], al, sum);
+                if (__ballot(al != 1.f))
+#pragma unroll
+                    for (int d = 0; d < DV / 16; ++d) o[mt][d] *= al;
+            }
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+                v8 vf;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const typename VecOf<T>::v4 r4 = ld_tr<T>(piece<DV>(va, 2 * d) + 16 * kt * DV * 2);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vf[4 * kt + j] = r4[j];
+                }
+#pragma unroll
+                for (int t2 = NS - 1; t2 >= 0; --t2)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) o[mt][d] = mma16(vf, pf[t2][mt], o[mt][d]);
+            }
+        };
+        {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 m[mt] = -INFINITY;
@@ -174,96 +235,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                 const uint32_t vm = vms[0];
                 if (vm) {
                     const int32_t k0 = key0 + (int32_t)(t * KT);
-                    const uint8_t * ks = mine + stage * P::STAGE, * vs = ks + 32 * DK * 2;
-                    f32x4 s[MT][2];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int d = 0; d < DK / 32; ++d) {
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt) {
-                            const uint32_t row = 16 * kt + l16;
-                            const v8 kf = *(const v8 *)(ks + row * (DK * 2) + (((4 * d + q4) ^ swz<DK>(row)) * 16));
-#pragma unroll
-                            for (int t2 = NS - 1; t2 >= 0; --t2)
-#pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mma16(kf, qf[t2][mt][d], s[mt][kt]);
-                        }
-                    }
-                    const bool whole = vm == 0xFFFFFFFFu && k0 >= all_lo && k0 + 32 <= all_hi;
-                    v8 pf[NS][MT], see[MT];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        float x[8], top = -INFINITY;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            x[j] = s[mt][j >> 2][j & 3];
-                            see[mt][j] = (T)1.f;
-                        }
-                        if (!whole) {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const uint32_t b = 16 * (j >> 2) + 4 * q4 + (j & 3);
-                                const int32_t key = k0 + (int32_t)b;
-                                const bool in = ((vm >> b) & 1) && key < rhi[mt] && key >= rlo[mt];
-                                x[j] = in ? x[j] : -INFINITY;
-                                see[mt][j] = (T)(in ? 1.f : 0.f);
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
-                        top = fmaxf(top, xor_lane(top, 16, lane));
-                        top = fmaxf(top, xor_lane(top, 32, lane));
-                        const float mn = fmaxf(m[mt], top * c[mt]), base = mn == -INFINITY ? 0.f : mn;
-                        const float al = __builtin_amdgcn_exp2f(m[mt] - base);
-                        m[mt] = mn;
-                        float sum = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(x[j], c[mt], -base)) * weight_unit<T>();
-                            sum += p;
-                            T h[NS];
-                            split<T, NS>(p, h);
-#pragma unroll
-                            for (int t2 = 0; t2 < NS; ++t2) pf[t2][mt][j] = h[t2];
-                        }
-                        l[mt] = fmaf(l[mt], al, sum);
-                        if (__ballot(al != 1.f))
-#pragma unroll
-                            for (int d = 0; d < DV / 16; ++d) o[mt][d] *= al;
-                    }
-#pragma unroll
-                    for (int d = 0; d < DV / 16; ++d) {
-                        v8 vf;
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt) {
-                            const uint32_t row = 16 * kt + 4 * q4 + (l16 >> 2), pc = 2 * d + ((l16 >> 1) & 1);
-                            const uint8_t * p = vs + row * (DV * 2) + ((pc ^ swz<DV>(row)) * 16) + (l16 & 1) * 8;
-                            const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
-                            const typename VecOf<T>::v4 r4 = __builtin_bit_cast(typename VecOf<T>::v4, r);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) vf[4 * kt + j] = r4[j];
-                        }
-                        if (__builtin_expect(!careful, 1)) {
-#pragma unroll
-                            for (int t2 = NS - 1; t2 >= 0; --t2)
-#pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) o[mt][d] = mma16(vf, pf[t2][mt], o[mt][d]);
-                        } else {
-                            const ValueClass<T> vc(vf);
-                            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                                for (int t2 = NS - 1; t2 >= 0; --t2) o[mt][d] = mma16(__builtin_bit_cast(v8, vc.fin), pf[t2][mt], o[mt][d]);
-                                const f32x4 cp = mma16(__builtin_bit_cast(v8, vc.pos), see[mt], z);
-                                const f32x4 cn = mma16(__builtin_bit_cast(v8, vc.neg), see[mt], z);
-                                const f32x4 cq = mma16(__builtin_bit_cast(v8, vc.nan), see[mt], z);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) o[mt][d][i] += odd_value(cp[i], cn[i], cq[i]);
-                            }
-                        }
-                    }
+                    tile(k0, vm, mine_at + stage * P::STAGE);
                 }
 #pragma unroll
                 for (int i = 0; i + 1 < NST; ++i) vms[i] = vms[i + 1];
@@ -279,7 +251,6 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             wait_vm<0>();
 
             // ---- the waves' sums: to the workgroup's maximum, then added in wave order
-            bool odd = false;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 l[mt] += xor_lane(l[mt], 16, lane);
@@ -291,15 +262,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                     for (int i = 0; i < 4; ++i) odd = odd || !finite(o[mt][d][i]);
                 if (q4 == 0) sm_m[wave * M + 16 * mt + l16] = m[mt];
             }
-            const uint32_t any = __ballot(odd) != 0;
-            if (lane == 0) sm_odd[wave] = any;
             __syncthreads();
-            uint32_t again = 0;
-#pragma unroll
-            for (int i = 0; i < W; ++i) again |= sm_odd[i];
-            if (careful || !again) break;
-            careful = true;
-            __syncthreads();                                          // (the flags are written again)
         }
         float * so = (float *)mine;                                   // [M][DV]
 #pragma unroll
@@ -318,7 +281,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             }
         }
         __syncthreads();
-        float * part = begins && ends ? nullptr : (float *)a.ws + (size_t)M * (DV + 2) * (2 * w + (begins ? 1 : 0));
+        float * part = begins && ends ? nullptr : attn_part<M, DV>(a, w, begins);
         for (uint32_t e = threadIdx.x; e < M * DV / 4; e += 64 * W) {
             const uint32_t r = e / (DV / 4), d = e % (DV / 4) * 4, row = it.strip * M + r;
             if (row >= rows) continue;
@@ -348,6 +311,14 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         u += nt;
         __syncthreads();                                              // the next item's stages
     }
+    const uint32_t any = __ballot(odd) != 0;
+    if (lane == 0) sm_odd[wave] = any;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t f = 0;
+        for (int i = 0; i < W; ++i) f |= sm_odd[i];
+        attn_flags<M, DV>(a)[w] = f;
+    }
 }
 
 namespace {
@@ -358,8 +329,7 @@ template <typename AT, typename T, int DK, int DV, int MT> int go(const AttnArgs
     if (int rc = lds_fits(k, P::LDS, "k_attn_dec")) return rc;
     hipLaunchKernelGGL((k_attn_dec<AT, T, DK, DV, MT>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_dec launch")) return rc;
-    if (a.grid < 2) return FLH_OK;
-    hipLaunchKernelGGL((k_attn_join<AT, M, P::KT, DV>), dim3(a.grid - 1, M / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
 template <typename AT, typename T, int MT> int dims(const AttnArgs & a, hipStream_t s) {
@@ -391,7 +361,7 @@ AttnPlan attn_dec_plan(const AttnArgs & a) {
     p.m = (uint64_t)a.max_q * a.group <= 16 ? 16 : 32;
     p.grid = (uint32_t)num_cus() * (per_cu ? per_cu : 1);
     p.min_units = 1;
-    p.ws = (size_t)p.grid * 2 * p.m * (p.dv + 2) * 4;
+    p.ws = attn_ws(p.grid, p.m, p.dv);
     return p;
 }
 

@@ -216,7 +216,9 @@ struct AttnArgs {
     const void * q; void * out; const void * k; const void * v;
     const uint32_t * q_start; const uint32_t * kv_len; const uint32_t * table;
     void * ws;
-    uint64_t q_tok, q_head, o_tok, o_head, k_page, k_tok, k_head, v_page, v_tok, v_head;
+    uint64_t q_tok, q_head, o_tok, o_head;
+    uint64_t k_head, v_head;            // the cache's strides in bytes
+    uint32_t k_page, k_tok, v_page, v_tok;
     uint32_t n_pages, sh, n_kv, dk, dv, group, n_seq, n_tok, max_q, table_stride, causal, window, pmask;
     uint32_t grid, min_units;           // the launch's (flh_attn.h)
     float scale;

@@ -37,6 +37,8 @@ int check_cache(const flh_kv_cache * c) {
         return set_error(FLH_ERR_UNSUPPORTED, "kv cache: d_k and d_v must be multiples of 8 up to 256");
     if ((c->k_page | c->k_tok | c->k_head | c->v_page | c->v_tok | c->v_head) & 7)
         return set_error(FLH_ERR_ARG, "kv cache: strides must be multiples of 8 elements");
+    if ((c->k_page | c->k_tok | c->v_page | c->v_tok) >= (1ull << 31) || (c->k_head | c->v_head) >= (1ull << 40))
+        return set_error(FLH_ERR_UNSUPPORTED, "kv cache: page and token strides must be below 2^31 elements, head strides below 2^40");
     return FLH_OK;
 }
 
@@ -90,8 +92,8 @@ int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
     a.q = p->q; a.out = p->out; a.q_start = p->q_start; a.kv_len = p->kv_len; a.table = p->table; a.ws = p->ws;
     a.k = c->k; a.v = c->v;
     a.q_tok = p->q_tok; a.q_head = p->q_head; a.o_tok = p->o_tok; a.o_head = p->o_head;
-    a.k_page = c->k_page; a.k_tok = c->k_tok; a.k_head = c->k_head;
-    a.v_page = c->v_page; a.v_tok = c->v_tok; a.v_head = c->v_head;
+    a.k_page = (uint32_t)(2 * c->k_page); a.k_tok = (uint32_t)(2 * c->k_tok); a.k_head = 2 * c->k_head;
+    a.v_page = (uint32_t)(2 * c->v_page); a.v_tok = (uint32_t)(2 * c->v_tok); a.v_head = 2 * c->v_head;
     a.n_pages = c->n_pages; a.sh = (uint32_t)__builtin_ctz(c->page_size); a.n_kv = c->n_kv_head;
     a.dk = c->d_k; a.dv = c->d_v; a.group = group;
     a.n_seq = p->n_seq; a.n_tok = p->n_tok; a.max_q = p->max_q; a.table_stride = p->table_stride;

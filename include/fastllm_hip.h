@@ -378,7 +378,8 @@ enum { FLH_DT_F32 = 0, FLH_DT_F16 = 1, FLH_DT_BF16 = 2 };
  * k + page*k_page + t*k_tok + h*k_head and d_v values at v + ... (strides in
  * elements, so heads may lie inside tokens or tokens inside heads, and k and v
  * may share an allocation).  dtype is F16 or BF16; d_k and d_v are multiples of
- * 8 up to 256; k and v are 16-byte aligned, strides multiples of 8.  A token's
+ * 8 up to 256; k and v are 16-byte aligned, strides multiples of 8 (page and token
+ * strides below 2^31, head strides below 2^40).  A token's
  * slot is page*page_size + t; n_pages*page_size < 2^32 - 1. */
 typedef struct flh_kv_cache {
     void * k, * v;

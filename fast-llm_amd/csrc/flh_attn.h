@@ -29,7 +29,6 @@ template <typename T> struct VecOf {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ f32x4 mma16(VecOf<_Float16>::v8 a, VecOf<_Float16>::v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -56,11 +55,15 @@ template <typename T, int NS> __device__ __forceinline__ void split(float x, T (
         x -= (float)o[i];
     }
 }
-// The weights exp2(score - max) are made 2^14 times larger for f16 terms, so that
+// The weights exp2(score - max) are made 2^7 times larger for f16 terms, so that
 // small ones do not become subnormal there; the sum has the same factor.  (A
-// factor, not 14 more in the exponent: that would cost the largest weights, whose
-// exponent is near 0, three bits.)
-template <typename T> constexpr float weight_unit() { return __is_same(T, _Float16) ? 0x1p14f : 1.f; }
+// factor, not 7 more in the exponent: that would cost the largest weights, whose
+// exponent is near 0, their last bits.)
+template <typename T> constexpr float weight_unit() { return __is_same(T, _Float16) ? 0x1p7f : 1.f; }
+// The running maximum moves (and the sums are rescaled) only when a score passes
+// it by more than this, in powers of two: a weight is below 2^8, 2^15 with the unit,
+// which f16 holds, and the sums' precision does not depend on it.
+constexpr float MAX_SLACK = 8.f;
 
 // ---------------------------------------------------------------- the line --
 struct AttnItem {
@@ -221,13 +224,33 @@ __device__ __forceinline__ uint32_t fresh(uint32_t v) {
     asm volatile("" : "+v"(v));
     return v;
 }
+// The same for what a branch computes with: the compiler cannot move it in
+// front of the branch and select afterwards, which it likes to do with register
+// arithmetic that the branch is there to save.
+__device__ __forceinline__ float fresh(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ uint64_t fresh(uint64_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// An operand that has arrived (the compiler would wait for its load, and with it for
+// every DMA, where it is first used: inside the loop)
+template <typename V> __device__ __forceinline__ void arrived(V & v) {
+    static_assert(sizeof(V) == 16, "four registers");
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    u4 r = __builtin_bit_cast(u4, v);
+    asm volatile("" : "+v"(r));
+    v = __builtin_bit_cast(V, r);
+}
 // base + page * stride + tok * tok_stride, in bytes (strides below 2^32)
 __device__ __forceinline__ uint64_t row_at(uint64_t base, uint32_t page, uint32_t stride, uint32_t tok, uint32_t tok_stride) {
     return base + (uint64_t)page * stride + (uint64_t)tok * tok_stride;
 }
 
-// what a DMA reads in the place of keys that are not there
-static __device__ __attribute__((aligned(16))) uint32_t g_attn_zero[4];
+// the row that a DMA reads in the place of a key that is not there
+static __device__ __attribute__((aligned(16))) uint32_t g_attn_zero[128];
 
 // A 16-byte piece of a row lies in LDS at piece ^ swz(row), so that what a
 // matrix-core operand reads at once spreads over the 64 banks: for K one
@@ -266,6 +289,26 @@ template <typename AT> __device__ __forceinline__ void store4(AT * p, float a, f
     __builtin_memcpy(p, &v, sizeof v);
 }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+
+// A wave's N DMAs, from number i0 on, of a tile's rows.  The addresses of the keys'
+// rows (g_attn_zero for a key that is not there) stand in LDS, a key a lane wrote
+// them; lane ln of DMA i brings piece e of row r.  Pieces behind d are zeros.
+template <int D, bool V, int N> __device__ __forceinline__ void dma_rows(uint32_t addr, uint32_t i0, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
+    uint64_t row[N];
+    uint32_t e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t o = (i0 + i) * 64 + ln, r = o / (D / 8);
+        if constexpr (V) e[i] = ((o % (D / 8)) ^ swz_v<D>(r)) * 8;
+        else e[i] = ((o % (D / 8)) ^ swz_k<D>(r)) * 8;
+        row[i] = *FLH_LDS(uint64_t, addr + 8 * r);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        row[i] = fresh(row[i]) + 2 * e[i];                            // (all are read first; a select, no branch)
+        dma16(e[i] < d ? row[i] : zero, lds + 1024 * (i0 + i));
+    }
+}
 
 // x where bit `at` of m is set, else -infinity
 __device__ __forceinline__ float seen(float x, uint32_t m, uint32_t at) {

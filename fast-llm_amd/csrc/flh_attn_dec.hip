@@ -17,7 +17,7 @@ template <int DK, int DV> struct DecShape {
     static constexpr int KT = 32 * W;                                 // keys of a unit
     static constexpr int NST = DK + DV == 320 ? 3 : 2;                // stages
     static constexpr int STAGE = 32 * (DK + DV) * 2;
-    static constexpr int TAB = 2 * 256;                               // page numbers of two tiles (a DMA writes 64)
+    static constexpr int TAB = 2 * 256 + 512;                         // page numbers of two tiles (a DMA writes 64), row addresses of one
     static constexpr int WAVE = NST * STAGE + TAB;
     static constexpr size_t LDS = (size_t)W * WAVE + 1088;            // and maxima, sums, flags
 };
@@ -96,6 +96,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             for (int s = 0; s < DK / 32; ++s)
                 if constexpr (NS == 1) {
                     qf[0][mt][s] = __builtin_bit_cast(v8, x[s]);
+                    arrived(qf[0][mt][s]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -123,19 +124,12 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             const uint32_t own = pgs[lane & 31];
             const int32_t key = k0 + (int32_t)(lane & 31);
             const uint32_t vm = (uint32_t)__ballot(key >= it.lo && key < it.hi && own < a.n_pages);
-            const uint32_t at = mine_at + stage * P::STAGE, ln = fresh(lane);
-#pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                const uint32_t o = i * 64 + ln, r = o / (DK / 8), e = ((o % (DK / 8)) ^ swz_k<DK>(r)) * 8;
-                const uint64_t from = row_at(kb, pgs[r], a.k_page, (uint32_t)(k0 + (int32_t)r) & a.pmask, a.k_tok) + 2 * e;
-                dma16((vm >> r) & 1 && e < a.dk ? from : zero, at + 1024 * i);
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t o = i * 64 + ln, r = o / (DV / 8), e = ((o % (DV / 8)) ^ swz_v<DV>(r)) * 8;
-                const uint64_t from = row_at(vb, pgs[r], a.v_page, (uint32_t)(k0 + (int32_t)r) & a.pmask, a.v_tok) + 2 * e;
-                dma16((vm >> r) & 1 && e < a.dv ? from : zero, at + 32 * DK * 2 + 1024 * i);
-            }
+            const uint32_t at = mine_at + stage * P::STAGE, ln = fresh(lane), tok = (uint32_t)key & a.pmask, rows_at = tab_at + 512;
+            uint64_t * rows_of = (uint64_t *)(mine + NST * P::STAGE + 512);   // K rows, V rows
+            const uint64_t from = lane < 32 ? row_at(kb, own, a.k_page, tok, a.k_tok) : row_at(vb, own, a.v_page, tok, a.v_tok);
+            rows_of[lane] = (vm >> (lane & 31)) & 1 ? from : zero;
+            dma_rows<DK, false, NK>(rows_at, 0, ln, a.dk, zero, at);
+            dma_rows<DV, true, NV>(rows_at + 256, 0, ln, a.dv, zero, at + 32 * DK * 2);
             return vm;
         };
 
@@ -164,7 +158,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = s[mt][j >> 2][j & 3];
                 if (!whole) {
-                    const uint32_t see = (vm & (uint32_t)bits_of(rlo[mt] - k0, rhi[mt] - k0)) >> (4 * q4);
+                    const uint32_t see = fresh((vm & (uint32_t)bits_of(rlo[mt] - k0, rhi[mt] - k0)) >> (4 * q4));
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] = seen(x[j], see, 16 * (j >> 2) + (j & 3));
                 }
@@ -172,9 +166,15 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
                 top = fmaxf(top, xor_lane(top, 16, lane));
                 top = fmaxf(top, xor_lane(top, 32, lane));
-                const float mn = fmaxf(m[mt], top * c[mt]), base = mn == -INFINITY ? 0.f : mn;
-                const float al = __builtin_amdgcn_exp2f(m[mt] - base);
-                m[mt] = mn;
+                top *= c[mt];
+                if (__ballot(top > m[mt] + MAX_SLACK)) {
+                    const float mn = top > m[mt] + MAX_SLACK ? top : m[mt], al = fresh(mn == m[mt] ? 1.f : __builtin_amdgcn_exp2f(m[mt] - mn));
+                    m[mt] = mn;
+                    l[mt] *= al;
+#pragma unroll
+                    for (int d = 0; d < DV / 16; ++d) o[mt][d] *= al;
+                }
+                const float base = m[mt] == -INFINITY ? 0.f : m[mt];
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -185,10 +185,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
 #pragma unroll
                     for (int t2 = 0; t2 < NS; ++t2) pf[t2][mt][j] = h[t2];
                 }
-                l[mt] = fmaf(l[mt], al, sum);
-                if (__ballot(al != 1.f))
-#pragma unroll
-                    for (int d = 0; d < DV / 16; ++d) o[mt][d] *= al;
+                l[mt] += sum;
             }
 #pragma unroll
             for (int d = 0; d < DV / 16; ++d) {

@@ -15,7 +15,7 @@ template <int DK, int DV> struct PreShape {
     static constexpr int W = 4;                                       // waves
     static constexpr int M = 32 * W, KT = 64, NST = 2;
     static constexpr int STAGE = KT * (DK + DV) * 2;
-    static constexpr int TAB = 2 * 256;                               // a wave's page numbers of two tiles
+    static constexpr int TAB = 2 * 256 + 1024;                        // a wave's page numbers of two tiles, row addresses of one
     static constexpr size_t LDS = (size_t)NST * STAGE + W * TAB + 64;
 };
 template <int DK, int DV> constexpr int pre_threads = 64 * PreShape<DK, DV>::W;
@@ -102,6 +102,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             for (int s = 0; s < DK / 16; ++s)
                 if constexpr (NS == 1) {
                     qf[0][s] = __builtin_bit_cast(v8, x[s]);
+                    arrived(qf[0][s]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -129,19 +130,13 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             const uint32_t own = pgs[lane];
             const int32_t key = k0 + (int32_t)lane;
             const uint64_t vm = __ballot(key >= it.lo && key < it.hi && own < a.n_pages);
-            const uint32_t at = sm_at + stage * P::STAGE, ln = fresh(lane);
-#pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                const uint32_t o = (wave * NK + i) * 64 + ln, r = o / (DK / 8), e = ((o % (DK / 8)) ^ swz_k<DK>(r)) * 8;
-                const uint64_t from = row_at(kb, pgs[r], a.k_page, (uint32_t)(k0 + (int32_t)r) & a.pmask, a.k_tok) + 2 * e;
-                dma16((vm >> r) & 1 && e < a.dk ? from : zero, at + 1024 * (wave * NK + i));
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t o = (wave * NV + i) * 64 + ln, r = o / (DV / 8), e = ((o % (DV / 8)) ^ swz_v<DV>(r)) * 8;
-                const uint64_t from = row_at(vb, pgs[r], a.v_page, (uint32_t)(k0 + (int32_t)r) & a.pmask, a.v_tok) + 2 * e;
-                dma16((vm >> r) & 1 && e < a.dv ? from : zero, at + KT * DK * 2 + 1024 * (wave * NV + i));
-            }
+            const bool in = (vm >> lane) & 1;
+            const uint32_t at = sm_at + stage * P::STAGE, ln = fresh(lane), tok = (uint32_t)key & a.pmask, rows_at = tab_at + 512;
+            uint64_t * rows_of = (uint64_t *)(tabs + 512);
+            rows_of[lane] = in ? row_at(kb, own, a.k_page, tok, a.k_tok) : zero;
+            rows_of[64 + lane] = in ? row_at(vb, own, a.v_page, tok, a.v_tok) : zero;
+            dma_rows<DK, false, NK>(rows_at, wave * NK, ln, a.dk, zero, at);
+            dma_rows<DV, true, NV>(rows_at + 512, wave * NV, ln, a.dv, zero, at + KT * DK * 2);
             return vm;
         };
 
@@ -154,16 +149,47 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+            // K in steps of 32 elements: a step's four operands are read while the step
+            // before is multiplied
+            v8 kf[2][2][2];
+            auto ld_k = [&](int step) {
 #pragma unroll
-            for (int d = 0; d < DK / 16; ++d)
+                for (int d = 0; d < 2; ++d)
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const v8 kf = ld_row<T>(piece<DK>(ka, 2 * d) + 32 * b * DK * 2);
+                    for (int b = 0; b < 2; ++b) kf[step & 1][d][b] = ld_row<T>(piece<DK>(ka, 4 * step + 2 * d) + 32 * b * DK * 2);
+            };
+            ld_k(0);
 #pragma unroll
-                    for (int t2 = NS - 1; t2 >= 0; --t2) s[b] = mma32(kf, qf[t2][d], s[b]);
-                }
+            for (int step = 0; step < DK / 32; ++step) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (step + 1 < DK / 32) ld_k(step + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < 2; ++d)
+#pragma unroll
+                    for (int t2 = NS - 1; t2 >= 0; --t2)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) s[b] = mma32(kf[step & 1][d][b], qf[t2][2 * step + d], s[b]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // V in steps of 16 keys and up to 128 columns, the same way; the first one is
+            // read behind the scores
+            constexpr int DC = DB < 4 ? DB : 4, VSTEPS = KT / 16 * (DB / DC);
+            v8 vf[2][DC];
+            auto ld_v = [&](int step) {
+                const int k = step / (DB / DC), d0 = step % (DB / DC) * DC;
+#pragma unroll
+                for (int d = 0; d < DC; ++d)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const typename VecOf<T>::v4 r4 = ld_tr<T>(piece<DV>(va[p], 4 * (d0 + d)) + 16 * k * DV * 2);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) vf[step & 1][d][4 * p + j] = r4[j];
+                    }
+            };
+            ld_v(0);
             if (!(vm == ~0ull && k0 >= all_lo && k0 + KT <= all_hi)) {
-                const uint64_t see = (vm & bits_of(rlo - k0, rhi - k0)) >> (4 * half);
+                const uint64_t see = fresh((vm & bits_of(rlo - k0, rhi - k0)) >> (4 * half));
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -176,9 +202,15 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
             top = fmaxf(top, xor_lane(top, 32, lane));
-            const float mn = fmaxf(m, top * c), base = mn == -INFINITY ? 0.f : mn;
-            const float al = __builtin_amdgcn_exp2f(m - base);
-            m = mn;
+            top *= c;
+            if (__ballot(top > m + MAX_SLACK)) {
+                const float mn = top > m + MAX_SLACK ? top : m, al = fresh(mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn));
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] *= al;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
             float sum = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -187,32 +219,26 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                     s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -base)) * weight_unit<T>();
                     sum += s[b][i];
                 }
-            l = fmaf(l, al, sum);
-            if (__ballot(al != 1.f))
+            l += sum;
+            v8 pf[NS];
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] *= al;
+            for (int step = 0; step < VSTEPS; ++step) {
+                const int k = step / (DB / DC), d0 = step % (DB / DC) * DC;
+                __builtin_amdgcn_sched_barrier(0);
+                if (step + 1 < VSTEPS) ld_v(step + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                if (d0 == 0)
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k) {                       // 16 keys
-                v8 pf[NS];
+                    for (int j = 0; j < 8; ++j) {
+                        T h[NS];
+                        split<T, NS>(s[k >> 1][8 * (k & 1) + j], h);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    T h[NS];
-                    split<T, NS>(s[k >> 1][8 * (k & 1) + j], h);
-#pragma unroll
-                    for (int t2 = 0; t2 < NS; ++t2) pf[t2][j] = h[t2];
-                }
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    v8 vf;
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const typename VecOf<T>::v4 r4 = ld_tr<T>(piece<DV>(va[p], 4 * d) + 16 * k * DV * 2);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) vf[4 * p + j] = r4[j];
+                        for (int t2 = 0; t2 < NS; ++t2) pf[t2][j] = h[t2];
                     }
 #pragma unroll
-                    for (int t2 = NS - 1; t2 >= 0; --t2) o[d] = mma32(vf, pf[t2], o[d]);
-                }
+                for (int t2 = NS - 1; t2 >= 0; --t2)
+#pragma unroll
+                    for (int d = 0; d < DC; ++d) o[d0 + d] = mma32(vf[step & 1][d], pf[t2], o[d0 + d]);
             }
         };
         {

@@ -6,7 +6,7 @@
 // are rows of one matrix: row r of request s and kv head h is token r / group,
 // head h*group + r % group.  A strip is M consecutive rows.
 //
-// The line of work.  (request, strip, kv head, tile of KT keys that some row of
+// The line of work.  (request, kv head, strip, tile of KT keys that some row of
 // the strip sees), in this order, is one line of U units; workgroup w of Ge
 // takes units [w*U/Ge, (w+1)*U/Ge).  Lengths are on the device only, so every
 // wave walks them itself (64 requests at a time, lane per request): no launch
@@ -79,7 +79,7 @@ template <int M, int KT> struct AttnWalk {
     const AttnArgs & a;
     const uint32_t lane;
     uint32_t base = 0, line0 = 0, all = 0;                            // this chunk of 64 requests: first one, first unit, units
-    uint32_t n = 0, r0 = 0, cost = 0, excl = 0;                       // the lane's request
+    uint32_t n = 0, r0 = 0, one = 0, excl = 0;                        // the lane's request: tokens, first row, units a kv head, units before it
     int32_t p0 = 0, cap = 0;
     __device__ AttnWalk(const AttnArgs & args, uint32_t l) : a(args), lane(l) {}
 
@@ -110,7 +110,7 @@ template <int M, int KT> struct AttnWalk {
     __device__ void load(uint32_t b) {
         base = b;
         const uint32_t s = b + lane;
-        n = r0 = cost = 0;
+        n = r0 = one = 0;
         p0 = cap = 0;
         if (s < a.n_seq) {
             const uint32_t x = min(a.q_start[s], a.n_tok), y = min(a.q_start[s + 1], a.n_tok), kv = a.kv_len[s];
@@ -123,7 +123,7 @@ template <int M, int KT> struct AttnWalk {
         }
         const uint32_t ns = strips(n, a.group);
         int32_t lo, hi;
-        if (ns == 1) cost = span(n, p0, cap, 0, lo, hi);
+        if (ns == 1) one = span(n, p0, cap, 0, lo, hi);
         uint64_t many = __ballot(ns > 1);
         while (many) {                                                // requests of many strips, lane per strip
             const int l = __builtin_ctzll(many);
@@ -134,11 +134,10 @@ template <int M, int KT> struct AttnWalk {
             for (uint32_t i = lane; i < bs; i += 64) c += span(bn, bp, bc, i, lo, hi);
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) c += __shfl_xor(c, d);
-            if (lane == (uint32_t)l) cost = c;
+            if (lane == (uint32_t)l) one = c;
         }
-        cost *= a.n_kv;
-        const uint32_t inc = scan(cost, lane);
-        excl = inc - cost;
+        const uint32_t inc = scan(one * a.n_kv, lane);
+        excl = inc - one * a.n_kv;
         all = __builtin_amdgcn_readlane(inc, 63);
     }
     // units in all; leaves the walk at the first request
@@ -166,12 +165,14 @@ template <int M, int KT> struct AttnWalk {
         it.p0 = __builtin_amdgcn_readlane(p0, l);
         it.cap = __builtin_amdgcn_readlane(cap, l);
         x -= __builtin_amdgcn_readlane(excl, l);
-        const uint32_t ns = strips(it.n, a.group);
+        const uint32_t c1 = __builtin_amdgcn_readlane(one, l), ns = strips(it.n, a.group);
+        it.kvh = x / c1;
+        x -= it.kvh * c1;
         it.strip = 0;
         if (ns > 1) {
             for (uint32_t i = 0;; i += 64) {
                 int32_t lo, hi;
-                const uint32_t c = i + lane < ns ? span(it.n, it.p0, it.cap, i + lane, lo, hi) * a.n_kv : 0u;
+                const uint32_t c = i + lane < ns ? span(it.n, it.p0, it.cap, i + lane, lo, hi) : 0u;
                 const uint32_t inc = scan(c, lane), sum = __builtin_amdgcn_readlane(inc, 63);
                 if (x >= sum && i + 64 < ns) {
                     x -= sum;
@@ -184,8 +185,7 @@ template <int M, int KT> struct AttnWalk {
             }
         }
         it.tiles = span(it.n, it.p0, it.cap, it.strip, it.lo, it.hi);
-        it.kvh = x / it.tiles;
-        it.u0 = u - x % it.tiles;
+        it.u0 = u - x;
     }
 };
 // workgroups that share U units (at least min_units each), and their borders

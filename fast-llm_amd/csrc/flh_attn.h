@@ -394,70 +394,168 @@ template <typename AT, typename T, int M> __device__ __forceinline__ void attn_r
 
 // What a launch leaves in the workspace: the parts of items that lie across a
 // border, [2 * workgroup + (1: the item begins in it)][M][DV] sums, then [M]
-// maxima, [M] weights; then a flag for each workgroup: a sum of it is not finite.
+// maxima, [M] weights; then a note for each workgroup.
+struct AttnNote {
+    uint32_t odd;                       // a sum of this workgroup is not finite
+    uint32_t parts;                     // of the item that its first border is the first one inside (0: none)
+    uint32_t seq, strip, kvh, r0, n;
+    int32_t p0, cap;
+    uint32_t wgs;                       // workgroups that had work (Ge)
+    uint32_t pad[6];
+};
 template <int M, int DV> __device__ __forceinline__ float * attn_part(const AttnArgs & a, uint32_t w, bool begins) {
     return (float *)a.ws + (size_t)M * (DV + 2) * (2 * w + (begins ? 1 : 0));
 }
-template <int M, int DV> __device__ __forceinline__ uint32_t * attn_flags(const AttnArgs & a) {
-    return (uint32_t *)((float *)a.ws + (size_t)M * (DV + 2) * 2 * a.grid);
+template <int M, int DV> __device__ __forceinline__ AttnNote * attn_notes(const AttnArgs & a) {
+    return (AttnNote *)((float *)a.ws + (size_t)M * (DV + 2) * 2 * a.grid);
 }
-inline size_t attn_ws(uint32_t grid, uint32_t m, uint32_t dv) { return (size_t)grid * (2 * m * (dv + 2) + 1) * 4; }
+inline size_t attn_ws(uint32_t grid, uint32_t m, uint32_t dv) { return (size_t)grid * (2 * m * (dv + 2) * 4 + sizeof(AttnNote)); }
 
-// Behind the main kernel.  Workgroups (w, y): if the border between main
-// workgroups w - 1 and w is the first one inside an item, the item's parts are
-// added up in order, a wave a row.  Rows of items with sums that are not
-// finite are done by attn_row instead.
-template <typename AT, typename T, int M, int KT, int DV>
+// The note of workgroup w about its first item (by one thread), which begins `skip` units before w.
+template <int M, int DV>
+__device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32_t U, uint32_t Ge, const AttnItem & it, uint32_t skip) {
+    AttnNote * n = attn_notes<M, DV>(a) + w;
+    uint32_t parts = 0;
+    if (skip && attn_border(w - 1, U, Ge) <= it.u0) {
+        uint32_t last = w;                                            // the last workgroup with a part
+        while (last + 1 < Ge && attn_border(last + 1, U, Ge) < it.u0 + it.tiles) ++last;
+        parts = last - w + 2;
+        n->seq = it.seq; n->strip = it.strip; n->kvh = it.kvh; n->r0 = it.r0; n->n = it.n;
+        n->p0 = it.p0; n->cap = it.cap;
+    }
+    n->parts = parts;
+}
+
+// Behind the main kernel.  Workgroups (w, y): the parts of w's note are added up in
+// order, four rows a wave; PW waves share the parts of the same rows (a few rows of
+// many parts: latency).  Rows of items with sums that are not finite are done by
+// attn_row instead.
+template <typename AT, typename T, int M, int KT, int DV, int PW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
-    const uint32_t lane = threadIdx.x & 63, w = blockIdx.x, r0 = blockIdx.y * 4 + (threadIdx.x >> 6), rs = 4 * gridDim.y;
-    AttnWalk<M, KT> walk(a, lane);
-    const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
-    if (w >= Ge) return;
-    const uint32_t * flags = attn_flags<M, DV>(a);
-    const uint32_t u = attn_border(w, U, Ge), end = attn_border(w + 1, U, Ge);
-    AttnItem it;
-    if (w) {
-        walk.find(u, it);
-        if (u != it.u0 && attn_border(w - 1, U, Ge) <= it.u0) {
-            uint32_t last = w, odd = flags[w - 1] | flags[w];         // the last workgroup with a part
-            while (last + 1 < Ge && attn_border(last + 1, U, Ge) < it.u0 + it.tiles) odd |= flags[++last];
-            const uint32_t parts = last - w + 2, rows = min((uint32_t)M, it.n * a.group - it.strip * M);
-            auto part = [&](uint32_t i) { return (const float *)(i == 0 ? attn_part<M, DV>(a, w - 1, true) : attn_part<M, DV>(a, w - 1 + i, false)); };
-            constexpr int V = DV / 64;                                // values a lane
-            for (uint32_t r = r0; r < rows; r += rs) {
-                if (odd) {
-                    attn_row<AT, T, M>(a, it, r);
-                    continue;
+    constexpr int V = DV / 64, R = 4;                                 // values a lane, rows a wave
+    __shared__ float red[PW > 1 ? PW : 1][R][PW > 1 ? DV : 1];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = blockIdx.x;
+    const AttnNote * notes = attn_notes<M, DV>(a);
+    // workgroups that the main kernel had no work for left no note: their number
+    // is not known here, but the note of workgroup 0 tells how many had
+    if (w >= notes[0].wgs) return;
+    const AttnNote me = notes[w];
+    const uint32_t rbase = (blockIdx.y * (4 / PW) + wave / PW) * R, pw = wave % PW;
+    if (me.parts) {
+        AttnItem it{};
+        it.seq = me.seq; it.strip = me.strip; it.kvh = me.kvh; it.r0 = me.r0; it.n = me.n; it.p0 = me.p0; it.cap = me.cap;
+        const uint32_t parts = me.parts, rows = min((uint32_t)M, it.n * a.group - it.strip * M);
+        // part i of row rbase + k: its maximum, weights and values
+        constexpr size_t P = (size_t)M * (DV + 2);
+        const float * p0 = attn_part<M, DV>(a, w - 1, true), * p1 = attn_part<M, DV>(a, w, false);
+        auto part = [&](uint32_t i) { return i == 0 ? p0 : p1 + 2 * P * (i - 1); };
+        float top[R], l[R], o[R][V];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            top[k] = -INFINITY;
+            l[k] = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[k][v] = 0.f;
+        }
+        uint32_t odd = 0;
+        if (rbase < rows) {
+            const uint32_t last_row = rows - 1;
+            constexpr int Q = PW > 1 ? 8 : 2;                         // parts read at once
+            float x[Q][R][V];
+            auto read = [&](uint32_t i0, uint32_t n) {                // (rows behind the last one: any values)
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    const float * p = part(min(i0 + q * PW, n - 1)) + (size_t)rbase * DV + lane * V;
+#pragma unroll
+                    for (int k = 0; k < R; ++k)
+#pragma unroll
+                        for (int v = 0; v < V; ++v) x[q][k][v] = p[k * DV + v];
                 }
-                float top = -INFINITY;
-                for (uint32_t i = lane; i < parts; i += 64) top = fmaxf(top, part(i)[(size_t)M * DV + r]);
+            };
+            for (uint32_t c = 0; c < parts; c += 64) {                // 64 parts, a lane each
+                const uint32_t mine = min(c + lane, parts - 1), cend = min(c + 64, parts);
+                float m[R], s[R], f[R];
 #pragma unroll
-                for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, xor_lane(top, d, lane));
-                const float base = top == -INFINITY ? 0.f : top;
-                float l = 0.f, o[V];
-#pragma unroll
-                for (int k = 0; k < V; ++k) o[k] = 0.f;
-#pragma unroll 4
-                for (uint32_t i = 0; i < parts; ++i) {
-                    const float * p = part(i);
-                    const float f = __builtin_amdgcn_exp2f(p[(size_t)M * DV + r] - base);
-                    l = fmaf(f, p[(size_t)M * (DV + 1) + r], l);
-#pragma unroll
-                    for (int k = 0; k < V; ++k) o[k] = fmaf(f, p[(size_t)r * DV + lane * V + k], o[k]);
+                for (int k = 0; k < R; ++k) {
+                    const float * p = part(mine) + (size_t)M * DV + min(rbase + k, last_row);
+                    m[k] = p[0];
+                    s[k] = p[M];
                 }
-                const uint32_t row = it.strip * M + r, tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
+                odd |= notes[w - 1 + mine].odd;
+                read(c + pw, cend);
+#pragma unroll
+                for (int k = 0; k < R; ++k) {
+                    float t = m[k];
+#pragma unroll
+                    for (int d = 1; d < 64; d <<= 1) t = fmaxf(t, xor_lane(t, d, lane));
+                    t = fmaxf(t, top[k]);
+                    const float base = t == -INFINITY ? 0.f : t, al = __builtin_amdgcn_exp2f(top[k] - base);
+                    top[k] = t;
+                    f[k] = c + lane < parts ? __builtin_amdgcn_exp2f(m[k] - base) : 0.f;
+                    l[k] = fmaf(l[k], al, f[k] * s[k]);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[k][v] *= al;
+                }
+                for (uint32_t i = c + pw;;) {
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) {
+                        const uint32_t j = i + q * PW;
+                        if (j < cend)
+#pragma unroll
+                            for (int k = 0; k < R; ++k) {
+                                const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[k]), j - c));
+#pragma unroll
+                                for (int v = 0; v < V; ++v) o[k][v] = fmaf(g, x[q][k][v], o[k][v]);
+                            }
+                    }
+                    i += Q * PW;
+                    if (i >= cend) break;
+                    read(i, cend);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) l[k] += xor_lane(l[k], d, lane);
+        }
+        if (__ballot(odd != 0)) {
+            if (pw == 0)
+                for (uint32_t r = rbase; r < min(rbase + R, rows); ++r) attn_row<AT, T, M>(a, it, r);
+        } else if (rbase < rows) {
+            if constexpr (PW > 1) {
+#pragma unroll
+                for (int k = 0; k < R; ++k)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) red[pw][k][lane * V + v] = o[k][v];
+                __syncthreads();
+            }
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                if (rbase + k >= rows || (PW > 1 && k % PW != (int)pw)) continue;
+                const uint32_t row = it.strip * M + rbase + k, tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
                 AT * out = (AT *)a.out + tok * a.o_tok + head * a.o_head;
 #pragma unroll
-                for (int k = 0; k < V; ++k)
-                    if (lane * V + k < a.dv) out[lane * V + k] = (AT)(l == 0.f ? 0.f : o[k] / l);
+                for (int v = 0; v < V; ++v) {
+                    float x = o[k][v];
+                    if constexpr (PW > 1) {
+                        x = red[0][k][lane * V + v];
+#pragma unroll
+                        for (int i = 1; i < PW; ++i) x += red[i][k][lane * V + v];
+                    }
+                    if (lane * V + v < a.dv) out[lane * V + v] = (AT)(l[k] == 0.f ? 0.f : x / l[k]);
+                }
             }
         }
     }
-    if (!flags[w]) return;
+    if (!me.odd || pw) return;
+    AttnWalk<M, KT> walk(a, lane);
+    const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
+    const uint32_t u = attn_border(w, U, Ge), end = attn_border(w + 1, U, Ge);
     for (uint32_t x = u; x < end;) {                                  // items of workgroup w alone
+        AttnItem it;
         walk.find(x, it);
         if (it.u0 >= u && it.u0 + it.tiles <= end)
-            for (uint32_t r = r0; r < min((uint32_t)M, it.n * a.group - it.strip * M); r += rs) attn_row<AT, T, M>(a, it, r);
+            for (uint32_t r = rbase; r < min((uint32_t)M, min(rbase + R, it.n * a.group - it.strip * M)); ++r) attn_row<AT, T, M>(a, it, r);
         x = it.u0 + it.tiles;
     }
 }

@@ -47,6 +47,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units), w = blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
+    const uint32_t first_u = u;
     const uint32_t end = attn_border(w + 1, U, Ge);
     bool odd = false;                                                 // a sum is not finite
     while (u < end) {
@@ -55,6 +56,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT + 32 * wave);   // this wave's first key
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
+        if (u == first_u && threadIdx.x == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group;
 
         // ---- the strip's queries, as the second operand: column l16, elements 32 s + 8 q4 ..
@@ -314,7 +316,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     if (threadIdx.x == 0) {
         uint32_t f = 0;
         for (int i = 0; i < W; ++i) f |= sm_odd[i];
-        attn_flags<M, DV>(a)[w] = f;
+        AttnNote * n = attn_notes<M, DV>(a) + w;
+        n->odd = f;
+        n->wgs = Ge;
     }
 }
 
@@ -326,7 +330,7 @@ template <typename AT, typename T, int DK, int DV, int MT> int go(const AttnArgs
     if (int rc = lds_fits(k, P::LDS, "k_attn_dec")) return rc;
     hipLaunchKernelGGL((k_attn_dec<AT, T, DK, DV, MT>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_dec launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
 template <typename AT, typename T, int MT> int dims(const AttnArgs & a, hipStream_t s) {

@@ -53,6 +53,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
     const uint32_t w = Ge == a.grid && a.grid % 8 == 0 ? (blockIdx.x & 7) * (a.grid / 8) + (blockIdx.x >> 3) : blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
+    const uint32_t first_u = u;
     const uint32_t end = attn_border(w + 1, U, Ge);
     bool odd = false;                                                 // a sum is not finite
     while (u < end) {
@@ -61,6 +62,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT);
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
+        if (u == first_u && threadIdx.x == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group, row = it.strip * M + 32 * wave + l32, tok = row / a.group;
         const uint32_t head = it.kvh * a.group + row % a.group;
         const int32_t win = (int32_t)min(a.window, 1u << 30);
@@ -323,7 +325,9 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
     if (threadIdx.x == 0) {
         uint32_t f = 0;
         for (int i = 0; i < W; ++i) f |= sm_odd[i];
-        attn_flags<M, DV>(a)[w] = f;
+        AttnNote * n = attn_notes<M, DV>(a) + w;
+        n->odd = f;
+        n->wgs = Ge;
     }
 }
 
@@ -334,7 +338,7 @@ template <typename AT, typename T, int DK, int DV> int go(const AttnArgs & a, hi
     if (int rc = lds_fits(k, P::LDS, "k_attn_pre")) return rc;
     hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_pre launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV>), dim3(a.grid, 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV, 1>), dim3(a.grid, P::M / 16), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
 template <typename AT, typename T> int dims(const AttnArgs & a, hipStream_t s) {

@@ -15,7 +15,8 @@ template <int DK, int DV> struct PreShape {
     static constexpr int W = 4;                                       // waves
     static constexpr int M = 32 * W, KT = 64, NST = 2;
     static constexpr int STAGE = KT * (DK + DV) * 2;
-    static constexpr int TAB = 2 * 256 + 1024;                        // a wave's page numbers of two tiles, row addresses of one
+    // a wave's page numbers of two tiles, row addresses: K of one tile, V of two
+    static constexpr int TAB = 2 * 256 + 3 * 512;
     static constexpr size_t LDS = (size_t)NST * STAGE + W * TAB + 64;
 };
 template <int DK, int DV> constexpr int pre_threads = 64 * PreShape<DK, DV>::W;
@@ -27,7 +28,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
     typedef PreShape<DK, DV> P;
     typedef typename VecOf<T>::v8 v8;
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = P::M, NS = split_terms<AT, T>();
-    constexpr int NK = DK / 8 / W, NV = DV / 8 / W, ND = NK + NV;     // DMAs of a tile, this wave's
+    constexpr int NK = DK / 8 / W, NV = DV / 8 / W;                   // DMAs of a tile, this wave's
     constexpr int DB = DV / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
     const uint32_t lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5, l16 = lane & 15;
@@ -66,14 +67,13 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         const uint32_t rows = it.n * a.group, row = it.strip * M + 32 * wave + l32, tok = row / a.group;
         const uint32_t head = it.kvh * a.group + row % a.group;
         const int32_t win = (int32_t)min(a.window, 1u << 30);
-        // keys that the lane's row sees; that a row of the wave sees; that all of them see
+        // keys that the lane's row sees; that all of the wave's rows see
         const int32_t rhi = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
         const int32_t rlo = win ? it.p0 + (int32_t)tok + 1 - win : 0;
         const uint32_t first = it.strip * M + 32 * wave;              // the wave's rows
         const bool here = first < rows;
         const int32_t tf = (int32_t)(first / a.group), tl = (int32_t)min(it.n - 1, (first + 31) / a.group);
         const int32_t all_lo = win ? it.p0 + tl + 1 - win : 0, all_hi = a.causal ? min(it.cap, it.p0 + tf + 1) : it.cap;
-        const int32_t any_lo = win ? it.p0 + tf + 1 - win : 0, any_hi = a.causal ? min(it.cap, it.p0 + tl + 1) : it.cap;
 
         // ---- queries: column l32, elements 16 s + 8 half ..
         v8 qf[NS][DK / 16];
@@ -124,72 +124,44 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             const uint32_t pg = (uint32_t)min(key, max(it.cap - 1, 0)) >> a.sh;
             dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (t & 1) * 256);
         };
-        // this wave's part of tile t's rows; returns the keys that a row of the strip
-        // sees and that have a page, a bit each
-        auto issue_kv = [&](uint32_t t, uint32_t stage) -> uint64_t {
-            const int32_t k0 = key0 + (int32_t)(t * KT);
-            const uint32_t * pgs = (const uint32_t *)(tabs + (t & 1) * 256);
-            const uint32_t own = pgs[lane];
-            const int32_t key = k0 + (int32_t)lane;
-            const uint64_t vm = __ballot(key >= it.lo && key < it.hi && own < a.n_pages);
-            const bool in = (vm >> lane) & 1;
-            const uint32_t at = sm_at + stage * P::STAGE, ln = fresh(lane), tok = (uint32_t)key & a.pmask, rows_at = tab_at + 512;
+        // this wave's part of tile t's K rows, and where its V rows are; returns the keys
+        // that a row of the strip sees and that have a page, a bit each
+        auto issue_k = [&](uint32_t t) -> uint64_t {
+            const int32_t key = key0 + (int32_t)(t * KT + lane);
+            const uint32_t own = *(const uint32_t *)(tabs + (t & 1) * 256 + 4 * lane), tok = (uint32_t)key & a.pmask;
+            const bool in = key >= it.lo && key < it.hi && own < a.n_pages;
             uint64_t * rows_of = (uint64_t *)(tabs + 512);
             rows_of[lane] = in ? row_at(kb, own, a.k_page, tok, a.k_tok) : zero;
-            rows_of[64 + lane] = in ? row_at(vb, own, a.v_page, tok, a.v_tok) : zero;
-            dma_rows<DK, false, NK>(rows_at, wave * NK, ln, a.dk, zero, at);
-            dma_rows<DV, true, NV>(rows_at + 512, wave * NV, ln, a.dv, zero, at + KT * DK * 2);
-            return vm;
+            rows_of[64 + 64 * (t & 1) + lane] = in ? row_at(vb, own, a.v_page, tok, a.v_tok) : zero;
+            dma_rows<DK, false, NK>(tab_at + 512, wave * NK, fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE);
+            return __ballot(in);
+        };
+        auto issue_v = [&](uint32_t t) {
+            dma_rows<DV, true, NV>(tab_at + 1024 + 512 * (t & 1), wave * NV, fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2);
         };
 
         float m, l;
         f32x16 o[DB];
-        auto tile = [&](int32_t k0, uint64_t vm, uint32_t at) {
-            f32x16 s[2];
-            const uint32_t ka = fresh(at + k_lane), va[2] = {fresh(at + v_lane[0]), fresh(at + v_lane[1])};
+        f32x16 s[2];                                                  // scores of the tile at hand
+        // the tile at `at` times the queries, in steps of 16 elements
+        auto scores = [&](uint32_t at, f32x16 (&x)[2]) {
+            const uint32_t ka = fresh(at + k_lane);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-            // K in steps of 32 elements: a step's four operands are read while the step
-            // before is multiplied
-            v8 kf[2][2][2];
-            auto ld_k = [&](int step) {
+                for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
 #pragma unroll
-                for (int d = 0; d < 2; ++d)
+            for (int d = 0; d < DK / 16; ++d)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) kf[step & 1][d][b] = ld_row<T>(piece<DK>(ka, 4 * step + 2 * d) + 32 * b * DK * 2);
-            };
-            ld_k(0);
+                for (int b = 0; b < 2; ++b) {
+                    const v8 kf = ld_row<T>(piece<DK>(ka, 2 * d) + 32 * b * DK * 2);
 #pragma unroll
-            for (int step = 0; step < DK / 32; ++step) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (step + 1 < DK / 32) ld_k(step + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int d = 0; d < 2; ++d)
-#pragma unroll
-                    for (int t2 = NS - 1; t2 >= 0; --t2)
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) s[b] = mma32(kf[step & 1][d][b], qf[t2][2 * step + d], s[b]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            // V in steps of 16 keys and up to 128 columns, the same way; the first one is
-            // read behind the scores
-            constexpr int DC = DB < 4 ? DB : 4, VSTEPS = KT / 16 * (DB / DC);
-            v8 vf[2][DC];
-            auto ld_v = [&](int step) {
-                const int k = step / (DB / DC), d0 = step % (DB / DC) * DC;
-#pragma unroll
-                for (int d = 0; d < DC; ++d)
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const typename VecOf<T>::v4 r4 = ld_tr<T>(piece<DV>(va[p], 4 * (d0 + d)) + 16 * k * DV * 2);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) vf[step & 1][d][4 * p + j] = r4[j];
-                    }
-            };
-            ld_v(0);
+                    for (int t2 = NS - 1; t2 >= 0; --t2) x[b] = mma32(kf, qf[t2][d], x[b]);
+                }
+        };
+        // s: a tile's scores -> sums; the scores of the next one (K at `next`) are
+        // multiplied meanwhile and end up in s
+        auto tile = [&](int32_t k0, uint64_t vm, uint32_t at, uint32_t next) {
             if (!(vm == ~0ull && k0 >= all_lo && k0 + KT <= all_hi)) {
                 const uint64_t see = fresh((vm & bits_of(rlo - k0, rhi - k0)) >> (4 * half));
 #pragma unroll
@@ -213,35 +185,79 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                 for (int d = 0; d < DB; ++d) o[d] *= al;
             }
             const float base = m == -INFINITY ? 0.f : m;
+            // ---- the products run under the vector instructions.  The order is fixed by
+            // hand (the barriers stop the compiler, which would gather the products): step i
+            // of the next tile's scores (one K operand, read three steps before) with a share
+            // of the weights of the first 32 keys; then V, 16 keys and up to 128 columns a
+            // step, the first steps with the weights of the other 32 keys.
             float sum = 0.f;
+            v8 pf[KT / 16][NS];
+            auto weights = [&](int e0, int e1) {                      // of the lane's elements e0 .. e1
+#pragma unroll
+                for (int e = e0; e < e1; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], c, -base)) * weight_unit<T>();
+                    sum += p;
+                    T h[NS];
+                    split<T, NS>(p, h);
+#pragma unroll
+                    for (int t2 = 0; t2 < NS; ++t2) pf[e >> 3][t2][e & 7] = h[t2];
+                }
+            };
+            f32x16 nx[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -base)) * weight_unit<T>();
-                    sum += s[b][i];
-                }
-            l += sum;
-            v8 pf[NS];
+                for (int i = 0; i < 16; ++i) nx[b][i] = 0.f;
+            constexpr int NF = DK / 8;                                // K operands of a tile
+            const uint32_t ka = fresh(next + k_lane), va[2] = {fresh(at + v_lane[0]), fresh(at + v_lane[1])};
+            v8 kf[4];
+            auto ld_k = [&](int i) { kf[i & 3] = ld_row<T>(piece<DK>(ka, 2 * (i >> 1)) + 32 * (i & 1) * DK * 2); };
+            constexpr int DC = DB < 4 ? DB : 4, VSTEPS = KT / 16 * (DB / DC);
+            v8 vf[2][DC];
+            auto ld_v = [&](int step) {
+                const int k = step / (DB / DC), d0 = step % (DB / DC) * DC;
+#pragma unroll
+                for (int d = 0; d < DC; ++d)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const typename VecOf<T>::v4 r4 = ld_tr<T>(piece<DV>(va[p], 4 * (d0 + d)) + 16 * k * DV * 2);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) vf[step & 1][d][4 * p + j] = r4[j];
+                    }
+            };
+            ld_k(0);
+            ld_k(1);
+            ld_k(2);
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + 3 < NF) ld_k(i + 3);
+                if (i + 3 == NF) ld_v(0);
+#pragma unroll
+                for (int t2 = NS - 1; t2 >= 0; --t2) nx[i & 1] = mma32(kf[i & 3], qf[t2][i >> 1], nx[i & 1]);
+                weights(16 * i / NF, 16 * (i + 1) / NF);
+            }
 #pragma unroll
             for (int step = 0; step < VSTEPS; ++step) {
                 const int k = step / (DB / DC), d0 = step % (DB / DC) * DC;
                 __builtin_amdgcn_sched_barrier(0);
                 if (step + 1 < VSTEPS) ld_v(step + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                if (d0 == 0)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        T h[NS];
-                        split<T, NS>(s[k >> 1][8 * (k & 1) + j], h);
-#pragma unroll
-                        for (int t2 = 0; t2 < NS; ++t2) pf[t2][j] = h[t2];
-                    }
 #pragma unroll
                 for (int t2 = NS - 1; t2 >= 0; --t2)
 #pragma unroll
-                    for (int d = 0; d < DC; ++d) o[d0 + d] = mma32(vf[step & 1][d], pf[t2], o[d0 + d]);
+                    for (int d = 0; d < DC; ++d) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        o[d0 + d] = mma32(vf[step & 1][d], pf[k][t2], o[d0 + d]);
+                        // the first half of the steps' products carry the weights 16 .. 31
+                        constexpr int H = VSTEPS / 2 * NS * DC;
+                        const int i = (step * NS + (NS - 1 - t2)) * DC + d;
+                        if (i < H) weights(16 + 16 * i / H, 16 + 16 * (i + 1) / H);
+                    }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            l += sum;
+            s[0] = nx[0];
+            s[1] = nx[1];
         };
         {
             m = -INFINITY;
@@ -250,34 +266,31 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-            // order of issue: T0, T1 KV0, T2 KV1, ..: a tile's pages are behind the tile before
-            uint64_t vm0 = 0, vm1 = 0;
+            // K runs a tile ahead of V: stage t & 1 has K of tile t, then of t + 2, while V
+            // of tile t is still needed.  Every wave brings its part at the begin of a round,
+            // behind the barrier that tells that the round before is over, and waits
+            // for it at the begin of the next.
+            uint64_t vm0, vm1 = 0, vm2 = 0;
             issue_tab(0);
             issue_tab(1);
-            wait_vm<1>();
-            vm0 = issue_kv(0, 0);
-            if (nt > 1) {
-                issue_tab(2);
-                wait_vm<ND + 1>();
-                vm1 = issue_kv(1, 1);
-            }
-            uint32_t stage = 0;
+            wait_vm<0>();
+            vm0 = issue_k(0);
+            issue_v(0);
+            if (nt > 1) vm1 = issue_k(1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (the page numbers have been read)
+            issue_tab(2);
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (here) scores(sm_at, s);
             for (uint32_t t = 0; t < nt; ++t) {
-                if (t + 1 < nt) wait_vm<ND + 1>();
-                else wait_vm<0>();
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // all parts of tile t are there
-                const uint64_t vm = vm0;
-                vm0 = vm1;
-                vm1 = 0;
-                const int32_t k0 = key0 + (int32_t)(t * KT);
-                if (here && vm && k0 < any_hi && k0 + KT > any_lo) tile(k0, vm, sm_at + stage * P::STAGE);
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the stage has been read
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (t + 2 < nt) {
+                    vm2 = issue_k(t + 2);
                     issue_tab(t + 3);
-                    wait_vm<ND + 1>();
-                    vm1 = issue_kv(t + 2, stage);
                 }
-                stage ^= 1;
+                if (t + 1 < nt) issue_v(t + 1);
+                if (here) tile(key0 + (int32_t)(t * KT), vm0, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE);
+                vm0 = vm1;
+                vm1 = vm2;
             }
             wait_vm<0>();
             odd = odd || !finite(l);
@@ -318,6 +331,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             }
         }
         u += nt;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the next item's stages
     }
     const uint32_t any = __ballot(odd) != 0;
     if (lane == 0) sm_odd[wave] = any;

@@ -65,6 +65,24 @@ template <typename T> constexpr float weight_unit() { return __is_same(T, _Float
 // which f16 holds, and the sums' precision does not depend on it.
 constexpr float MAX_SLACK = 8.f;
 
+// A value that the compiler takes for a new one: what is computed from it is
+// computed where it stands (a few instructions a tile), not kept in registers
+// around the loop over the tiles.
+__device__ __forceinline__ uint32_t fresh(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// The same for what a branch computes with: the compiler cannot move it in
+// front of the branch and select afterwards, which it likes to do with register
+// arithmetic that the branch is there to save.
+__device__ __forceinline__ float fresh(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ uint64_t fresh(uint64_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 // ---------------------------------------------------------------- the line --
 struct AttnItem {
     uint32_t seq, strip, kvh;
@@ -76,18 +94,22 @@ struct AttnItem {
 };
 
 template <int M, int KT> struct AttnWalk {
+    // the wave's 64 requests at hand, in LDS (they are looked at once an item)
+    struct Chunk {
+        uint32_t n[64], r0[64], one[64], excl[64];                    // tokens, first row, units a kv head, units before it
+        int32_t p0[64], cap[64];                                      // position of the first row, keys with a table entry
+    };
     const AttnArgs & a;
-    const uint32_t lane;
-    uint32_t base = 0, line0 = 0, all = 0;                            // this chunk of 64 requests: first one, first unit, units
-    uint32_t n = 0, r0 = 0, one = 0, excl = 0;                        // the lane's request: tokens, first row, units a kv head, units before it
-    int32_t p0 = 0, cap = 0;
-    __device__ AttnWalk(const AttnArgs & args, uint32_t l) : a(args), lane(l) {}
+    Chunk & ch;
+    uint32_t base = 0, line0 = 0, all = 0;                            // the chunk's first request, first unit, units
+    __device__ AttnWalk(const AttnArgs & args, Chunk & c) : a(args), ch(c) {}
+    template <typename V> __device__ static V get(const V & v) { return (V)__builtin_amdgcn_readfirstlane((int)v); }
 
     __device__ static uint32_t scan(uint32_t v, uint32_t lane) {      // inclusive, over the wave
 #pragma unroll
         for (uint32_t d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(v, d);
-            if (lane >= d) v += o;
+            v += lane >= d ? o : 0u;
         }
         return v;
     }
@@ -107,23 +129,24 @@ template <int M, int KT> struct AttnWalk {
     }
     __device__ static uint32_t strips(uint32_t n_, uint32_t group) { return (n_ * group + M - 1) / M; }
 
+    // (No branch that only some lanes take, here and around the kernels' tiles: where
+    // such branches join, the compiler has put copies of live registers in front of
+    // the instruction that switches the other lanes on again, and their values were lost.)
     __device__ void load(uint32_t b) {
+        const uint32_t lane = threadIdx.x & 63;
         base = b;
-        const uint32_t s = b + lane;
-        n = r0 = one = 0;
-        p0 = cap = 0;
-        if (s < a.n_seq) {
-            const uint32_t x = min(a.q_start[s], a.n_tok), y = min(a.q_start[s + 1], a.n_tok), kv = a.kv_len[s];
-            n = y > x ? y - x : 0;
-            r0 = x;
-            // positions and keys behind 2^30 have no table entry (see the host's check)
-            const int64_t k = min((int64_t)kv, (int64_t)1 << 30);
-            cap = (int32_t)min(k, (int64_t)a.table_stride << a.sh);
-            p0 = (int32_t)(k - n);
-        }
+        const uint32_t s = min(b + lane, a.n_seq - 1);
+        const bool real = b + lane < a.n_seq;
+        const uint32_t x = min(a.q_start[s], a.n_tok), y = min(a.q_start[s + 1], a.n_tok), kv = a.kv_len[s];
+        const uint32_t n = real && y > x ? y - x : 0;
+        // positions and keys behind 2^30 have no table entry (see the host's check)
+        const int32_t k = (int32_t)min(kv, 1u << 30);
+        const int32_t cap = (int32_t)min((uint64_t)k, (uint64_t)a.table_stride << a.sh);
+        const int32_t p0 = k - (int32_t)n;
         const uint32_t ns = strips(n, a.group);
         int32_t lo, hi;
-        if (ns == 1) one = span(n, p0, cap, 0, lo, hi);
+        uint32_t one = fresh(span(max(n, 1u), p0, cap, 0, lo, hi));
+        one = ns == 1 ? one : 0;
         uint64_t many = __ballot(ns > 1);
         while (many) {                                                // requests of many strips, lane per strip
             const int l = __builtin_ctzll(many);
@@ -131,14 +154,22 @@ template <int M, int KT> struct AttnWalk {
             const uint32_t bn = __builtin_amdgcn_readlane(n, l), bs = __builtin_amdgcn_readlane(ns, l);
             const int32_t bp = __builtin_amdgcn_readlane(p0, l), bc = __builtin_amdgcn_readlane(cap, l);
             uint32_t c = 0;
-            for (uint32_t i = lane; i < bs; i += 64) c += span(bn, bp, bc, i, lo, hi);
+            for (uint32_t i = 0; i < bs; i += 64) {
+                const uint32_t v = fresh(span(bn, bp, bc, i + lane, lo, hi));
+                c += i + lane < bs ? v : 0u;
+            }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) c += __shfl_xor(c, d);
-            if (lane == (uint32_t)l) one = c;
+            one = lane == (uint32_t)l ? c : one;
         }
         const uint32_t inc = scan(one * a.n_kv, lane);
-        excl = inc - one * a.n_kv;
         all = __builtin_amdgcn_readlane(inc, 63);
+        ch.n[lane] = n;
+        ch.r0[lane] = x;
+        ch.one[lane] = one;
+        ch.excl[lane] = inc - one * a.n_kv;
+        ch.p0[lane] = p0;
+        ch.cap[lane] = cap;
     }
     // units in all; leaves the walk at the first request
     __device__ uint32_t total() {
@@ -157,22 +188,23 @@ template <int M, int KT> struct AttnWalk {
             line0 += all;
             load(base + 64);
         }
+        const uint32_t lane = threadIdx.x & 63;
         uint32_t x = u - line0;
-        const int l = 63 - __builtin_clzll(__ballot(excl <= x));      // (requests of no units share the next one's excl)
+        const int l = 63 - __builtin_clzll(__ballot(ch.excl[lane] <= x));   // (requests of no units share the next one's excl)
         it.seq = base + l;
-        it.n = __builtin_amdgcn_readlane(n, l);
-        it.r0 = __builtin_amdgcn_readlane(r0, l);
-        it.p0 = __builtin_amdgcn_readlane(p0, l);
-        it.cap = __builtin_amdgcn_readlane(cap, l);
-        x -= __builtin_amdgcn_readlane(excl, l);
-        const uint32_t c1 = __builtin_amdgcn_readlane(one, l), ns = strips(it.n, a.group);
+        it.n = get(ch.n[l]);
+        it.r0 = get(ch.r0[l]);
+        it.p0 = get(ch.p0[l]);
+        it.cap = get(ch.cap[l]);
+        x -= get(ch.excl[l]);
+        const uint32_t c1 = get(ch.one[l]), ns = strips(it.n, a.group);
         it.kvh = x / c1;
         x -= it.kvh * c1;
         it.strip = 0;
         if (ns > 1) {
             for (uint32_t i = 0;; i += 64) {
                 int32_t lo, hi;
-                const uint32_t c = i + lane < ns ? span(it.n, it.p0, it.cap, i + lane, lo, hi) : 0u;
+                const uint32_t v = fresh(span(it.n, it.p0, it.cap, i + lane, lo, hi)), c = i + lane < ns ? v : 0u;
                 const uint32_t inc = scan(c, lane), sum = __builtin_amdgcn_readlane(inc, 63);
                 if (x >= sum && i + 64 < ns) {
                     x -= sum;
@@ -217,24 +249,6 @@ __device__ __forceinline__ uint32_t lds_at(const void * p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
 
-// A value that the compiler takes for a new one: what is computed from it is
-// computed where it stands (a few instructions a tile), not kept in registers
-// around the loop over the tiles.
-__device__ __forceinline__ uint32_t fresh(uint32_t v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-// The same for what a branch computes with: the compiler cannot move it in
-// front of the branch and select afterwards, which it likes to do with register
-// arithmetic that the branch is there to save.
-__device__ __forceinline__ float fresh(float v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-__device__ __forceinline__ uint64_t fresh(uint64_t v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
 // An operand that has arrived (the compiler would wait for its load, and with it for
 // every DMA, where it is first used: inside the loop)
 template <typename V> __device__ __forceinline__ void arrived(V & v) {
@@ -293,21 +307,29 @@ __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0
 // A wave's N DMAs, from number i0 on, of a tile's rows.  The addresses of the keys'
 // rows (g_attn_zero for a key that is not there) stand in LDS, a key a lane wrote
 // them; lane ln of DMA i brings piece e of row r.  Pieces behind d are zeros.
-template <int D, bool V, int N> __device__ __forceinline__ void dma_rows(uint32_t addr, uint32_t i0, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
+template <int D, bool V, int N> struct DmaRows {
     uint64_t row[N];
-    uint32_t e[N];
+    __device__ __forceinline__ static uint32_t index(uint32_t i, uint32_t ln) { return (i * 64 + ln) / (D / 8); }
+    __device__ __forceinline__ void read(uint32_t addr, uint32_t i0, uint32_t ln) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t o = (i0 + i) * 64 + ln, r = o / (D / 8);
-        if constexpr (V) e[i] = ((o % (D / 8)) ^ swz_v<D>(r)) * 8;
-        else e[i] = ((o % (D / 8)) ^ swz_k<D>(r)) * 8;
-        row[i] = *FLH_LDS(uint64_t, addr + 8 * r);
+        for (int i = 0; i < N; ++i) row[i] = *FLH_LDS(uint64_t, addr + 8 * index(i0 + i, ln));
     }
+    __device__ __forceinline__ void issue(uint32_t i0, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        row[i] = fresh(row[i]) + 2 * e[i];                            // (all are read first; a select, no branch)
-        dma16(e[i] < d ? row[i] : zero, lds + 1024 * (i0 + i));
+        for (int i = 0; i < N; ++i) {
+            const uint32_t r = index(i0 + i, ln), p = ((i0 + i) * 64 + ln) % (D / 8);
+            uint32_t e;
+            if constexpr (V) e = (p ^ swz_v<D>(r)) * 8;
+            else e = (p ^ swz_k<D>(r)) * 8;
+            row[i] = fresh(row[i]) + 2 * e;                           // (a select follows, no branch)
+            dma16(e < d ? row[i] : zero, lds + 1024 * (i0 + i));
+        }
     }
+};
+template <int D, bool V, int N> __device__ __forceinline__ void dma_rows(uint32_t addr, uint32_t i0, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
+    DmaRows<D, V, N> x;
+    x.read(addr, i0, ln);
+    x.issue(i0, ln, d, zero, lds);
 }
 
 // x where bit `at` of m is set, else -infinity
@@ -321,7 +343,17 @@ __device__ __forceinline__ uint64_t bits_of(int32_t lo, int32_t hi) {
     return lo <= 0 ? a : lo >= 64 ? 0ull : a & (~0ull << lo);
 }
 // 8 elements as they are in memory, at any element alignment
-template <typename AT> struct Eight { AT v[8]; };
+template <typename AT> struct Eight {
+    AT v[8];
+    // these, or zeros
+    __device__ __forceinline__ void keep(bool on) {
+        uint32_t w[sizeof(AT) * 2];
+        __builtin_memcpy(w, v, sizeof v);
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(AT) * 2; ++i) w[i] = on ? w[i] : 0u;
+        __builtin_memcpy(v, w, sizeof v);
+    }
+};
 template <typename AT> __device__ __forceinline__ Eight<AT> load8(const AT * p) {
     Eight<AT> x;
     __builtin_memcpy(&x, p, sizeof x);
@@ -411,7 +443,8 @@ template <int M, int DV> __device__ __forceinline__ AttnNote * attn_notes(const 
 }
 inline size_t attn_ws(uint32_t grid, uint32_t m, uint32_t dv) { return (size_t)grid * (2 * m * (dv + 2) * 4 + sizeof(AttnNote)); }
 
-// The note of workgroup w about its first item (by one thread), which begins `skip` units before w.
+// The note of workgroup w about its first item, which begins `skip` units before w (by a
+// whole wave, every lane the same).
 template <int M, int DV>
 __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32_t U, uint32_t Ge, const AttnItem & it, uint32_t skip) {
     AttnNote * n = attn_notes<M, DV>(a) + w;
@@ -434,7 +467,8 @@ template <typename AT, typename T, int M, int KT, int DV, int PW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     constexpr int V = DV / 64, R = 4;                                 // values a lane, rows a wave
     __shared__ float red[PW > 1 ? PW : 1][R][PW > 1 ? DV : 1];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = blockIdx.x;
+    const uint32_t lane = threadIdx.x & 63, w = blockIdx.x;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const AttnNote * notes = attn_notes<M, DV>(a);
     // workgroups that the main kernel had no work for left no note: their number
     // is not known here, but the note of workgroup 0 tells how many had
@@ -533,7 +567,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
             for (int k = 0; k < R; ++k) {
                 if (rbase + k >= rows || (PW > 1 && k % PW != (int)pw)) continue;
                 const uint32_t row = it.strip * M + rbase + k, tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
-                AT * out = (AT *)a.out + tok * a.o_tok + head * a.o_head;
+                AT y[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float x = o[k][v];
@@ -542,13 +576,16 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
 #pragma unroll
                         for (int i = 1; i < PW; ++i) x += red[i][k][lane * V + v];
                     }
-                    if (lane * V + v < a.dv) out[lane * V + v] = (AT)(l[k] == 0.f ? 0.f : x / l[k]);
+                    y[v] = (AT)(l[k] == 0.f ? 0.f : x / l[k]);
                 }
+                // (d_v is a multiple of 8, so of V)
+                if (lane * V < a.dv) __builtin_memcpy((AT *)a.out + tok * a.o_tok + head * a.o_head + lane * V, y, sizeof y);
             }
         }
     }
     if (!me.odd || pw) return;
-    AttnWalk<M, KT> walk(a, lane);
+    __shared__ typename AttnWalk<M, KT>::Chunk chunks[4];
+    AttnWalk<M, KT> walk(a, chunks[wave]);
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     const uint32_t u = attn_border(w, U, Ge), end = attn_border(w + 1, U, Ge);
     for (uint32_t x = u; x < end;) {                                  // items of workgroup w alone

@@ -19,7 +19,8 @@ template <int DK, int DV> struct DecShape {
     static constexpr int STAGE = 32 * (DK + DV) * 2;
     static constexpr int TAB = 2 * 256 + 512;                         // page numbers of two tiles (a DMA writes 64), row addresses of one
     static constexpr int WAVE = NST * STAGE + TAB;
-    static constexpr size_t LDS = (size_t)W * WAVE + 1088;            // and maxima, sums, flags
+    static constexpr int WALK = 6 * 256;                              // AttnWalk::Chunk
+    static constexpr size_t LDS = (size_t)W * (WAVE + WALK) + 1088;            // and maxima, sums, flags
 };
 template <int DK, int DV> constexpr int dec_threads = 64 * DecShape<DK, DV>::W;
 
@@ -30,7 +31,8 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = 16 * MT, NS = split_terms<AT, T>();
     constexpr int NK = DK / 16, NV = DV / 16, ND = NK + NV;           // DMAs of a tile
     extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q4 = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, q4 = lane >> 4;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     uint8_t * mine = sm + wave * P::WAVE;
     const uint32_t mine_at = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_at(mine)), tab_at = mine_at + NST * P::STAGE;
     float * sm_m = (float *)(sm + W * P::WAVE), * sm_l = sm_m + W * M;   // [W][M] each
@@ -43,7 +45,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     const uint32_t k_lane = l16 * (DK * 2) + (q4 ^ swz_k<DK>(l16)) * 16;
     const uint32_t v_row = 4 * q4 + (l16 >> 2);
     const uint32_t v_lane = 32 * DK * 2 + v_row * (DV * 2) + (((l16 >> 1) & 1) ^ swz_v<DV>(v_row)) * 16 + (l16 & 1) * 8;
-    AttnWalk<M, KT> walk(a, lane);
+    typedef typename AttnWalk<M, KT>::Chunk Chunk;
+    static_assert(sizeof(Chunk) == P::WALK, "chunk");
+    AttnWalk<M, KT> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units), w = blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
@@ -56,7 +60,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT + 32 * wave);   // this wave's first key
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
-        if (u == first_u && threadIdx.x == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
+        if (u == first_u && wave == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group;
 
         // ---- the strip's queries, as the second operand: column l16, elements 32 s + 8 q4 ..
@@ -69,18 +73,21 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const uint32_t r = it.strip * M + 16 * mt + l16, tok = r / a.group, head = it.kvh * a.group + r % a.group;
-            const bool real = r < rows && a.scale != 0.f;             // scale 0: every score is 0
-            const AT * q = (const AT *)a.q + (it.r0 + tok) * a.q_tok + head * a.q_head;
+            // scale 0: every score is 0.  A lane with no row or elements behind d reads the
+            // first of the item instead.
+            const bool real = r < rows && a.scale != 0.f;
+            const AT * q = (const AT *)a.q + (it.r0 + (r < rows ? tok : 0u)) * a.q_tok + (r < rows ? head : it.kvh * a.group) * a.q_head;
             rhi[mt] = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
             rlo[mt] = a.window ? it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30) : 0;
             c[mt] = a.scale == 0.f ? 1.f : a.scale * 1.4426950408889634f;
             Eight<AT> x[DK / 32];
 #pragma unroll
             for (int s = 0; s < DK / 32; ++s) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[s].v[j] = (AT)0.f;
-                if (real && 32 * s + 8 * q4 < a.dk) x[s] = load8(q + 32 * s + 8 * q4);
+                const uint32_t e = 32 * s + 8 * q4;
+                x[s] = load8(q + (e < a.dk ? e : 0u));
             }
+#pragma unroll
+            for (int s = 0; s < DK / 32; ++s) x[s].keep(real & (32 * s + 8 * q4 < a.dk));
             int ex = 0;
             if constexpr (NS == 2) {
                 // f16 terms: the row's largest element to [2^13, 2^14), and back in c
@@ -125,11 +132,13 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             const uint32_t * pgs = (const uint32_t *)(mine + NST * P::STAGE + (t & 1) * 256);
             const uint32_t own = pgs[lane & 31];
             const int32_t key = k0 + (int32_t)(lane & 31);
-            const uint32_t vm = (uint32_t)__ballot(key >= it.lo && key < it.hi && own < a.n_pages);
+            const bool in = (key >= it.lo) & (key < it.hi) & (own < a.n_pages);
+            const uint32_t vm = (uint32_t)__ballot(in);
             const uint32_t at = mine_at + stage * P::STAGE, ln = fresh(lane), tok = (uint32_t)key & a.pmask, rows_at = tab_at + 512;
             uint64_t * rows_of = (uint64_t *)(mine + NST * P::STAGE + 512);   // K rows, V rows
-            const uint64_t from = lane < 32 ? row_at(kb, own, a.k_page, tok, a.k_tok) : row_at(vb, own, a.v_page, tok, a.v_tok);
-            rows_of[lane] = (vm >> (lane & 31)) & 1 ? from : zero;
+            const bool isk = lane < 32;
+            const uint64_t from = fresh(row_at(isk ? kb : vb, own, isk ? a.k_page : a.v_page, tok, isk ? a.k_tok : a.v_tok));
+            rows_of[lane] = in ? from : zero;
             dma_rows<DK, false, NK>(rows_at, 0, ln, a.dk, zero, at);
             dma_rows<DV, true, NV>(rows_at + 256, 0, ln, a.dv, zero, at + 32 * DK * 2);
             return vm;
@@ -259,7 +268,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                 for (int d = 0; d < DV / 16; ++d)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) odd = odd || !finite(o[mt][d][i]);
-                if (q4 == 0) sm_m[wave * M + 16 * mt + l16] = m[mt];
+                sm_m[wave * M + 16 * mt + l16] = m[mt];               // (q4: the same value)
             }
             __syncthreads();
         }
@@ -271,7 +280,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
 #pragma unroll
             for (int i = 0; i < W; ++i) top = fmaxf(top, sm_m[i * M + r]);
             const float f = m[mt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[mt] - top);
-            if (q4 == 0) sm_l[wave * M + r] = l[mt] * f;
+            sm_l[wave * M + r] = l[mt] * f;
 #pragma unroll
             for (int d = 0; d < DV / 16; ++d) {
                 f32x4 v = o[mt][d];
@@ -310,10 +319,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         u += nt;
         __syncthreads();                                              // the next item's stages
     }
-    const uint32_t any = __ballot(odd) != 0;
-    if (lane == 0) sm_odd[wave] = any;
+    sm_odd[wave] = __ballot(odd) != 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (wave == 0) {
         uint32_t f = 0;
         for (int i = 0; i < W; ++i) f |= sm_odd[i];
         AttnNote * n = attn_notes<M, DV>(a) + w;

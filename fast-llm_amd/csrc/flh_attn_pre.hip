@@ -17,7 +17,8 @@ template <int DK, int DV> struct PreShape {
     static constexpr int STAGE = KT * (DK + DV) * 2;
     // a wave's page numbers of two tiles, row addresses: K of one tile, V of two
     static constexpr int TAB = 2 * 256 + 3 * 512;
-    static constexpr size_t LDS = (size_t)NST * STAGE + W * TAB + 64;
+    static constexpr int WALK = 6 * 256;                              // AttnWalk::Chunk
+    static constexpr size_t LDS = (size_t)NST * STAGE + W * (TAB + WALK) + 64;
 };
 template <int DK, int DV> constexpr int pre_threads = 64 * PreShape<DK, DV>::W;
 // waves per SIMD that the registers are cut for
@@ -47,7 +48,9 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         const uint32_t r = 8 * p + 4 * half + (l16 >> 2), pc = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
         v_lane[p] = KT * DK * 2 + r * (DV * 2) + (pc ^ swz_v<DV>(r)) * 16 + (l16 & 1) * 8;
     }
-    AttnWalk<M, KT> walk(a, lane);
+    typedef typename AttnWalk<M, KT>::Chunk Chunk;
+    static_assert(sizeof(Chunk) == P::WALK, "chunk");
+    AttnWalk<M, KT> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 64 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     // neighbours on the line share keys: they go to one XCD (workgroups are dealt
     // to the 8 XCDs in turn)
@@ -63,7 +66,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT);
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
-        if (u == first_u && threadIdx.x == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
+        if (u == first_u && wave == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group, row = it.strip * M + 32 * wave + l32, tok = row / a.group;
         const uint32_t head = it.kvh * a.group + row % a.group;
         const int32_t win = (int32_t)min(a.window, 1u << 30);
@@ -79,16 +82,19 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         v8 qf[NS][DK / 16];
         float c = a.scale == 0.f ? 1.f : a.scale * 1.4426950408889634f;   // scale * log2(e), by row
         {
-            const bool real = row < rows && a.scale != 0.f;           // scale 0: every score is 0
-            const AT * q = (const AT *)a.q + (it.r0 + tok) * a.q_tok + head * a.q_head + 8 * half;
+            // scale 0: every score is 0.  A lane with no row or elements behind d reads the
+            // first of the item instead.
+            const bool real = row < rows && a.scale != 0.f;
+            const AT * q = (const AT *)a.q + (it.r0 + (row < rows ? tok : 0u)) * a.q_tok + (row < rows ? head : it.kvh * a.group) * a.q_head;
             Eight<AT> x[DK / 16];
             float top = 0.f;
 #pragma unroll
             for (int s = 0; s < DK / 16; ++s) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[s].v[j] = (AT)0.f;
-                if (real && 16 * s + 8 * half < a.dk) x[s] = load8(q + 16 * s);
+                const uint32_t e = 16 * s + 8 * half;
+                x[s] = load8(q + (e < a.dk ? e : 0u));
             }
+#pragma unroll
+            for (int s = 0; s < DK / 16; ++s) x[s].keep(real & (16 * s + 8 * half < a.dk));
             int ex = 0;
             if constexpr (NS == 2) {
                 // f16 terms: the row's largest element to [2^13, 2^14), and back in c
@@ -124,21 +130,25 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             const uint32_t pg = (uint32_t)min(key, max(it.cap - 1, 0)) >> a.sh;
             dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (t & 1) * 256);
         };
-        // this wave's part of tile t's K rows, and where its V rows are; returns the keys
-        // that a row of the strip sees and that have a page, a bit each
-        auto issue_k = [&](uint32_t t) -> uint64_t {
+        // from tile t's page numbers, the addresses of its keys' rows (a lane a key); returns the
+        // keys that a row of the strip sees and that have a page, a bit each
+        auto find_rows = [&](uint32_t t) -> uint64_t {
             const int32_t key = key0 + (int32_t)(t * KT + lane);
             const uint32_t own = *(const uint32_t *)(tabs + (t & 1) * 256 + 4 * lane), tok = (uint32_t)key & a.pmask;
-            const bool in = key >= it.lo && key < it.hi && own < a.n_pages;
+            const bool in = (key >= it.lo) & (key < it.hi) & (own < a.n_pages);
             uint64_t * rows_of = (uint64_t *)(tabs + 512);
-            rows_of[lane] = in ? row_at(kb, own, a.k_page, tok, a.k_tok) : zero;
-            rows_of[64 + 64 * (t & 1) + lane] = in ? row_at(vb, own, a.v_page, tok, a.v_tok) : zero;
-            dma_rows<DK, false, NK>(tab_at + 512, wave * NK, fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE);
+            const uint64_t kr = fresh(row_at(kb, own, a.k_page, tok, a.k_tok)), vr = fresh(row_at(vb, own, a.v_page, tok, a.v_tok));
+            rows_of[lane] = in ? kr : zero;
+            rows_of[64 + 64 * (t & 1) + lane] = in ? vr : zero;
             return __ballot(in);
         };
-        auto issue_v = [&](uint32_t t) {
-            dma_rows<DV, true, NV>(tab_at + 1024 + 512 * (t & 1), wave * NV, fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2);
-        };
+        // this wave's part of tile t's rows
+        DmaRows<DK, false, NK> dk;
+        DmaRows<DV, true, NV> dv;
+        auto read_k = [&]() { dk.read(tab_at + 512, wave * NK, fresh(lane)); };
+        auto read_v = [&](uint32_t t) { dv.read(tab_at + 1024 + 512 * (t & 1), wave * NV, fresh(lane)); };
+        auto issue_k = [&](uint32_t t) { dk.issue(wave * NK, fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE); };
+        auto issue_v = [&](uint32_t t) { dv.issue(wave * NV, fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2); };
 
         float m, l;
         f32x16 o[DB];
@@ -160,8 +170,8 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                 }
         };
         // s: a tile's scores -> sums; the scores of the next one (K at `next`) are
-        // multiplied meanwhile and end up in s
-        auto tile = [&](int32_t k0, uint64_t vm, uint32_t at, uint32_t next) {
+        // multiplied meanwhile and end up in s; `midway` is called on the way
+        auto tile = [&](int32_t k0, uint64_t vm, uint32_t at, uint32_t next, auto && midway) {
             if (!(vm == ~0ull && k0 >= all_lo && k0 + KT <= all_hi)) {
                 const uint64_t see = fresh((vm & bits_of(rlo - k0, rhi - k0)) >> (4 * half));
 #pragma unroll
@@ -192,16 +202,32 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             // step, the first steps with the weights of the other 32 keys.
             float sum = 0.f;
             v8 pf[KT / 16][NS];
-            auto weights = [&](int e0, int e1) {                      // of the lane's elements e0 .. e1
+            // a weight in three pieces of work, which are put a step apart (the results of
+            // one come late for the next)
+            auto arg = [&](int e0, int e1) {
+#pragma unroll
+                for (int e = e0; e < e1; ++e) s[e >> 4][e & 15] = fmaf(s[e >> 4][e & 15], c, -base);
+            };
+            auto exps = [&](int e0, int e1) {
+#pragma unroll
+                for (int e = e0; e < e1; ++e) s[e >> 4][e & 15] = __builtin_amdgcn_exp2f(s[e >> 4][e & 15]);
+            };
+            auto pack = [&](int e0, int e1) {
 #pragma unroll
                 for (int e = e0; e < e1; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], c, -base)) * weight_unit<T>();
+                    const float p = s[e >> 4][e & 15] * weight_unit<T>();
                     sum += p;
                     T h[NS];
                     split<T, NS>(p, h);
 #pragma unroll
                     for (int t2 = 0; t2 < NS; ++t2) pf[e >> 3][t2][e & 7] = h[t2];
                 }
+            };
+            // step i of n of the 16 weights from e0 on
+            auto weights = [&](int i, int n, int e0) {
+                const int q = n - 2;
+                if (i < q) exps(e0 + 16 * i / q, e0 + 16 * (i + 1) / q);
+                if (i >= 1 && i <= q) pack(e0 + 16 * (i - 1) / q, e0 + 16 * i / q);
             };
             f32x16 nx[2];
 #pragma unroll
@@ -235,7 +261,9 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                 if (i + 3 == NF) ld_v(0);
 #pragma unroll
                 for (int t2 = NS - 1; t2 >= 0; --t2) nx[i & 1] = mma32(kf[i & 3], qf[t2][i >> 1], nx[i & 1]);
-                weights(16 * i / NF, 16 * (i + 1) / NF);
+                arg(32 * i / NF, 32 * (i + 1) / NF);
+                if (i) weights(i - 1, NF - 1, 0);
+                if (i == NF / 2) midway();
             }
 #pragma unroll
             for (int step = 0; step < VSTEPS; ++step) {
@@ -251,7 +279,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                         // the first half of the steps' products carry the weights 16 .. 31
                         constexpr int H = VSTEPS / 2 * NS * DC;
                         const int i = (step * NS + (NS - 1 - t2)) * DC + d;
-                        if (i < H) weights(16 + 16 * i / H, 16 + 16 * (i + 1) / H);
+                        if (i < H) weights(i, H, 16);
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -269,28 +297,39 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             // K runs a tile ahead of V: stage t & 1 has K of tile t, then of t + 2, while V
             // of tile t is still needed.  Every wave brings its part at the begin of a round,
             // behind the barrier that tells that the round before is over, and waits
-            // for it at the begin of the next.
-            uint64_t vm0, vm1 = 0, vm2 = 0;
+            // for it at the begin of the next.  Row addresses are made a round before.
+            uint64_t vm0, vm1, vm2, vm3 = 0;
             issue_tab(0);
             issue_tab(1);
             wait_vm<0>();
-            vm0 = issue_k(0);
+            vm0 = find_rows(0);
+            read_k();
+            read_v(0);
+            issue_k(0);
             issue_v(0);
-            if (nt > 1) vm1 = issue_k(1);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (the page numbers have been read)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (page numbers and addresses have been read)
             issue_tab(2);
+            vm1 = find_rows(1);
+            read_k();
+            issue_k(1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            issue_tab(3);
             asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            vm2 = find_rows(2);
             if (here) scores(sm_at, s);
             for (uint32_t t = 0; t < nt; ++t) {
+                read_k();                                             // of tile t + 2
+                read_v(t + 1);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (t + 2 < nt) {
-                    vm2 = issue_k(t + 2);
-                    issue_tab(t + 3);
-                }
+                if (t + 2 < nt) issue_k(t + 2);
                 if (t + 1 < nt) issue_v(t + 1);
-                if (here) tile(key0 + (int32_t)(t * KT), vm0, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE);
+                if (t + 4 < nt) issue_tab(t + 4);
+                auto midway = [&]() { vm3 = find_rows(t + 3); };
+                if (here) tile(key0 + (int32_t)(t * KT), vm0, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE, midway);
+                else midway();
                 vm0 = vm1;
                 vm1 = vm2;
+                vm2 = vm3;
             }
             wait_vm<0>();
             odd = odd || !finite(l);
@@ -333,10 +372,9 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         u += nt;
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the next item's stages
     }
-    const uint32_t any = __ballot(odd) != 0;
-    if (lane == 0) sm_odd[wave] = any;
+    sm_odd[wave] = __ballot(odd) != 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (wave == 0) {
         uint32_t f = 0;
         for (int i = 0; i < W; ++i) f |= sm_odd[i];
         AttnNote * n = attn_notes<M, DV>(a) + w;

@@ -210,7 +210,7 @@ struct RopeArgs {
     const int32_t * pos; const uint32_t * slot;
     uint64_t q_tok, q_head, qo_tok, qo_head, k_tok, k_head, v_tok, v_head;
     uint64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head;
-    uint32_t n_tok, n_head, n_kv, d, dv, n_rot, first, halves, pos_stride, n_slot, sh;
+    uint32_t n_tok, tok0, n_head, n_kv, d, dv, n_rot, first, halves, pos_stride, n_slot, sh;
 };
 struct AttnArgs {
     const void * q; void * out; const void * k; const void * v;

@@ -184,51 +184,168 @@ __device__ __forceinline__ void rope_cs(const RopePair & t, const int32_t * pos,
     s = q & 2 ? -b : b;
 }
 
-template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+template <int N, typename T> __device__ __forceinline__ Vec<T, N> ld_vec(const T * p) { return *(const Vec<T, N> *)p; }
+template <int N, typename T> __device__ __forceinline__ void st_vec(T * p, const float * y) {
+    Vec<T, N> o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o.v[i] = (T)y[i];
+    *(Vec<T, N> *)p = o;
+}
 
-// One thread per pair or element: token blockIdx.x, the heads of q, k and v one
-// after the other.
-template <typename AT, typename CT>
-__global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
-    const uint32_t tok = blockIdx.x, nk = a.kc ? a.n_kv : 0, P = a.rot ? a.n_rot / 2 : 0;
+// Token tok0 + blockIdx.x; its heads of q and then k are cut into units of N pairs or
+// 2N other elements (the last may have N), its heads of v into units of N, and
+// the workgroups of blockIdx.y share them.  Nothing is used twice but the
+// angles: a workgroup makes each once, behind the loads of its threads' first
+// units, and every head reads them from LDS.
+struct RopeUnits {
+    uint32_t pu, u, n, step_h, step_e;     // a head's pair units and all its units, their number, and a step in (head, unit)
+};
+constexpr uint32_t ROPE_T = 256;
+template <typename AT, typename CT, int N>
+__global__ __launch_bounds__(ROPE_T) void k_rope(RopeArgs a, RopeUnits ru) {
+    __shared__ float2 cs[512];
+    constexpr int B = 2;                   // units in flight
+    const uint32_t tok = a.tok0 + blockIdx.x, nk = a.kc ? a.n_kv : 0, P = a.rot ? a.n_rot / 2 : 0;
+    const uint32_t first = blockIdx.y * ROPE_T + threadIdx.x, step = gridDim.y * ROPE_T;
     const uint32_t slot = nk ? a.slot[tok] : 0;
     const bool live = nk && slot < a.n_slot;
     const uint64_t page = slot >> a.sh, off = slot & ((1u << a.sh) - 1u);
-    const uint32_t rest = a.d - 2 * P, per = P + rest;            // units of a head: pairs, then single elements
-    for (uint32_t u = threadIdx.x; u < per * (a.n_head + nk); u += 256) {
-        const uint32_t h = u / per, e = u % per;
-        const bool isq = h < a.n_head;
-        if (!isq && !live) continue;
-        const AT * x = isq ? (const AT *)a.q + tok * a.q_tok + h * a.q_head : (const AT *)a.k + tok * a.k_tok + (h - a.n_head) * a.k_head;
-        AT * yq = (AT *)a.qo + tok * a.qo_tok + h * a.qo_head;
-        CT * yk = (CT *)a.kc + page * a.kc_page + off * a.kc_tok + (h - a.n_head) * a.kc_head;
-        if (e < P) {
-            const uint32_t i = a.first + (a.halves ? e : 2 * e), j = i + (a.halves ? P : 1);
-            float c, s;
-            rope_cs(a.rot[e], a.pos, a.pos_stride, tok, c, s);
-            const float v = to_f(x[i]), w = to_f(x[j]);
-            const float ya = v * c - w * s, yb = v * s + w * c;
-            if (isq) { yq[i] = (AT)ya; yq[j] = (AT)yb; }
-            else { yk[i] = (CT)ya; yk[j] = (CT)yb; }
-        } else {
-            const uint32_t k = e - P, i = k < a.first || !P ? k : k + 2 * P;
-            if (isq) yq[i] = x[i];
-            else yk[i] = (CT)to_f(x[i]);
+    const AT * q = (const AT *)a.q + tok * a.q_tok, * k = (const AT *)a.k + tok * a.k_tok;
+    AT * qo = (AT *)a.qo + tok * a.qo_tok;
+    CT * kc = (CT *)a.kc + page * a.kc_page + off * a.kc_tok;
+
+    uint32_t h = first / ru.u, e = first - h * ru.u;
+    for (uint32_t at = first, round = 0; round == 0 || at - threadIdx.x < ru.n; ++round) {
+        Vec<AT, N> x[B], w[B];
+        uint32_t hs[B], es[B], is[B], js[B];
+        bool on[B], two[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            on[b] = at < ru.n && (h < a.n_head || live);
+            two[b] = true;
+            hs[b] = h; es[b] = e;
+            if (e < ru.pu) {
+                is[b] = a.first + (a.halves ? e * N : e * 2 * N);
+                js[b] = is[b] + (a.halves ? P : N);
+            } else {
+                const uint32_t r = (e - ru.pu) * 2 * N;          // among the elements that are not turned
+                is[b] = r < a.first || !P ? r : r + 2 * P;
+                js[b] = r + N < a.first || !P ? r + N : r + N + 2 * P;
+                two[b] = r + N < a.d - 2 * P;
+            }
+            if (on[b]) {
+                const AT * src = h < a.n_head ? q + h * a.q_head : k + (h - a.n_head) * a.k_head;
+                x[b] = ld_vec<N>(src + is[b]);
+                if (two[b]) w[b] = ld_vec<N>(src + js[b]);
+            }
+            at += step; h += ru.step_h; e += ru.step_e;
+            if (e >= ru.u) { e -= ru.u; ++h; }
+        }
+        if (round == 0) {
+            for (uint32_t i = threadIdx.x; i < P; i += ROPE_T)
+                rope_cs(a.rot[i], a.pos, a.pos_stride, tok, cs[i].x, cs[i].y);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (!on[b]) continue;
+            float y[N], z[N];
+            if (es[b] < ru.pu) {
+                const float2 * t = cs + es[b] * N;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float c = t[i].x, s = t[i].y;
+                    // halves: pair i is (x[i], w[i]); pairs: the 2N elements x, w one after the other
+                    const float v = (float)(a.halves ? x[b].v[i] : 2 * i < N ? x[b].v[2 * i % N] : w[b].v[2 * i % N]);
+                    const float u = (float)(a.halves ? w[b].v[i] : 2 * i + 1 < N ? x[b].v[(2 * i + 1) % N] : w[b].v[(2 * i + 1) % N]);
+                    const float ya = v * c - u * s, yb = v * s + u * c;
+                    if (a.halves) {
+                        y[i] = ya;
+                        z[i] = yb;
+                    } else if constexpr (N == 1) {
+                        y[0] = ya;
+                        z[0] = yb;
+                    } else if (2 * i < N) {
+                        y[2 * i % N] = ya;
+                        y[(2 * i + 1) % N] = yb;
+                    } else {
+                        z[2 * i % N] = ya;
+                        z[(2 * i + 1) % N] = yb;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    y[i] = (float)x[b].v[i];
+                    z[i] = (float)w[b].v[i];
+                }
+            }
+            if (hs[b] < a.n_head) {
+                AT * d = qo + hs[b] * a.qo_head;
+                st_vec<N>(d + is[b], y);
+                if (two[b]) st_vec<N>(d + js[b], z);
+            } else {
+                CT * d = kc + (hs[b] - a.n_head) * a.kc_head;
+                st_vec<N>(d + is[b], y);
+                if (two[b]) st_vec<N>(d + js[b], z);
+            }
         }
     }
     if (!live) return;
-    for (uint32_t u = threadIdx.x; u < nk * a.dv; u += 256) {
-        const uint32_t h = u / a.dv, i = u % a.dv;
-        ((CT *)a.vc)[page * a.vc_page + off * a.vc_tok + h * a.vc_head + i] =
-            (CT)to_f(((const AT *)a.v)[tok * a.v_tok + h * a.v_head + i]);
+    const uint32_t vu = a.dv / N;
+    const AT * v = (const AT *)a.v + tok * a.v_tok;
+    CT * vc = (CT *)a.vc + page * a.vc_page + off * a.vc_tok;
+    for (uint32_t at = first; at < nk * vu; at += step) {
+        const uint32_t hv = at / vu, i = (at - hv * vu) * N;
+        const Vec<AT, N> x = ld_vec<N>(v + hv * a.v_head + i);
+        float y[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] = (float)x.v[j];
+        st_vec<N>(vc + hv * a.vc_head + i, y);
     }
 }
 
+template <typename AT, typename CT, int N>
+static int rope_n(RopeArgs a, hipStream_t s) {
+    const uint32_t P = a.rot ? a.n_rot / 2 : 0, nk = a.kc ? a.n_kv : 0, rest = a.d - 2 * P;
+    RopeUnits ru;
+    ru.pu = P / N;
+    ru.u = ru.pu + (rest + 2 * N - 1) / (2 * N);
+    ru.n = ru.u * (a.n_head + nk);
+    const uint32_t most = (uint32_t)((std::max<uint64_t>(ru.n, nk * a.dv / N) + ROPE_T - 1) / ROPE_T);
+    const uint32_t parts = std::max(1u, std::min(most, 512 / a.n_tok));
+    ru.step_h = parts * ROPE_T / ru.u;
+    ru.step_e = parts * ROPE_T % ru.u;
+    constexpr uint32_t MOST_TOK = 1u << 22;            // of a launch: its threads are counted in 32 bits
+    for (uint64_t t = 0; t < a.n_tok; t += MOST_TOK) {
+        a.tok0 = (uint32_t)t;
+        hipLaunchKernelGGL((k_rope<AT, CT, N>), dim3(std::min(a.n_tok - a.tok0, MOST_TOK), parts), dim3(ROPE_T), 0, s, a, ru);
+        if (int rc = hip_check(hipGetLastError(), "k_rope launch")) return rc;
+    }
+    return FLH_OK;
+}
+// whether every head of every token allows units of n elements
+static bool rope_fits(const RopeArgs & a, uint32_t el, uint32_t n) {
+    auto fit = [n](const void * p, uint32_t e, uint64_t tok, uint64_t head) {
+        return (uintptr_t)p % (e * n) == 0 && tok % n == 0 && head % n == 0;
+    };
+    const uint32_t P = a.rot ? a.n_rot / 2 : 0;
+    if (P % n || (P && a.first % n) || a.d % n) return false;
+    if (a.n_head && !(fit(a.q, el, a.q_tok, a.q_head) && fit(a.qo, el, a.qo_tok, a.qo_head))) return false;
+    return !a.kc || (fit(a.k, el, a.k_tok, a.k_head) && fit(a.v, el, a.v_tok, a.v_head) && a.dv % n == 0 &&
+                     fit(a.kc, 2, a.kc_page | a.kc_tok, a.kc_head) && fit(a.vc, 2, a.vc_page | a.vc_tok, a.vc_head));
+}
+// Units of 16 bytes where alignment allows them, else single elements.
+template <typename AT, typename CT>
+static int rope_c(const RopeArgs & a, hipStream_t s) {
+    constexpr int N = 16 / sizeof(AT);
+    if (rope_fits(a, sizeof(AT), N)) return rope_n<AT, CT, N>(a, s);
+    return rope_n<AT, CT, 1>(a, s);
+}
 template <typename AT>
 static int rope_go(const RopeArgs & a, uint32_t cdt, hipStream_t s) {
-    if (cdt == FLH_DT_BF16) hipLaunchKernelGGL((k_rope<AT, __bf16>), dim3(a.n_tok), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rope<AT, _Float16>), dim3(a.n_tok), dim3(256), 0, s, a);
-    return hip_check(hipGetLastError(), "k_rope launch");
+    return cdt == FLH_DT_BF16 ? rope_c<AT, __bf16>(a, s) : rope_c<AT, _Float16>(a, s);
 }
 int launch_rope(const RopeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s) {
     if (dtype == FLH_DT_F32) return rope_go<float>(a, cache_dtype, s);

@@ -185,3 +185,33 @@ def test_append_values_past_the_range(flh, gpu):
     flh.rope_kv_append(None, cache.c, p, gpu)
     for c in cache.pull():
         assert torch.equal(torch.nan_to_num(c[0, 2, 0].float(), nan=9.0), torch.nan_to_num(x[0].half().float(), nan=9.0))
+
+
+# heads whose unturned part is cut by the turned one at odd multiples of the units
+# of 16 bytes, and many heads of few tokens (shared by several workgroups)
+UNITS = [("F32", 5, 3, 76, 64, 4, "HALVES", 1, 1000, 0, 0), ("F32", 5, 3, 76, 64, 8, "PAIRS", 2, 1000, 4, 4),
+         ("F32", 3, 700, 12, 8, 4, "PAIRS", 1, 1000, 0, 0), ("F16", 4, 3, 88, 64, 8, "HALVES", 1, 1000, 0, 0),
+         ("BF16", 4, 3, 104, 64, 24, "PAIRS", 1, 1000, 8, 8), ("BF16", 1, 300, 136, 16, 120, "PAIRS", 3, 1000, 0, 8),
+         ("F16", 2, 65, 16, 16, 0, "PAIRS", 1, 1000, 0, 0), ("F32", 513, 33, 132, 128, 0, "HALVES", 1, 1000, 0, 0)]
+
+
+@pytest.mark.parametrize("case", UNITS)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rope_units(flh, gpu, case, in_place):
+    test_rope(flh, gpu, *case, in_place)
+
+
+def test_rope_more_tokens_than_a_launch(flh, gpu):
+    """2^24 + 5 tokens of one pair: rows at both ends and around 2^22 and 2^24."""
+    n = (1 << 24) + 5
+    x = torch.arange(2 * n, dtype=torch.float32).remainder_(251).to(torch.float16)
+    pos = (torch.arange(n, dtype=torch.int64) * 7919 % 100003).to(torch.int32)
+    bx, bp = put(flh, gpu, x), put(flh, gpu, pos)
+    t = flh.RopeTable(2, base=10.0)
+    flh.rope(t, flh.Dtype.F16, bx, 2, 2, bx, 2, 2, n, 1, 2, bp, n, gpu)
+    got = get(bx, x, gpu)
+    rows = np.concatenate([np.arange(c - 5, c + 5) for c in (5, 1 << 22, 1 << 23, 3 << 22, 1 << 24)])
+    want, mag = turned(x.reshape(n, 1, 2)[rows].double().numpy(), pos[rows][None].numpy(), np.array([1.0]), [0], 0, True)
+    err = np.abs(got.reshape(n, 1, 2)[rows].double().numpy() - want)
+    assert (err <= bound(want, mag, "F16")).all(), err.max()
+    t.close()

@@ -304,32 +304,43 @@ template <typename AT> __device__ __forceinline__ void store4(AT * p, float a, f
 }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
-// A wave's N DMAs, from number i0 on, of a tile's rows.  The addresses of the keys'
-// rows (g_attn_zero for a key that is not there) stand in LDS, a key a lane wrote
-// them; lane ln of DMA i brings piece e of row r.  Pieces behind d are zeros.
+// A wave's N DMAs of a tile's rows (all, or from a multiple of 16 on; row numbers here
+// count from there).  The addresses of the keys' rows (g_attn_zero for a key that is not
+// there) stand in LDS, a key a lane wrote them; lane ln of DMA i brings one piece of row
+// index(i, ln).  Pieces behind d are zeros.
 template <int D, bool V, int N> struct DmaRows {
     uint64_t row[N];
-    __device__ __forceinline__ static uint32_t index(uint32_t i, uint32_t ln) { return (i * 64 + ln) / (D / 8); }
-    __device__ __forceinline__ void read(uint32_t addr, uint32_t i0, uint32_t ln) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) row[i] = *FLH_LDS(uint64_t, addr + 8 * index(i0 + i, ln));
-    }
-    __device__ __forceinline__ void issue(uint32_t i0, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
+    __device__ __forceinline__ static uint32_t swz(uint32_t r) { return V ? swz_v<V ? D : 64>(r) : swz_k<D>(r); }
+    __device__ __forceinline__ void read(uint32_t addr, uint32_t ln) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t r = index(i0 + i, ln), p = ((i0 + i) * 64 + ln) % (D / 8);
-            uint32_t e;
-            if constexpr (V) e = (p ^ swz_v<D>(r)) * 8;
-            else e = (p ^ swz_k<D>(r)) * 8;
-            row[i] = fresh(row[i]) + 2 * e;                           // (a select follows, no branch)
-            dma16(e < d ? row[i] : zero, lds + 1024 * (i0 + i));
+            if constexpr ((D & (D - 1)) == 0) row[i] = *FLH_LDS(uint64_t, addr + 8 * (ln / (D / 8)) + 8 * i * (512 / D));
+            else row[i] = *FLH_LDS(uint64_t, addr + 8 * ((i * 64 + ln) / (D / 8)));
         }
     }
+    // (the piece's place in the row: the swizzle moves bits of the row number, so the
+    // lane's share and the DMA's, which is a constant, come apart)
+    __device__ __forceinline__ void issue(uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
+        uint64_t at[N];
+        uint32_t e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr ((D & (D - 1)) == 0) e[i] = ((ln % (D / 8)) ^ swz(ln / (D / 8)) ^ swz(i * (512 / D))) * 16;
+            else e[i] = ((i * 64 + ln) % (D / 8) ^ swz((i * 64 + ln) / (D / 8))) * 16;
+            at[i] = fresh(row[i] + e[i]);                             // (a select follows, no branch)
+        }
+        if (d != D) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) at[i] = e[i] < 2 * d ? at[i] : zero;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) dma16(at[i], lds + 1024 * i);
+    }
 };
-template <int D, bool V, int N> __device__ __forceinline__ void dma_rows(uint32_t addr, uint32_t i0, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
+template <int D, bool V, int N> __device__ __forceinline__ void dma_rows(uint32_t addr, uint32_t ln, uint32_t d, uint64_t zero, uint32_t lds) {
     DmaRows<D, V, N> x;
-    x.read(addr, i0, ln);
-    x.issue(i0, ln, d, zero, lds);
+    x.read(addr, ln);
+    x.issue(ln, d, zero, lds);
 }
 
 // x where bit `at` of m is set, else -infinity
@@ -371,7 +382,7 @@ inline int attn_dims(const AttnArgs & a) {
     return a.dk <= 64 && a.dv <= 64 ? 0 : a.dk <= 128 && a.dv <= 128 ? 1 : a.dk <= 192 && a.dv <= 128 ? 2 : 3;
 }
 AttnPlan attn_dec_plan(const AttnArgs & a);
-AttnPlan attn_pre_plan(const AttnArgs & a);
+AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype);
 int launch_attn_dec(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 

@@ -139,8 +139,8 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             const bool isk = lane < 32;
             const uint64_t from = fresh(row_at(isk ? kb : vb, own, isk ? a.k_page : a.v_page, tok, isk ? a.k_tok : a.v_tok));
             rows_of[lane] = in ? from : zero;
-            dma_rows<DK, false, NK>(rows_at, 0, ln, a.dk, zero, at);
-            dma_rows<DV, true, NV>(rows_at + 256, 0, ln, a.dv, zero, at + 32 * DK * 2);
+            dma_rows<DK, false, NK>(rows_at, ln, a.dk, zero, at);
+            dma_rows<DV, true, NV>(rows_at + 256, ln, a.dv, zero, at + 32 * DK * 2);
             return vm;
         };
 

@@ -15,17 +15,18 @@ template <int DK, int DV> struct PreShape {
     static constexpr int W = 4;                                       // waves
     static constexpr int M = 32 * W, KT = 64, NST = 2;
     static constexpr int STAGE = KT * (DK + DV) * 2;
-    // a wave's page numbers of two tiles, row addresses: K of one tile, V of two
-    static constexpr int TAB = 2 * 256 + 3 * 512;
+    // a wave's page numbers of 4 tiles, 16 keys each; row addresses of 8 tiles' keys, K and V
+    static constexpr int TAB = 256 + 2 * 1024;
     static constexpr int WALK = 6 * 256;                              // AttnWalk::Chunk
-    static constexpr size_t LDS = (size_t)NST * STAGE + W * (TAB + WALK) + 64;
+    static constexpr size_t LDS = (size_t)NST * STAGE + W * (TAB + WALK) + 128;
 };
 template <int DK, int DV> constexpr int pre_threads = 64 * PreShape<DK, DV>::W;
-// waves per SIMD that the registers are cut for
-template <typename AT, typename T, int DK, int DV> constexpr int pre_waves = DK + DV <= 256 && split_terms<AT, T>() == 1 ? 2 : 1;
+// waves per SIMD that the registers are cut for, and so workgroups per CU: the grid is what
+// runs at once, else some workgroups of even shares start when others are done
+constexpr int pre_waves(bool split, int dk, int dv) { return dk + dv <= (split ? 128 : 256) ? 2 : 1; }
 
 template <typename AT, typename T, int DK, int DV>
-__global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) void k_attn_pre(AttnArgs a) {
+__global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>() > 1, DK, DV)) void k_attn_pre(AttnArgs a) {
     typedef PreShape<DK, DV> P;
     typedef typename VecOf<T>::v8 v8;
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = P::M, NS = split_terms<AT, T>();
@@ -38,6 +39,8 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
     uint8_t * tabs = sm + NST * P::STAGE + wave * P::TAB;
     const uint32_t tab_at = sm_at + NST * P::STAGE + wave * P::TAB;
     uint32_t * sm_odd = (uint32_t *)(sm + NST * P::STAGE + W * P::TAB);   // [W]
+    // keys of 8 tiles that have a page and that a row of the strip sees: a bit each
+    uint64_t * sm_live = (uint64_t *)(sm_odd + 16);
 
     // the lane's addresses in a stage: K rows l32 (+ 32 b), pieces half (+ 2 d); V
     // rows 4 half + l16 / 4 + 8 p (+ 16 k), pieces of 16 columns by lane bit 4 (+ 4 d)
@@ -50,7 +53,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
     }
     typedef typename AttnWalk<M, KT>::Chunk Chunk;
     static_assert(sizeof(Chunk) == P::WALK, "chunk");
-    AttnWalk<M, KT> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 64 + wave * P::WALK));
+    AttnWalk<M, KT> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 128 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     // neighbours on the line share keys: they go to one XCD (workgroups are dealt
     // to the 8 XCDs in turn)
@@ -125,34 +128,39 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
         const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
         const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
         const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
-        auto issue_tab = [&](uint32_t t) {                            // page numbers of tile t: lane l's key
-            const int32_t key = key0 + (int32_t)(t * KT + lane);
-            const uint32_t pg = (uint32_t)min(key, max(it.cap - 1, 0)) >> a.sh;
-            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (t & 1) * 256);
+        // The rows of four tiles are found together, 16 keys of each by the wave that brings
+        // them (lane l: key l % 16 of tile 4 g + l / 16).
+        auto key_of = [&](uint32_t g) { return key0 + (int32_t)((4 * g + (lane >> 4)) * KT + 16 * wave + l16); };
+        auto issue_tab = [&](uint32_t g) {                            // page numbers
+            const uint32_t pg = (uint32_t)min(key_of(g), max(it.cap - 1, 0)) >> a.sh;
+            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at);
         };
-        // from tile t's page numbers, the addresses of its keys' rows (a lane a key); returns the
-        // keys that a row of the strip sees and that have a page, a bit each
-        auto find_rows = [&](uint32_t t) -> uint64_t {
-            const int32_t key = key0 + (int32_t)(t * KT + lane);
-            const uint32_t own = *(const uint32_t *)(tabs + (t & 1) * 256 + 4 * lane), tok = (uint32_t)key & a.pmask;
+        auto find_rows = [&](uint32_t g) {                            // from them, row addresses and live keys
+            const int32_t key = key_of(g);
+            const uint32_t own = *(const uint32_t *)(tabs + 4 * lane), tok = (uint32_t)key & a.pmask;
             const bool in = (key >= it.lo) & (key < it.hi) & (own < a.n_pages);
-            uint64_t * rows_of = (uint64_t *)(tabs + 512);
+            uint64_t * rows_of = (uint64_t *)(tabs + 256) + 64 * (g & 1) + lane;
             const uint64_t kr = fresh(row_at(kb, own, a.k_page, tok, a.k_tok)), vr = fresh(row_at(vb, own, a.v_page, tok, a.v_tok));
-            rows_of[lane] = in ? kr : zero;
-            rows_of[64 + 64 * (t & 1) + lane] = in ? vr : zero;
-            return __ballot(in);
+            rows_of[0] = in ? kr : zero;
+            rows_of[128] = in ? vr : zero;
+            // (the 16 lanes of a tile write the same)
+            ((uint16_t *)(sm_live + 4 * (g & 1) + (lane >> 4)))[wave] = (uint16_t)(__ballot(in) >> (lane & 48));
+        };
+        auto live = [&](uint32_t t) -> uint64_t {                     // of tile t
+            const uint64_t v = sm_live[t & 7];
+            return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
         };
         // this wave's part of tile t's rows
         DmaRows<DK, false, NK> dk;
         DmaRows<DV, true, NV> dv;
-        auto read_k = [&]() { dk.read(tab_at + 512, wave * NK, fresh(lane)); };
-        auto read_v = [&](uint32_t t) { dv.read(tab_at + 1024 + 512 * (t & 1), wave * NV, fresh(lane)); };
-        auto issue_k = [&](uint32_t t) { dk.issue(wave * NK, fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE); };
-        auto issue_v = [&](uint32_t t) { dv.issue(wave * NV, fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2); };
+        auto read_k = [&](uint32_t t) { dk.read(tab_at + 256 + 128 * (t & 7), fresh(lane)); };
+        auto read_v = [&](uint32_t t) { dv.read(tab_at + 1280 + 128 * (t & 7), fresh(lane)); };
+        auto issue_k = [&](uint32_t t) { dk.issue(fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE + 1024 * NK * wave); };
+        auto issue_v = [&](uint32_t t) { dv.issue(fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2 + 1024 * NV * wave); };
 
         float m, l;
         f32x16 o[DB];
-        f32x16 s[2];                                                  // scores of the tile at hand
+        f32x16 sa[2], sb[2];                                          // scores of the tile at hand and the next
         // the tile at `at` times the queries, in steps of 16 elements
         auto scores = [&](uint32_t at, f32x16 (&x)[2]) {
             const uint32_t ka = fresh(at + k_lane);
@@ -170,8 +178,8 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                 }
         };
         // s: a tile's scores -> sums; the scores of the next one (K at `next`) are
-        // multiplied meanwhile and end up in s; `midway` is called on the way
-        auto tile = [&](int32_t k0, uint64_t vm, uint32_t at, uint32_t next, auto && midway) {
+        // multiplied meanwhile into nx; `midway` is called on the way
+        auto tile = [&](int32_t k0, uint64_t vm, uint32_t at, uint32_t next, f32x16 (&s)[2], f32x16 (&nx)[2], auto && midway) {
             if (!(vm == ~0ull && k0 >= all_lo && k0 + KT <= all_hi)) {
                 const uint64_t see = fresh((vm & bits_of(rlo - k0, rhi - k0)) >> (4 * half));
 #pragma unroll
@@ -229,7 +237,6 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
                 if (i < q) exps(e0 + 16 * i / q, e0 + 16 * (i + 1) / q);
                 if (i >= 1 && i <= q) pack(e0 + 16 * (i - 1) / q, e0 + 16 * i / q);
             };
-            f32x16 nx[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -284,8 +291,6 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             }
             __builtin_amdgcn_sched_barrier(0);
             l += sum;
-            s[0] = nx[0];
-            s[1] = nx[1];
         };
         {
             m = -INFINITY;
@@ -297,39 +302,37 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), (pre_waves<AT, T, DK, DV>)) 
             // K runs a tile ahead of V: stage t & 1 has K of tile t, then of t + 2, while V
             // of tile t is still needed.  Every wave brings its part at the begin of a round,
             // behind the barrier that tells that the round before is over, and waits
-            // for it at the begin of the next.  Row addresses are made a round before.
-            uint64_t vm0, vm1, vm2, vm3 = 0;
+            // for it at the begin of the next.  Rows of the next four tiles are found in
+            // round 1 of four, from page numbers asked for in round 0.
             issue_tab(0);
-            issue_tab(1);
             wait_vm<0>();
-            vm0 = find_rows(0);
-            read_k();
+            find_rows(0);
+            read_k(0);
             read_v(0);
             issue_k(0);
             issue_v(0);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (page numbers and addresses have been read)
-            issue_tab(2);
-            vm1 = find_rows(1);
-            read_k();
+            read_k(1);
             issue_k(1);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            issue_tab(3);
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-            vm2 = find_rows(2);
-            if (here) scores(sm_at, s);
-            for (uint32_t t = 0; t < nt; ++t) {
-                read_k();                                             // of tile t + 2
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            uint64_t vm = live(0);
+            if (here) scores(sm_at, sa);
+            auto round = [&](uint32_t t, f32x16 (&s)[2], f32x16 (&nx)[2]) {
+                read_k(t + 2);
                 read_v(t + 1);
+                const uint64_t now = vm;
+                vm = live(t + 1);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (t + 2 < nt) issue_k(t + 2);
                 if (t + 1 < nt) issue_v(t + 1);
-                if (t + 4 < nt) issue_tab(t + 4);
-                auto midway = [&]() { vm3 = find_rows(t + 3); };
-                if (here) tile(key0 + (int32_t)(t * KT), vm0, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE, midway);
+                if ((t & 3) == 0 && t + 4 < nt) issue_tab(t / 4 + 1);
+                auto midway = [&]() { if ((t & 3) == 1 && t + 3 < nt) find_rows(t / 4 + 1); };
+                if (here) tile(key0 + (int32_t)(t * KT), now, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE, s, nx, midway);
                 else midway();
-                vm0 = vm1;
-                vm1 = vm2;
-                vm2 = vm3;
+            };
+            for (uint32_t t = 0; t < nt; ++t) {
+                round(t, sa, sb);
+                sa[0] = sb[0];
+                sa[1] = sb[1];
             }
             wait_vm<0>();
             odd = odd || !finite(l);
@@ -401,23 +404,23 @@ template <typename AT, typename T> int dims(const AttnArgs & a, hipStream_t s) {
         default: return go<AT, T, 256, 256>(a, s);
     }
 }
-template <int DK, int DV> void shape(AttnPlan & p, uint32_t & per_cu) {
+template <int DK, int DV> void shape(AttnPlan & p, bool split) {
+    static_assert(pre_waves(false, DK, DV) * PreShape<DK, DV>::LDS <= 160 * 1024, "workgroups per CU");
     p.dv = DV;
     p.m = PreShape<DK, DV>::M;
-    per_cu = (uint32_t)(160 * 1024 / PreShape<DK, DV>::LDS);
+    p.grid = (uint32_t)(num_cus() * pre_waves(split, DK, DV));
 }
 }  // namespace
 
-AttnPlan attn_pre_plan(const AttnArgs & a) {
+AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype) {
     AttnPlan p{};
-    uint32_t per_cu = 1;
+    const bool split = dtype == FLH_DT_F32;
     switch (attn_dims(a)) {
-        case 0: shape<64, 64>(p, per_cu); break;
-        case 1: shape<128, 128>(p, per_cu); break;
-        case 2: shape<192, 128>(p, per_cu); break;
-        default: shape<256, 256>(p, per_cu); break;
+        case 0: shape<64, 64>(p, split); break;
+        case 1: shape<128, 128>(p, split); break;
+        case 2: shape<192, 128>(p, split); break;
+        default: shape<256, 256>(p, split); break;
     }
-    p.grid = (uint32_t)num_cus() * (per_cu < 1 ? 1 : per_cu > 2 ? 2 : per_cu);
     p.min_units = 2;
     p.ws = attn_ws(p.grid, p.m, p.dv);
     return p;

@@ -197,7 +197,11 @@ template <int N, typename T> __device__ __forceinline__ void st_vec(T * p, const
 // 2N other elements (the last may have N), its heads of v into units of N, and
 // the workgroups of blockIdx.y share them.  Nothing is used twice but the
 // angles: a workgroup makes each once, behind the loads of its threads' first
-// units, and every head reads them from LDS.
+// units, and every head reads them from LDS.  Bytes bound it: 4999 tokens of 32 + 8 heads
+// of 128 with values in bf16 take 29 us (4.2 TB/s; a large copy reaches 5.1), 1000 tokens
+// of 16 + 16 heads of 192 in fp32 11.7 us (4.7 TB/s), one token 7.3 us, a launch and
+// its chain of loads.  One thread per pair with its own angle took 64.5, 23.6 and 7.3;
+// two units in flight instead of one 30.6.
 struct RopeUnits {
     uint32_t pu, u, n, step_h, step_e;     // a head's pair units and all its units, their number, and a step in (head, unit)
 };
@@ -205,7 +209,6 @@ constexpr uint32_t ROPE_T = 256;
 template <typename AT, typename CT, int N>
 __global__ __launch_bounds__(ROPE_T) void k_rope(RopeArgs a, RopeUnits ru) {
     __shared__ float2 cs[512];
-    constexpr int B = 2;                   // units in flight
     const uint32_t tok = a.tok0 + blockIdx.x, nk = a.kc ? a.n_kv : 0, P = a.rot ? a.n_rot / 2 : 0;
     const uint32_t first = blockIdx.y * ROPE_T + threadIdx.x, step = gridDim.y * ROPE_T;
     const uint32_t slot = nk ? a.slot[tok] : 0;
@@ -217,48 +220,39 @@ __global__ __launch_bounds__(ROPE_T) void k_rope(RopeArgs a, RopeUnits ru) {
 
     uint32_t h = first / ru.u, e = first - h * ru.u;
     for (uint32_t at = first, round = 0; round == 0 || at - threadIdx.x < ru.n; ++round) {
-        Vec<AT, N> x[B], w[B];
-        uint32_t hs[B], es[B], is[B], js[B];
-        bool on[B], two[B];
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            on[b] = at < ru.n && (h < a.n_head || live);
-            two[b] = true;
-            hs[b] = h; es[b] = e;
-            if (e < ru.pu) {
-                is[b] = a.first + (a.halves ? e * N : e * 2 * N);
-                js[b] = is[b] + (a.halves ? P : N);
-            } else {
-                const uint32_t r = (e - ru.pu) * 2 * N;          // among the elements that are not turned
-                is[b] = r < a.first || !P ? r : r + 2 * P;
-                js[b] = r + N < a.first || !P ? r + N : r + N + 2 * P;
-                two[b] = r + N < a.d - 2 * P;
-            }
-            if (on[b]) {
-                const AT * src = h < a.n_head ? q + h * a.q_head : k + (h - a.n_head) * a.k_head;
-                x[b] = ld_vec<N>(src + is[b]);
-                if (two[b]) w[b] = ld_vec<N>(src + js[b]);
-            }
-            at += step; h += ru.step_h; e += ru.step_e;
-            if (e >= ru.u) { e -= ru.u; ++h; }
+        Vec<AT, N> x, w;
+        uint32_t i0, j0;                   // where the unit's two vectors are in the head
+        bool two = true;
+        const bool on = at < ru.n && (h < a.n_head || live), isq = h < a.n_head;
+        if (e < ru.pu) {
+            i0 = a.first + (a.halves ? e * N : e * 2 * N);
+            j0 = i0 + (a.halves ? P : N);
+        } else {
+            const uint32_t r = (e - ru.pu) * 2 * N;              // among the elements that are not turned
+            i0 = r < a.first || !P ? r : r + 2 * P;
+            j0 = r + N < a.first || !P ? r + N : r + N + 2 * P;
+            two = r + N < a.d - 2 * P;
+        }
+        if (on) {
+            const AT * src = isq ? q + h * a.q_head : k + (h - a.n_head) * a.k_head;
+            x = ld_vec<N>(src + i0);
+            if (two) w = ld_vec<N>(src + j0);
         }
         if (round == 0) {
             for (uint32_t i = threadIdx.x; i < P; i += ROPE_T)
                 rope_cs(a.rot[i], a.pos, a.pos_stride, tok, cs[i].x, cs[i].y);
             __syncthreads();
         }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            if (!on[b]) continue;
+        if (on) {
             float y[N], z[N];
-            if (es[b] < ru.pu) {
-                const float2 * t = cs + es[b] * N;
+            if (e < ru.pu) {
+                const float2 * t = cs + e * N;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float c = t[i].x, s = t[i].y;
                     // halves: pair i is (x[i], w[i]); pairs: the 2N elements x, w one after the other
-                    const float v = (float)(a.halves ? x[b].v[i] : 2 * i < N ? x[b].v[2 * i % N] : w[b].v[2 * i % N]);
-                    const float u = (float)(a.halves ? w[b].v[i] : 2 * i + 1 < N ? x[b].v[(2 * i + 1) % N] : w[b].v[(2 * i + 1) % N]);
+                    const float v = (float)(a.halves ? x.v[i] : 2 * i < N ? x.v[2 * i % N] : w.v[2 * i % N]);
+                    const float u = (float)(a.halves ? w.v[i] : 2 * i + 1 < N ? x.v[(2 * i + 1) % N] : w.v[(2 * i + 1) % N]);
                     const float ya = v * c - u * s, yb = v * s + u * c;
                     if (a.halves) {
                         y[i] = ya;
@@ -277,20 +271,22 @@ __global__ __launch_bounds__(ROPE_T) void k_rope(RopeArgs a, RopeUnits ru) {
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    y[i] = (float)x[b].v[i];
-                    z[i] = (float)w[b].v[i];
+                    y[i] = (float)x.v[i];
+                    z[i] = (float)w.v[i];
                 }
             }
-            if (hs[b] < a.n_head) {
-                AT * d = qo + hs[b] * a.qo_head;
-                st_vec<N>(d + is[b], y);
-                if (two[b]) st_vec<N>(d + js[b], z);
+            if (isq) {
+                AT * d = qo + h * a.qo_head;
+                st_vec<N>(d + i0, y);
+                if (two) st_vec<N>(d + j0, z);
             } else {
-                CT * d = kc + (hs[b] - a.n_head) * a.kc_head;
-                st_vec<N>(d + is[b], y);
-                if (two[b]) st_vec<N>(d + js[b], z);
+                CT * d = kc + (h - a.n_head) * a.kc_head;
+                st_vec<N>(d + i0, y);
+                if (two) st_vec<N>(d + j0, z);
             }
         }
+        at += step; h += ru.step_h; e += ru.step_e;
+        if (e >= ru.u) { e -= ru.u; ++h; }
     }
     if (!live) return;
     const uint32_t vu = a.dv / N;

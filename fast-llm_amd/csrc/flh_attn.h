@@ -15,7 +15,10 @@
 // item (request, strip, kv head) that lies across a border is worked on by
 // several workgroups, which leave unscaled sums in the workspace; k_attn_join
 // adds them up in line order.  Every strip has at least one unit, so
-// rows that see nothing are written too.
+// rows that see nothing are written too.  An item's tiles stand behind C units
+// with nothing in them, the cost of its begin and end in tiles: a workgroup of many
+// short items gets as much time as one of a few long ones (a border among them
+// stands for the item's begin).
 #pragma once
 #include "flh_common.h"
 #include "flh_internal.h"
@@ -90,10 +93,12 @@ struct AttnItem {
     int32_t p0;                         // position of its first row's token
     int32_t cap;                        // keys with a table entry
     int32_t lo, hi;                     // keys that some row of the strip sees
-    uint32_t u0, tiles;                 // first unit of the item, units
+    uint32_t u0, tiles;                 // first unit of the item, tiles (units: C more)
 };
+// tiles in front of unit x of an item
+template <int C> __device__ __forceinline__ uint32_t tiles_at(uint32_t x) { return x > C ? x - C : 0u; }
 
-template <int M, int KT> struct AttnWalk {
+template <int M, int KT, int C> struct AttnWalk {
     // the wave's 64 requests at hand, in LDS (they are looked at once an item)
     struct Chunk {
         uint32_t n[64], r0[64], one[64], excl[64];                    // tokens, first row, units a kv head, units before it
@@ -146,7 +151,7 @@ template <int M, int KT> struct AttnWalk {
         const uint32_t ns = strips(n, a.group);
         int32_t lo, hi;
         uint32_t one = fresh(span(max(n, 1u), p0, cap, 0, lo, hi));
-        one = ns == 1 ? one : 0;
+        one = ns == 1 ? one + C : 0;
         uint64_t many = __ballot(ns > 1);
         while (many) {                                                // requests of many strips, lane per strip
             const int l = __builtin_ctzll(many);
@@ -156,7 +161,7 @@ template <int M, int KT> struct AttnWalk {
             uint32_t c = 0;
             for (uint32_t i = 0; i < bs; i += 64) {
                 const uint32_t v = fresh(span(bn, bp, bc, i + lane, lo, hi));
-                c += i + lane < bs ? v : 0u;
+                c += i + lane < bs ? v + C : 0u;
             }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) c += __shfl_xor(c, d);
@@ -204,7 +209,7 @@ template <int M, int KT> struct AttnWalk {
         if (ns > 1) {
             for (uint32_t i = 0;; i += 64) {
                 int32_t lo, hi;
-                const uint32_t v = fresh(span(it.n, it.p0, it.cap, i + lane, lo, hi)), c = i + lane < ns ? v : 0u;
+                const uint32_t v = fresh(span(it.n, it.p0, it.cap, i + lane, lo, hi)), c = i + lane < ns ? v + C : 0u;
                 const uint32_t inc = scan(c, lane), sum = __builtin_amdgcn_readlane(inc, 63);
                 if (x >= sum && i + 64 < ns) {
                     x -= sum;
@@ -454,15 +459,15 @@ template <int M, int DV> __device__ __forceinline__ AttnNote * attn_notes(const 
 }
 inline size_t attn_ws(uint32_t grid, uint32_t m, uint32_t dv) { return (size_t)grid * (2 * m * (dv + 2) * 4 + sizeof(AttnNote)); }
 
-// The note of workgroup w about its first item, which begins `skip` units before w (by a
+// The note of workgroup w about its first item, which begins `skip` tiles before w (by a
 // whole wave, every lane the same).
-template <int M, int DV>
+template <int M, int DV, int C>
 __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32_t U, uint32_t Ge, const AttnItem & it, uint32_t skip) {
     AttnNote * n = attn_notes<M, DV>(a) + w;
     uint32_t parts = 0;
-    if (skip && attn_border(w - 1, U, Ge) <= it.u0) {
+    if (skip && attn_border(w - 1, U, Ge) <= it.u0 + C) {
         uint32_t last = w;                                            // the last workgroup with a part
-        while (last + 1 < Ge && attn_border(last + 1, U, Ge) < it.u0 + it.tiles) ++last;
+        while (last + 1 < Ge && attn_border(last + 1, U, Ge) < it.u0 + it.tiles + C) ++last;
         parts = last - w + 2;
         n->seq = it.seq; n->strip = it.strip; n->kvh = it.kvh; n->r0 = it.r0; n->n = it.n;
         n->p0 = it.p0; n->cap = it.cap;
@@ -474,7 +479,7 @@ __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32
 // order, four rows a wave; PW waves share the parts of the same rows (a few rows of
 // many parts: latency).  Rows of items with sums that are not finite are done by
 // attn_row instead.
-template <typename AT, typename T, int M, int KT, int DV, int PW>
+template <typename AT, typename T, int M, int KT, int DV, int PW, int C>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     constexpr int V = DV / 64, R = 4;                                 // values a lane, rows a wave
     __shared__ float red[PW > 1 ? PW : 1][R][PW > 1 ? DV : 1];
@@ -595,16 +600,16 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
         }
     }
     if (!me.odd || pw) return;
-    __shared__ typename AttnWalk<M, KT>::Chunk chunks[4];
-    AttnWalk<M, KT> walk(a, chunks[wave]);
+    __shared__ typename AttnWalk<M, KT, C>::Chunk chunks[4];
+    AttnWalk<M, KT, C> walk(a, chunks[wave]);
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     const uint32_t u = attn_border(w, U, Ge), end = attn_border(w + 1, U, Ge);
     for (uint32_t x = u; x < end;) {                                  // items of workgroup w alone
         AttnItem it;
         walk.find(x, it);
-        if (it.u0 >= u && it.u0 + it.tiles <= end)
+        if (it.u0 + C >= u && it.u0 + it.tiles + C <= end)
             for (uint32_t r = rbase; r < min((uint32_t)M, min(rbase + R, it.n * a.group - it.strip * M)); ++r) attn_row<AT, T, M>(a, it, r);
-        x = it.u0 + it.tiles;
+        x = it.u0 + it.tiles + C;
     }
 }
 

@@ -45,9 +45,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     const uint32_t k_lane = l16 * (DK * 2) + (q4 ^ swz_k<DK>(l16)) * 16;
     const uint32_t v_row = 4 * q4 + (l16 >> 2);
     const uint32_t v_lane = 32 * DK * 2 + v_row * (DV * 2) + (((l16 >> 1) & 1) ^ swz_v<DV>(v_row)) * 16 + (l16 & 1) * 8;
-    typedef typename AttnWalk<M, KT>::Chunk Chunk;
+    typedef typename AttnWalk<M, KT, 0>::Chunk Chunk;
     static_assert(sizeof(Chunk) == P::WALK, "chunk");
-    AttnWalk<M, KT> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
+    AttnWalk<M, KT, 0> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units), w = blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
@@ -60,7 +60,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT + 32 * wave);   // this wave's first key
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
-        if (u == first_u && wave == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
+        if (u == first_u && wave == 0) attn_note<M, DV, 0>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group;
 
         // ---- the strip's queries, as the second operand: column l16, elements 32 s + 8 q4 ..
@@ -338,7 +338,7 @@ template <typename AT, typename T, int DK, int DV, int MT> int go(const AttnArgs
     if (int rc = lds_fits(k, P::LDS, "k_attn_dec")) return rc;
     hipLaunchKernelGGL((k_attn_dec<AT, T, DK, DV, MT>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_dec launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4, 0>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
 template <typename AT, typename T, int MT> int dims(const AttnArgs & a, hipStream_t s) {

@@ -11,6 +11,9 @@ namespace flh {
 // are a lane's own but for one exchange with the other half of the wave, and the
 // weights are, as they are, the second operand of O^T += V^T P^T (the order of the
 // keys inside a product does not matter, V^T is read in the same one).
+// C of the line of work.  8192 tokens of 32 / 8 heads in bf16 take 690 us with 0 (the first
+// workgroup has 32 items and takes a third longer than most), 648 with 3.
+constexpr int PRE_ITEM = 3;
 template <int DK, int DV> struct PreShape {
     static constexpr int W = 4;                                       // waves
     static constexpr int M = 32 * W, KT = 64, NST = 2;
@@ -51,9 +54,9 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         const uint32_t r = 8 * p + 4 * half + (l16 >> 2), pc = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
         v_lane[p] = KT * DK * 2 + r * (DV * 2) + (pc ^ swz_v<DV>(r)) * 16 + (l16 & 1) * 8;
     }
-    typedef typename AttnWalk<M, KT>::Chunk Chunk;
+    typedef typename AttnWalk<M, KT, PRE_ITEM>::Chunk Chunk;
     static_assert(sizeof(Chunk) == P::WALK, "chunk");
-    AttnWalk<M, KT> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 128 + wave * P::WALK));
+    AttnWalk<M, KT, PRE_ITEM> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 128 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     // neighbours on the line share keys: they go to one XCD (workgroups are dealt
     // to the 8 XCDs in turn)
@@ -66,10 +69,11 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
     while (u < end) {
         AttnItem it;
         walk.find(u, it);
-        const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
+        const uint32_t skip = tiles_at<PRE_ITEM>(u - it.u0), nt = tiles_at<PRE_ITEM>(min(it.tiles + PRE_ITEM, end - it.u0)) - skip;
+        if (u == first_u && wave == 0) attn_note<M, DV, PRE_ITEM>(a, w, U, Ge, it, skip);
+        if (nt == 0) break;                                           // (the workgroup ends among the item's empty units)
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT);
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
-        if (u == first_u && wave == 0) attn_note<M, DV>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group, row = it.strip * M + 32 * wave + l32, tok = row / a.group;
         const uint32_t head = it.kvh * a.group + row % a.group;
         const int32_t win = (int32_t)min(a.window, 1u << 30);
@@ -372,7 +376,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                 }
             }
         }
-        u += nt;
+        u = it.u0 + PRE_ITEM + skip + nt;
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the next item's stages
     }
     sm_odd[wave] = __ballot(odd) != 0;
@@ -393,7 +397,7 @@ template <typename AT, typename T, int DK, int DV> int go(const AttnArgs & a, hi
     if (int rc = lds_fits(k, P::LDS, "k_attn_pre")) return rc;
     hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_pre launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV, 1>), dim3(a.grid, P::M / 16), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV, 1, PRE_ITEM>), dim3(a.grid, P::M / 16), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
 template <typename AT, typename T> int dims(const AttnArgs & a, hipStream_t s) {

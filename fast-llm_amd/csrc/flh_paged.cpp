@@ -85,8 +85,8 @@ int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
     if (p->window && !p->causal) return set_error(FLH_ERR_ARG, "attention: a window needs causal");
     const uint64_t keys = (uint64_t)p->table_stride * c->page_size;
     if (keys > (1ull << 30)) return set_error(FLH_ERR_UNSUPPORTED, "attention: table_stride * page_size must be at most 2^30");
-    // units of work are counted in 32 bits (strips of 16 rows or more, tiles of 64 keys or more)
-    if ((double)c->n_kv_head * ((double)p->n_tok * group / 16 + 2.0 * p->n_seq) * ((double)keys / 64 + 2) >= 4.0e9)
+    // units of work are counted in 32 bits (strips of 16 rows or more, tiles of 64 keys or more and 3 units a strip)
+    if ((double)c->n_kv_head * ((double)p->n_tok * group / 16 + 2.0 * p->n_seq) * ((double)keys / 64 + 5) >= 4.0e9)
         return set_error(FLH_ERR_UNSUPPORTED, "attention: too much work for one call (rows times table length)");
     a = AttnArgs{};
     a.q = p->q; a.out = p->out; a.q_start = p->q_start; a.kv_len = p->kv_len; a.table = p->table; a.ws = p->ws;

@@ -262,6 +262,8 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                         for (int j = 0; j < 4; ++j) vf[step & 1][d][4 * p + j] = r4[j];
                     }
             };
+            // (of a SIMD's two waves the one with products goes first: 640 -> 618 us, 8192 tokens, bf16)
+            __builtin_amdgcn_s_setprio(1);
             ld_k(0);
             ld_k(1);
             ld_k(2);
@@ -294,6 +296,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             l += sum;
         };
         {

@@ -63,6 +63,16 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         if (u == first_u && wave == 0) attn_note<M, DV, 0>(a, w, U, Ge, it, skip);
         const uint32_t rows = it.n * a.group;
 
+        const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
+        const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
+        // page numbers of this wave's keys of tile t: one DMA, lane l's key (lanes from 32 on repeat)
+        auto issue_tab = [&](uint32_t t) {
+            const int32_t key = key0 + (int32_t)(t * KT + (lane & 31));
+            const uint32_t pg = (uint32_t)min(key, max(it.cap - 1, 0)) >> a.sh;
+            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (t & 1) * 256);
+        };
+        issue_tab(0);                                                 // (they arrive with the queries)
+
         // ---- the strip's queries, as the second operand: column l16, elements 32 s + 8 q4 ..
         v8 qf[NS][MT][DK / 32];
         float c[MT];                                                  // scale * log2(e), by column
@@ -118,14 +128,6 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         }
 
         const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
-        const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
-        const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
-        // page numbers of this wave's keys of tile t: one DMA, lane l's key (lanes from 32 on repeat)
-        auto issue_tab = [&](uint32_t t) {
-            const int32_t key = key0 + (int32_t)(t * KT + (lane & 31));
-            const uint32_t pg = (uint32_t)min(key, max(it.cap - 1, 0)) >> a.sh;
-            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (t & 1) * 256);
-        };
         // keys that a row of the strip sees and that have a page: bit per key
         auto issue_kv = [&](uint32_t t, uint32_t stage) -> uint32_t {
             const int32_t k0 = key0 + (int32_t)(t * KT);
@@ -223,7 +225,6 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             }
             // order of issue: T0, T1 KV0, T2 KV1, ..: a tile's pages are behind the tile before
             uint32_t vms[NST];
-            issue_tab(0);
 #pragma unroll
             for (int i = 0; i < NST; ++i) {
                 vms[i] = 0;

@@ -85,6 +85,17 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         const int32_t tf = (int32_t)(first / a.group), tl = (int32_t)min(it.n - 1, (first + 31) / a.group);
         const int32_t all_lo = win ? it.p0 + tl + 1 - win : 0, all_hi = a.causal ? min(it.cap, it.p0 + tf + 1) : it.cap;
 
+        const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
+        const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
+        // The rows of four tiles are found together, 16 keys of each by the wave that brings
+        // them (lane l: key l % 16 of tile 4 g + l / 16).
+        auto key_of = [&](uint32_t g) { return key0 + (int32_t)((4 * g + (lane >> 4)) * KT + 16 * wave + l16); };
+        auto issue_tab = [&](uint32_t g) {                            // page numbers
+            const uint32_t pg = (uint32_t)min(key_of(g), max(it.cap - 1, 0)) >> a.sh;
+            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at);
+        };
+        issue_tab(0);                                                 // (they arrive with the queries)
+
         // ---- queries: column l32, elements 16 s + 8 half ..
         v8 qf[NS][DK / 16];
         float c = a.scale == 0.f ? 1.f : a.scale * 1.4426950408889634f;   // scale * log2(e), by row
@@ -130,15 +141,6 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         }
 
         const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
-        const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
-        const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
-        // The rows of four tiles are found together, 16 keys of each by the wave that brings
-        // them (lane l: key l % 16 of tile 4 g + l / 16).
-        auto key_of = [&](uint32_t g) { return key0 + (int32_t)((4 * g + (lane >> 4)) * KT + 16 * wave + l16); };
-        auto issue_tab = [&](uint32_t g) {                            // page numbers
-            const uint32_t pg = (uint32_t)min(key_of(g), max(it.cap - 1, 0)) >> a.sh;
-            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at);
-        };
         auto find_rows = [&](uint32_t g) {                            // from them, row addresses and live keys
             const int32_t key = key_of(g);
             const uint32_t own = *(const uint32_t *)(tabs + 4 * lane), tok = (uint32_t)key & a.pmask;
@@ -311,7 +313,6 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
             // behind the barrier that tells that the round before is over, and waits
             // for it at the begin of the next.  Rows of the next four tiles are found in
             // round 1 of four, from page numbers asked for in round 0.
-            issue_tab(0);
             wait_vm<0>();
             find_rows(0);
             read_k(0);

@@ -478,7 +478,8 @@ __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32
 // Behind the main kernel.  Workgroups (w, y): the parts of w's note are added up in
 // order, four rows a wave; PW waves share the parts of the same rows (a few rows of
 // many parts: latency).  Rows of items with sums that are not finite are done by
-// attn_row instead.
+// attn_row instead.  The parts' bytes bound it where there are many (16 us for those of 512
+// workgroups with 128 rows of 128, up to 134 KB each), else a launch (4 us).
 template <typename AT, typename T, int M, int KT, int DV, int PW, int C>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     constexpr int V = DV / 64, R = 4;                                 // values a lane, rows a wave

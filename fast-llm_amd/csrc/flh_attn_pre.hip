@@ -1,5 +1,5 @@
 // flh_attn_pre.hip -- attention of many rows per kv head (prompts, chunks): the
-// matrix cores are what bounds it.
+// matrix cores and the vector instructions of the softmax are what bounds it.
 #include "flh_attn.h"
 #include "flh_status.h"
 
@@ -10,7 +10,20 @@ namespace flh {
 // products), so a lane holds one row's scores of 32 keys: the maximum and the sum
 // are a lane's own but for one exchange with the other half of the wave, and the
 // weights are, as they are, the second operand of O^T += V^T P^T (the order of the
-// keys inside a product does not matter, V^T is read in the same one).
+// keys inside a product does not matter, V^T is read in the same one).  The next tile's
+// scores are multiplied while this tile's weights are made (an instruction of each in
+// turn), so that neither unit waits for the other.
+// Roundings: with 16-bit activations a weight is rounded to the cache's type for the product
+// with V (half a step of that type, as much as the rounding of the result), sums stay fp32;
+// fp32 activations and their weights are split into terms that hold all their bits, so only
+// fp32 accumulation rounds.
+// 8192 tokens, causal, 32 / 8 heads of 128: 620 to 640 us in bf16 (860 TFLOP/s; a large library
+// product reaches 1220), of which k_attn_join is 16.  The matrix cores are busy 40% of the
+// time (at about 2.0 GHz under this load), the vector units about as long.  fp32 over f16 (two terms, twice the
+// products) 647 us for 5 ragged chunks (800 TFLOP/s of products).  32 rows a wave and two
+// workgroups a CU: the registers hold a wave's sums, queries and two tiles' scores (256); a
+// third workgroup of narrow heads (64) would need 168 registers, spilled, and took 69 us
+// instead of 63 for 8 x 20 heads over 1500 keys.
 // C of the line of work.  8192 tokens of 32 / 8 heads in bf16 take 690 us with 0 (the first
 // workgroup has 32 items and takes a third longer than most), 648 with 3.
 constexpr int PRE_ITEM = 3;
@@ -429,7 +442,9 @@ AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype) {
         case 2: shape<192, 128>(p, split); break;
         default: shape<256, 256>(p, split); break;
     }
-    p.min_units = 2;
+    // (64 tokens over 4096 keys: 48 us with 1 or 2, 38 with 4: fewer parts to join; over 512 keys
+    // 23 us with 2, 24 with 4)
+    p.min_units = 4;
     p.ws = attn_ws(p.grid, p.m, p.dv);
     return p;
 }

@@ -15,7 +15,11 @@ namespace flh {
 // threads flat, each finding its request by a binary search over the scan in
 // LDS.  More rows go to k_kv_slots, a launch over all CUs behind this one.  One
 // workgroup, so taken and kv_len may be updated in place: nobody else reads
-// them.  Sums are 64-bit (a garbage length costs its own rows only).
+// them.  Sums are 64-bit (a garbage length costs its own rows only).  A launch and
+// a chain of loads, scans and searches bound it: 64 requests of a token each take
+// 6.7 us, 500 with 64000 rows 11.2 (two launches).  Rows in the same launch cost one
+// workgroup 1 us for about 1200 of them, a second launch 4 to 5 us: 2048 rows take 8.8
+// us in one and 12.1 in two, 8192 13.4 and 12.2, 16384 19.9 and 12.1.
 constexpr uint32_t PLAN_T = 1024;
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, uint32_t d) {
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(256) void k_kv_slots(flh_kv_plan_p p, uint32_t sh) 
 }
 
 int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s) {
-    constexpr uint32_t PLAN_ROWS = 16384;
+    constexpr uint32_t PLAN_ROWS = 6144;
     const uint32_t sh = (uint32_t)__builtin_ctz(p.page_size);
     const bool one = p.max_tok <= PLAN_ROWS;
     hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(PLAN_T), 0, s, p, sh, one ? 1 : 0);
@@ -198,8 +202,8 @@ template <int N, typename T> __device__ __forceinline__ void st_vec(T * p, const
 // the workgroups of blockIdx.y share them.  Nothing is used twice but the
 // angles: a workgroup makes each once, behind the loads of its threads' first
 // units, and every head reads them from LDS.  Bytes bound it: 4999 tokens of 32 + 8 heads
-// of 128 with values in bf16 take 29 us (4.2 TB/s; a large copy reaches 5.1), 1000 tokens
-// of 16 + 16 heads of 192 in fp32 11.7 us (4.7 TB/s), one token 7.3 us, a launch and
+// of 128 with values in bf16 take 27 us (4.5 TB/s; a large copy reaches 5.1), 1000 tokens
+// of 16 + 16 heads of 192 in fp32 11.0 us (5.0 TB/s), one token 6.9 us, a launch and
 // its chain of loads.  One thread per pair with its own angle took 64.5, 23.6 and 7.3;
 // two units in flight instead of one 30.6.
 struct RopeUnits {
@@ -310,6 +314,8 @@ static int rope_n(RopeArgs a, hipStream_t s) {
     ru.u = ru.pu + (rest + 2 * N - 1) / (2 * N);
     ru.n = ru.u * (a.n_head + nk);
     const uint32_t most = (uint32_t)((std::max<uint64_t>(ru.n, nk * a.dv / N) + ROPE_T - 1) / ROPE_T);
+    // few tokens: workgroups share a token's units (one token of 128 + 8 heads of 192: 8.3 us
+    // with a unit a thread, 11.1 in one workgroup; of 32 + 8 heads of 128 the same)
     const uint32_t parts = std::max(1u, std::min(most, 512 / a.n_tok));
     ru.step_h = parts * ROPE_T / ru.u;
     ru.step_e = parts * ROPE_T % ru.u;

@@ -173,3 +173,9 @@ def test_steps_in_place_and_captured(flh, gpu, max_tok):
         check(p.read(), want)
         held, table, taken, slot, pos = want["kv_len"], want["table"], int(want["taken"][0]), want["slot"], want["pos"]
     g.close()
+
+
+@pytest.mark.parametrize("max_tok", [6143, 6144, 6145])
+def test_rows_around_the_second_launch(flh, gpu, max_tok):
+    """The rows of one launch and of two."""
+    test_plan(flh, gpu, 76, 300, 80, 80, 16, 3, max_tok - 76 * 80, 0)

@@ -356,3 +356,66 @@ def test_offsets_past_32_bits(flh, gpu):
     flh.paged_attn(cache, small.p, gpu)
     small.check()
     del rng
+
+
+def short_items(seed, n_seq, most_rows, most_keys):
+    """Requests of few rows over few keys, now and then one over many."""
+    rng = np.random.default_rng(seed)
+    lens = []
+    for i in range(n_seq):
+        n = int(rng.integers(0, most_rows + 1))
+        kv = n + int(rng.integers(0, most_keys if i % 17 else 40 * most_keys))
+        lens.append((n, kv))
+    return lens + [(most_rows, most_rows)]
+
+
+@pytest.mark.parametrize("act,cdt", TYPES)
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64), (192, 128)])
+@pytest.mark.parametrize("n_seq", [40, 200, 700])
+def test_short_items(flh, gpu, act, cdt, dk, dv, n_seq):
+    """Many strips of a tile or two per workgroup: shares end inside, at the begin
+    and at the end of them."""
+    c = Case(flh, gpu, act, cdt, 8, 1, dk, dv, 16, "head", short_items(n_seq, n_seq, 20, 70), 22)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("act,cdt", TYPES)
+@pytest.mark.parametrize("n_seq", [30, 300])
+def test_short_items_with_values_not_seen(flh, gpu, act, cdt, n_seq):
+    """An infinite value at every request's last key, which only its last row sees."""
+    c = Case(flh, gpu, act, cdt, 8, 1, 64, 64, 16, "head", short_items(n_seq + 1, n_seq, 20, 70), 23)
+    for i, kv in enumerate(c.kv_len):
+        if kv:
+            j = int(kv) - 1
+            c.cache.view[1][int(c.table[i, j // 16]), j % 16, 0, 5] = math.inf
+    c.cache.push()
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("act,cdt", TYPES)
+def test_wide_groups(flh, gpu, act, cdt):
+    """One token of more query heads per kv head than the streaming kernel has rows."""
+    c = Case(flh, gpu, act, cdt, 96, 2, 64, 64, 16, "token", [(1, kv) for kv in (1, 63, 64, 65, 500, 3000)], 24)
+    c.run()
+    c.check()
+
+
+def test_tiles_in_fours(flh, gpu):
+    """Keys around multiples of four tiles of 64 (rows are found for four at once)."""
+    lens = [(40, kv) for kv in (64, 128, 192, 255, 256, 257, 319, 320, 321, 448, 511, 512, 513, 768, 1023, 1025)]
+    for window in (0, 200, 330):
+        c = Case(flh, gpu, "BF16", "BF16", 4, 4, 128, 128, 8, "head", lens, 25, window=window)
+        c.run()
+        c.check()
+
+
+def test_a_torch_stream(flh, gpu):
+    """A stream that was made elsewhere."""
+    c = Case(flh, gpu, "F32", "F16", 8, 2, 128, 128, 16, "head", [(1, 700), (30, 300)], 26)
+    gpu.sync()
+    t = torch.cuda.Stream()
+    c.run(flh.Stream.wrap(t.cuda_stream))
+    t.synchronize()
+    c.check()

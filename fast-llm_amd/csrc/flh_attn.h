@@ -107,6 +107,7 @@ template <int M, int KT, int C> struct AttnWalk {
     const AttnArgs & a;
     Chunk & ch;
     uint32_t base = 0, line0 = 0, all = 0;                            // the chunk's first request, first unit, units
+    float about = 0.f;                                                // its units, however many
     __device__ AttnWalk(const AttnArgs & args, Chunk & c) : a(args), ch(c) {}
     template <typename V> __device__ static V get(const V & v) { return (V)__builtin_amdgcn_readfirstlane((int)v); }
 
@@ -169,6 +170,9 @@ template <int M, int KT, int C> struct AttnWalk {
         }
         const uint32_t inc = scan(one * a.n_kv, lane);
         all = __builtin_amdgcn_readlane(inc, 63);
+        about = (float)one * (float)a.n_kv;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) about += __shfl_xor(about, d);
         ch.n[lane] = n;
         ch.r0[lane] = x;
         ch.one[lane] = one;
@@ -176,13 +180,17 @@ template <int M, int KT, int C> struct AttnWalk {
         ch.p0[lane] = p0;
         ch.cap[lane] = cap;
     }
-    // units in all; leaves the walk at the first request
+    // units in all; leaves the walk at the first request.  0 where they pass 32 bits: the host
+    // bounds what n_tok rows can give, but a q_start that does not ascend can give more.
     __device__ uint32_t total() {
         uint32_t u = 0;
+        float sum = 0.f;
         for (uint32_t b = 0; b < a.n_seq; b += 64) {
             load(b);
             u += all;
+            sum += about;
         }
+        if (__builtin_amdgcn_readfirstlane(sum >= 4.2e9f)) return 0;
         line0 = 0;
         if (a.n_seq > 64) load(0);
         return u;
@@ -448,7 +456,7 @@ struct AttnNote {
     uint32_t parts;                     // of the item that its first border is the first one inside (0: none)
     uint32_t seq, strip, kvh, r0, n;
     int32_t p0, cap;
-    uint32_t wgs;                       // workgroups that had work (Ge)
+    uint32_t wgs;                       // workgroups that had work (Ge; 0 if there was none)
     uint32_t pad[6];
 };
 template <int M, int DV> __device__ __forceinline__ float * attn_part(const AttnArgs & a, uint32_t w, bool begins) {

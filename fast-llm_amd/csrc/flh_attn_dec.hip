@@ -331,7 +331,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         for (int i = 0; i < W; ++i) f |= sm_odd[i];
         AttnNote * n = attn_notes<M, DV>(a) + w;
         n->odd = f;
-        n->wgs = Ge;
+        n->wgs = U ? Ge : 0;
     }
 }
 

@@ -403,7 +403,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         for (int i = 0; i < W; ++i) f |= sm_odd[i];
         AttnNote * n = attn_notes<M, DV>(a) + w;
         n->odd = f;
-        n->wgs = Ge;
+        n->wgs = U ? Ge : 0;
     }
 }
 

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from paged_cases import Cache, NONE, TORCH, attn_bound, attn_oracle, get, put
+from paged_cases import Cache, NONE, TORCH, attn_bound, attn_oracle, get, put, raw
 
 pytestmark = pytest.mark.gpu
 
@@ -419,3 +419,42 @@ def test_a_torch_stream(flh, gpu):
     c.run(flh.Stream.wrap(t.cuda_stream))
     t.synchronize()
     c.check()
+
+
+@pytest.mark.parametrize("act,cdt", TYPES)
+@pytest.mark.parametrize("max_q", [1, 100])
+def test_rows_of_no_request_alone(flh, gpu, act, cdt, max_q):
+    """A padded step in which no request adds a token, behind one that left its notes in
+    the workspace."""
+    c = Case(flh, gpu, act, cdt, 4, 2, 128, 128, 16, "head", [(max_q, 5000), (max_q, 300)], 27)
+    c.p.max_q = max_q
+    c.ws()
+    c.run()
+    c.check()
+    c.b["out"].upload(raw(c.out0), gpu)
+    c.b["start"].upload(np.zeros(3, np.uint32), gpu)
+    for _ in range(2):
+        c.run()
+        assert torch.equal(c.result(), c.out0)
+
+
+@pytest.mark.parametrize("max_q", [1, 100])
+def test_starts_that_do_not_ascend(flh, gpu, max_q):
+    """35 requests that all claim the same rows, before 35 of none, give more units of work
+    than 32 bits hold: nothing is done, and nothing out of bounds."""
+    n, d, page = 1 << 20, 8, 65536
+    cache = Cache(flh, gpu, "F16", 1, page, 1, d, d, "head", 0)
+    cache.push()
+    table = np.full((70, 16), NONE, np.uint32)
+    start = np.array([0, n] * 35 + [0], np.uint32)
+    kv = np.full(70, 1 << 20, np.uint32)
+    q = torch.zeros(n, d, dtype=torch.float16)
+    out0 = torch.full((n, d), 3.0, dtype=torch.float16)
+    b = [put(flh, gpu, torch.from_numpy(x.view(np.int32))) for x in (start, kv, table)] + [put(flh, gpu, q), put(flh, gpu, out0)]
+    p = flh.AttnP(q=b[3].ptr, out=b[4].ptr, q_start=b[0].ptr, kv_len=b[1].ptr, table=b[2].ptr, q_tok=d, q_head=d, o_tok=d, o_head=d,
+                  dtype=flh.Dtype.F16, n_head=1, n_seq=70, n_tok=n, max_q=max_q, table_stride=16, scale=1.0, causal=0, window=0)
+    p.ws_bytes = flh.paged_attn_ws_bytes(cache.c, p)
+    ws = flh.DeviceBuffer(p.ws_bytes)
+    p.ws = ws.ptr
+    flh.paged_attn(cache.c, p, gpu)
+    assert torch.equal(get(b[4], out0, gpu), out0)

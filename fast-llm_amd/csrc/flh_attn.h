@@ -58,6 +58,19 @@ template <typename T, int NS> __device__ __forceinline__ void split(float x, T (
         x -= (float)o[i];
     }
 }
+// The same for two values (one conversion for both; the rest is exact)
+template <typename T, int NS> __device__ __forceinline__ void split(float x, float y, T (&o)[NS][2]) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const t2 h = __builtin_convertvector(f2{x, y}, t2);
+        o[i][0] = h[0];
+        o[i][1] = h[1];
+        x -= (float)h[0];
+        y -= (float)h[1];
+    }
+}
 // The weights exp2(score - max) are made 2^7 times larger for f16 terms, so that
 // small ones do not become subnormal there; the sum has the same factor.  (A
 // factor, not 7 more in the exponent: that would cost the largest weights, whose

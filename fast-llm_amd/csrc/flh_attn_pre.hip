@@ -48,6 +48,10 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = P::M, NS = split_terms<AT, T>();
     constexpr int NK = DK / 8 / W, NV = DV / 8 / W;                   // DMAs of a tile, this wave's
     constexpr int DB = DV / 32;
+    // Where the registers allow it: two tiles a turn of the loop, so that no scores are copied,
+    // and terms of two weights at once (5 ragged chunks in fp32 over f16: 643 us without,
+    // 626 with the first, 610 with both; in the forms of 256 registers either spills).
+    constexpr bool ROOM = pre_waves(NS > 1, DK, DV) == 1 && DK + DV <= 320, PAIRS = ROOM && NS > 1;
     extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
     const uint32_t lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5, l16 = lane & 15;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -244,17 +248,29 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                 for (int e = e0; e < e1; ++e) {
                     const float p = s[e >> 4][e & 15] * weight_unit<T>();
                     sum += p;
-                    T h[NS];
-                    split<T, NS>(p, h);
+                    if constexpr (PAIRS) {
+                        if ((e & 1) == 0) continue;
+                        T h[NS][2];
+                        split<T, NS>(s[e >> 4][(e & 15) - 1] * weight_unit<T>(), p, h);
 #pragma unroll
-                    for (int t2 = 0; t2 < NS; ++t2) pf[e >> 3][t2][e & 7] = h[t2];
+                        for (int t2 = 0; t2 < NS; ++t2) {
+                            pf[e >> 3][t2][(e & 7) - 1] = h[t2][0];
+                            pf[e >> 3][t2][e & 7] = h[t2][1];
+                        }
+                    } else {
+                        T h[NS];
+                        split<T, NS>(p, h);
+#pragma unroll
+                        for (int t2 = 0; t2 < NS; ++t2) pf[e >> 3][t2][e & 7] = h[t2];
+                    }
                 }
             };
             // step i of n of the 16 weights from e0 on
             auto weights = [&](int i, int n, int e0) {
                 const int q = n - 2;
-                if (i < q) exps(e0 + 16 * i / q, e0 + 16 * (i + 1) / q);
-                if (i >= 1 && i <= q) pack(e0 + 16 * (i - 1) / q, e0 + 16 * i / q);
+                constexpr int S = PAIRS ? 2 : 1;
+                if (i < q) exps(e0 + 16 / S * i / q * S, e0 + 16 / S * (i + 1) / q * S);
+                if (i >= 1 && i <= q) pack(e0 + 16 / S * (i - 1) / q * S, e0 + 16 / S * i / q * S);
             };
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -350,10 +366,17 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                 if (here) tile(key0 + (int32_t)(t * KT), now, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE, s, nx, midway);
                 else midway();
             };
-            for (uint32_t t = 0; t < nt; ++t) {
-                round(t, sa, sb);
-                sa[0] = sb[0];
-                sa[1] = sb[1];
+            if constexpr (ROOM) {
+                for (uint32_t t = 0; t < nt; t += 2) {
+                    round(t, sa, sb);
+                    if (t + 1 < nt) round(t + 1, sb, sa);
+                }
+            } else {
+                for (uint32_t t = 0; t < nt; ++t) {
+                    round(t, sa, sb);
+                    sa[0] = sb[0];
+                    sa[1] = sb[1];
+                }
             }
             wait_vm<0>();
             odd = odd || !finite(l);

@@ -614,11 +614,13 @@ int flh_graph_capture_end(void * stream, void ** graph_exec) {
 int flh_graph_launch(void * ge, void * stream) {
     const graph_handle * h = (const graph_handle *)ge;
     if (!h) return set_error(FLH_ERR_ARG, "null graph");
-    // A replay is one operation of its stream.  The runtime's launch is one by
-    // itself.  A chain is one because its thread has the stream to itself
-    // meanwhile (every entry point that issues work takes part in that), so it is
-    // only for a stream made here, on the device in force and not being captured.
-    const StreamTurn turn(stream, !h->chain.empty());
+    // A replay is one operation of its stream because its thread has the stream to
+    // itself meanwhile (every entry point that issues work takes part in that).  That
+    // holds for the runtime's launch too: three threads that launched graphs of six nodes
+    // on one stream at once were seen to leave the sums of seven dots behind one
+    // zeroing instead of four.  A chain is only for a stream made here, on the device in
+    // force and not being captured.
+    const StreamTurn turn(stream, true);
     int dev = -1;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     if (h->chain.empty() || turn.device() != h->device || hipGetDevice(&dev) != hipSuccess || dev != h->device ||

@@ -12,8 +12,8 @@
 
 namespace flh {
 
-// Held by an entry point while it issues work on a stream.  A replay that is
-// launched kernel by kernel holds it whole: it waits for the calls that are
+// Held by an entry point while it issues work on a stream.  A graph's replay
+// holds it whole: it waits for the calls that are
 // issuing on that stream, and later ones wait for it, so no other thread's work
 // falls between its kernels.  The other calls do not exclude each other, and
 // streams never wait for one another (a turn is found by the stream's handle).

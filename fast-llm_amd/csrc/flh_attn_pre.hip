@@ -19,8 +19,8 @@ namespace flh {
 // fp32 accumulation rounds.
 // 8192 tokens, causal, 32 / 8 heads of 128: 620 to 640 us in bf16 (860 TFLOP/s; a large library
 // product reaches 1220), of which k_attn_join is 16.  The matrix cores are busy 40% of the
-// time (at about 2.0 GHz under this load), the vector units about as long.  fp32 over f16 (two terms, twice the
-// products) 647 us for 5 ragged chunks (800 TFLOP/s of products).  32 rows a wave and two
+// time (at about 1.9 GHz under this load), the vector units about as long.  fp32 over f16 (two terms, twice the
+// products) 612 us for 5 ragged chunks (830 TFLOP/s of products).  32 rows a wave and two
 // workgroups a CU: the registers hold a wave's sums, queries and two tiles' scores (256); a
 // third workgroup of narrow heads (64) would need 168 registers, spilled, and took 69 us
 // instead of 63 for 8 x 20 heads over 1500 keys.

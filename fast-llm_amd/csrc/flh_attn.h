@@ -108,6 +108,21 @@ struct AttnItem {
     int32_t lo, hi;                     // keys that some row of the strip sees
     uint32_t u0, tiles;                 // first unit of the item, tiles (units: C more)
 };
+// keys [lo, hi) that a token of the item's request sees (any lo; none where hi <= lo or hi <= 0)
+__device__ __forceinline__ int32_t key_hi(const AttnArgs & a, const AttnItem & it, uint32_t tok) {
+    return a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
+}
+__device__ __forceinline__ int32_t key_lo(const AttnArgs & a, const AttnItem & it, uint32_t tok) {
+    return a.window ? it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30) : 0;
+}
+// whether one of the keys [lo, hi) (lo >= 0, hi <= cap) has a page; by a whole wave
+__device__ __forceinline__ bool any_page(const AttnArgs & a, const AttnItem & it, int32_t lo, int32_t hi) {
+    const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
+    bool any = false;
+    for (int64_t p = (lo >> a.sh) + (int64_t)(threadIdx.x & 63); __ballot(p << a.sh < hi) && !any; p += 64)
+        any = __ballot(p << a.sh < hi ? tab[p] < a.n_pages : false) != 0;
+    return any;
+}
 // tiles in front of unit x of an item
 template <int C> __device__ __forceinline__ uint32_t tiles_at(uint32_t x) { return x > C ? x - C : 0u; }
 
@@ -413,17 +428,19 @@ int launch_attn_dec(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hi
 int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 
 // One row by one wave, a key a lane, in fp32: for items whose sums are not
-// finite.  0 * inf is NaN, so in a matrix product a key that a row does not see
-// (weight 0), or the vanished low term of a split weight, carries an infinite or NaN
-// value into the row.  Here only the keys seen are looked at.
+// finite, and rows that have keys but no weight: all their scores are -infinity, or
+// finite ones passed fp32's range when they were multiplied by log2(e).  0 * inf is NaN, so in a matrix product a key
+// that a row does not see (weight 0), or the vanished low term of a split weight, carries an
+// infinite or NaN value into the row.  Here only the keys seen are looked at, and
+// scores stay what they are, so that they are finite wherever scale q.k is.
 template <typename AT, typename T, int M> __device__ __forceinline__ void attn_row(const AttnArgs & a, const AttnItem & it, uint32_t r) {
     const uint32_t lane = threadIdx.x & 63, row = it.strip * M + r, tok = row / a.group, head = it.kvh * a.group + row % a.group;
     const AT * q = (const AT *)a.q + (it.r0 + tok) * a.q_tok + head * a.q_head;
-    const int32_t hi = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
-    const int32_t lo = a.window ? max(0, it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30)) : 0;
+    const int32_t hi = key_hi(a, it, tok), lo = max(0, key_lo(a, it, tok));
     const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
     const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    bool any = false;                                                 // a key is seen
     for (int32_t j0 = lo; j0 < hi; j0 += 64) {
         const int32_t j = j0 + (int32_t)lane;
         const uint32_t pg = j < hi ? tab[(uint32_t)j >> a.sh] : FLH_KV_NONE;
@@ -447,6 +464,7 @@ template <typename AT, typename T, int M> __device__ __forceinline__ void attn_r
         m = mn;
         for (int c = 0; c < 4; ++c) o[c] *= al;
         uint64_t left = __ballot(in);
+        any = any || left;
         while (left) {
             const int k = __builtin_ctzll(left);
             left &= left - 1;
@@ -458,7 +476,7 @@ template <typename AT, typename T, int M> __device__ __forceinline__ void attn_r
     }
     AT * out = (AT *)a.out + (it.r0 + tok) * a.o_tok + head * a.o_head;
     for (uint32_t c = 0; c < 4; ++c)
-        if (64 * c + lane < a.dv) out[64 * c + lane] = (AT)(l == 0.f ? 0.f : o[c] / l);
+        if (64 * c + lane < a.dv) out[64 * c + lane] = (AT)(any ? o[c] / l : 0.f);
 }
 
 // What a launch leaves in the workspace: the parts of items that lie across a
@@ -498,8 +516,8 @@ __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32
 
 // Behind the main kernel.  Workgroups (w, y): the parts of w's note are added up in
 // order, four rows a wave; PW waves share the parts of the same rows (a few rows of
-// many parts: latency).  Rows of items with sums that are not finite are done by
-// attn_row instead.  The parts' bytes bound it where there are many (16 us for those of 512
+// many parts: latency).  Rows of items with sums that are not finite, and rows that lost all their
+// weight, are done by attn_row instead.  The parts' bytes bound it where there are many (16 us for those of 512
 // workgroups with 128 rows of 128, up to 134 KB each), else a launch (4 us).
 template <typename AT, typename T, int M, int KT, int DV, int PW, int C>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
@@ -590,10 +608,17 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) l[k] += xor_lane(l[k], d, lane);
         }
-        if (__ballot(odd != 0)) {
-            if (pw == 0)
-                for (uint32_t r = rbase; r < min(rbase + R, rows); ++r) attn_row<AT, T, M>(a, it, r);
-        } else if (rbase < rows) {
+        if (rbase < rows) {
+            // a bit for each row that attn_row does
+            uint32_t again = 0, lost = 0;
+#pragma unroll
+            for (int k = 0; k < R; ++k) lost |= l[k] > 0.f ? 0u : 1u << k;   // (not a number: too)
+            if (__ballot(odd != 0)) again = (1u << R) - 1;
+            else
+                for (uint32_t left = __builtin_amdgcn_readfirstlane(lost); left; left &= left - 1) {
+                    const uint32_t k = __builtin_ctz(left), tok = (it.strip * M + min(rbase + k, rows - 1)) / a.group;
+                    if (any_page(a, it, max(key_lo(a, it, tok), 0), key_hi(a, it, tok))) again |= 1u << k;
+                }
             if constexpr (PW > 1) {
 #pragma unroll
                 for (int k = 0; k < R; ++k)
@@ -603,7 +628,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
             }
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                if (rbase + k >= rows || (PW > 1 && k % PW != (int)pw)) continue;
+                if (rbase + k >= rows || (again >> k & 1) || (PW > 1 && k % PW != (int)pw)) continue;
                 const uint32_t row = it.strip * M + rbase + k, tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
                 AT y[V];
 #pragma unroll
@@ -619,6 +644,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
                 // (d_v is a multiple of 8, so of V)
                 if (lane * V < a.dv) __builtin_memcpy((AT *)a.out + tok * a.o_tok + head * a.o_head + lane * V, y, sizeof y);
             }
+            for (uint32_t k = PW > 1 ? pw : 0; k < R; k += PW)
+                if ((again >> k & 1) && rbase + k < rows) attn_row<AT, T, M>(a, it, rbase + k);
         }
     }
     if (!me.odd || pw) return;

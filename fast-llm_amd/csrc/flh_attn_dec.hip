@@ -57,7 +57,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     uint32_t u = attn_border(w, U, Ge);
     const uint32_t first_u = u;
     const uint32_t end = attn_border(w + 1, U, Ge);
-    bool odd = false;                                                 // a sum is not finite
+    bool odd = false;                                                 // a sum is not finite, or a row lost its weight
     while (u < end) {
         AttnItem it;
         walk.find(u, it);
@@ -91,8 +91,8 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             // first of the item instead.
             const bool real = r < rows && a.scale != 0.f;
             const AT * q = (const AT *)a.q + (it.r0 + (r < rows ? tok : 0u)) * a.q_tok + (r < rows ? head : it.kvh * a.group) * a.q_head;
-            rhi[mt] = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
-            rlo[mt] = a.window ? it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30) : 0;
+            rhi[mt] = key_hi(a, it, tok);
+            rlo[mt] = key_lo(a, it, tok);
             c[mt] = a.scale == 0.f ? 1.f : a.scale * 1.4426950408889634f;
             Eight<AT> x[DK / 32];
 #pragma unroll
@@ -295,6 +295,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         }
         __syncthreads();
         float * part = begins && ends ? nullptr : attn_part<M, DV>(a, w, begins);
+        bool lost = false;                                            // a row that has keys got no weight
         for (uint32_t e = threadIdx.x; e < M * DV / 4; e += 64 * W) {
             const uint32_t r = e / (DV / 4), d = e % (DV / 4) * 4, row = it.strip * M + r;
             if (row >= rows) continue;
@@ -316,11 +317,13 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                 }
             } else if (d < a.dv) {
                 const uint32_t tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
+                if (!(sum > 0.f)) lost = lost || key_hi(a, it, row / a.group) > max(key_lo(a, it, row / a.group), 0);
                 if (sum == 0.f) v = f32x4{0.f, 0.f, 0.f, 0.f};
                 else v /= sum;
                 store4((AT *)a.out + tok * a.o_tok + head * a.o_head + d, v[0], v[1], v[2], v[3]);
             }
         }
+        if (__ballot(lost)) odd = odd || any_page(a, it, it.lo, it.hi);
         u += nt;
         __syncthreads();                                              // the next item's stages
     }

@@ -82,7 +82,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
     uint32_t u = attn_border(w, U, Ge);
     const uint32_t first_u = u;
     const uint32_t end = attn_border(w + 1, U, Ge);
-    bool odd = false;                                                 // a sum is not finite
+    bool odd = false;                                                 // a sum is not finite, or a row lost its weight
     while (u < end) {
         AttnItem it;
         walk.find(u, it);
@@ -95,8 +95,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         const uint32_t head = it.kvh * a.group + row % a.group;
         const int32_t win = (int32_t)min(a.window, 1u << 30);
         // keys that the lane's row sees; that all of the wave's rows see
-        const int32_t rhi = a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
-        const int32_t rlo = win ? it.p0 + (int32_t)tok + 1 - win : 0;
+        const int32_t rhi = key_hi(a, it, tok), rlo = key_lo(a, it, tok);
         const uint32_t first = it.strip * M + 32 * wave;              // the wave's rows
         const bool here = first < rows;
         const int32_t tf = (int32_t)(first / a.group), tl = (int32_t)min(it.n - 1, (first + 31) / a.group);
@@ -386,8 +385,13 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                 for (int i = 0; i < 16; ++i) odd = odd || !finite(o[d][i]);
         }
         l += xor_lane(l, 32, lane);
+        const bool whole = begins && ends;
+        // a row that has keys got no weight
+        const bool lost = !(l > 0.f) & (row < rows);
+        if (__ballot(lost) && whole && any_page(a, it, it.lo, it.hi))
+            odd = odd || (lost & (key_hi(a, it, tok) > max(key_lo(a, it, tok), 0)));
         if (row < rows) {
-            if (begins && ends) {
+            if (whole) {
                 AT * out = (AT *)a.out + (it.r0 + tok) * a.o_tok + head * a.o_head;
                 const float f = 1.f / l;
 #pragma unroll

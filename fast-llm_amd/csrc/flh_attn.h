@@ -171,12 +171,14 @@ template <int M, int KT, int C> struct AttnWalk {
         base = b;
         const uint32_t s = min(b + lane, a.n_seq - 1);
         const bool real = b + lane < a.n_seq;
-        const uint32_t x = min(a.q_start[s], a.n_tok), y = min(a.q_start[s + 1], a.n_tok), kv = a.kv_len[s];
-        const uint32_t n = real && y > x ? y - x : 0;
+        const uint32_t first = a.q_start[s], last = a.q_start[s + 1], kv = a.kv_len[s];
+        const uint32_t x = min(first, a.n_tok), y = min(last, a.n_tok), n = real && y > x ? y - x : 0;
         // positions and keys behind 2^30 have no table entry (see the host's check)
         const int32_t k = (int32_t)min(kv, 1u << 30);
         const int32_t cap = (int32_t)min((uint64_t)k, (uint64_t)a.table_stride << a.sh);
-        const int32_t p0 = k - (int32_t)n;
+        // (rows that n_tok cuts off count for the positions of the others; a row behind
+        // 2^30 in front of the first key sees nothing there either)
+        const int32_t p0 = (int32_t)max((int64_t)k - (int64_t)(last > first ? last - first : 0u), -(int64_t)(1 << 30));
         const uint32_t ns = strips(n, a.group);
         int32_t lo, hi;
         uint32_t one = fresh(span(max(n, 1u), p0, cap, 0, lo, hi));

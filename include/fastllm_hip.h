@@ -454,10 +454,10 @@ typedef struct flh_rope_kv_p {
 int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, const flh_rope_kv_p * p, void * stream);
 
 /* Attention of new tokens over the paged cache.  Request s has query rows
- * q_start[s] .. q_start[s+1] (ascending, cut off at n_tok; rows of no request are left as
- * they are in out) and keys 0 .. kv_len[s] - 1, key j at token j % page_size of page
+ * q_start[s] .. q_start[s+1] (ascending; rows from n_tok on are not computed, rows of no
+ * request are left as they are in out) and keys 0 .. kv_len[s] - 1, key j at token j % page_size of page
  * table[s*table_stride + j / page_size].  causal: the rows are the last
- * tokens, row i of n at position p = kv_len - n + i, and see the keys
+ * tokens, row i of n = q_start[s+1] - q_start[s] at position p = kv_len - n + i, and see the keys
  * j <= p, with window > 0 also j > p - window; else every row sees every
  * key (an encoder's states as the cache) and window must be 0.  Query head h
  * reads kv head h / (n_head / n_kv_head).

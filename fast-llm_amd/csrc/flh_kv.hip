@@ -63,9 +63,15 @@ __device__ __forceinline__ uint32_t slot_of(uint32_t page, uint32_t at, uint32_t
     return page > (0xFFFFFFFEu >> sh) ? FLH_KV_NONE : (page << sh) | (at & ((1u << sh) - 1u));
 }
 
+// tokens [from, to) of a request, all in the page `page`, that have no slot
+__device__ __forceinline__ uint32_t lost_in(uint32_t page, uint64_t from, uint64_t to, uint32_t sh) {
+    if (slot_of(page, 0, sh) == FLH_KV_NONE) return (uint32_t)(to - from);
+    return slot_of(page, (uint32_t)(to - 1), sh) == FLH_KV_NONE;  // (a page's last slot may be that number itself)
+}
+
 __global__ __launch_bounds__(PLAN_T) void k_kv_plan(flh_kv_plan_p p, uint32_t sh, int rows_too) {
     __shared__ uint64_t ws[PLAN_T / 64], l_page[PLAN_T];
-    __shared__ uint32_t l_row[PLAN_T], l_held[PLAN_T], l_before[PLAN_T];
+    __shared__ uint32_t l_row[PLAN_T], l_rows[PLAN_T], l_held[PLAN_T], l_before[PLAN_T];
     const uint32_t tid = threadIdx.x;
     const uint64_t ps = 1ull << sh;
     uint64_t row0 = 0, page0 = p.taken_in ? *p.taken_in : 0, lost = 0;
@@ -83,29 +89,27 @@ __global__ __launch_bounds__(PLAN_T) void k_kv_plan(flh_kv_plan_p p, uint32_t sh
         const uint64_t first = page0 + scan_wg(need, ws, &sum) - need;
         const uint64_t pages = sum;
         l_row[tid] = r0;
+        l_rows[tid] = r1 - r0;
         l_held[tid] = (uint32_t)held;
         l_before[tid] = (uint32_t)before;
         l_page[tid] = first - page0;
         if (in) {
-            // rows with a slot: in the page begun before (if the table holds one), and
-            // in the new pages that the free list had
-            uint64_t ok = 0;
-            if (held < before << sh) {
-                const uint32_t g = p.table[(uint64_t)s * p.table_stride + before - 1];
-                if (slot_of(g, 0, sh) != FLH_KV_NONE) ok = min(kv, before << sh) - held;
-            }
-            const uint64_t got = first >= p.n_free ? 0 : min(need, p.n_free - first);
-            if (need) ok += min(kv, (before + got) << sh) - min(kv, before << sh);
-            lost += add - ok;
+            // rows without a slot: those cut off, those behind the table's row, and in the page
+            // begun before; the new pages' are counted where the pages are dealt
+            const uint64_t end_at = (before + need) << sh, begun = min(kv, before << sh);
+            lost += add - (r1 - r0) + (kv - max(min(kv, end_at), held));
+            if (begun > held) lost += lost_in(p.table[(uint64_t)s * p.table_stride + before - 1], held, begun, sh);
             p.q_start[s] = r0;
             p.kv_len[s] = sat32(kv);
         }
         __syncthreads();
         for (uint64_t i = tid; i < pages; i += PLAN_T) {
             const uint32_t q = owner(l_page, nb, i);
-            const uint64_t at = page0 + i;
-            p.table[(uint64_t)(base + q) * p.table_stride + l_before[q] + (i - l_page[q])] =
-                at < p.n_free ? p.free_pages[at] : FLH_KV_NONE;
+            const uint64_t at = page0 + i, pg = l_before[q] + (i - l_page[q]);
+            const uint32_t g = at < p.n_free ? p.free_pages[at] : FLH_KV_NONE;
+            p.table[(uint64_t)(base + q) * p.table_stride + pg] = g;
+            const uint64_t held = l_held[q];
+            lost += lost_in(g, max(held, pg << sh), min(held + l_rows[q], (pg + 1) << sh), sh);
         }
         if (rows_too) {
             const uint32_t e = (uint32_t)min(row0, (uint64_t)p.max_tok);

@@ -177,14 +177,15 @@ int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s) {
 
 // ------------------------------------------------------------------- rope --
 // cos and sin of pair `t` at its position: turn = pos * frac mod 2^64 is the
-// angle as a fraction of a turn, exact to 2^-33 of a turn for every 32-bit
-// position (frac is rounded once, to 2^-65).  The nearest quarter turn comes off in
-// integers, so the rest, at most an eighth of a turn, keeps 24 bits as a float.
+// angle as a fraction of a turn, off by at most |pos| * 2^-65 (frac is rounded once; below
+// 2^-34 for every 32-bit position).  The nearest quarter turn comes off in integers, so the
+// rest, at most an eighth of a turn, keeps 24 bits as a float however small it is: the sines of
+// slow pairs at near positions are as good as their cosines.
 __device__ __forceinline__ void rope_cs(const RopePair & t, const int32_t * pos, uint32_t pos_stride, uint32_t tok,
                                         float & c, float & s) {
     const uint64_t turn = (uint64_t)(int64_t)pos[(size_t)t.axis * pos_stride + tok] * t.frac;
-    const uint32_t hi = (uint32_t)(turn >> 32), q = (hi + 0x20000000u) >> 30;
-    const float r = (float)(int32_t)(hi - (q << 30)) * 0x1p-31f;  // half turns
+    const uint32_t q = (uint32_t)((turn + (1ull << 61)) >> 62);
+    const float r = (float)(int64_t)(turn - ((uint64_t)q << 62)) * 0x1p-63f;   // half turns
     float s0, c0;
     sincospif(r, &s0, &c0);
     const float a = q & 1 ? s0 : c0, b = q & 1 ? c0 : s0;

@@ -9,8 +9,10 @@
 #include <string>
 #include <vector>
 #include <atomic>
+#include <iterator>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <unordered_map>
 #include "../../include/fastllm_hip.h"
 #include "flh_common.h"
@@ -300,13 +302,14 @@ static void merge_tiles(const flh_task * t, uint32_t n, uint32_t & i, DotArgs & 
 
 using namespace flh;
 
-// The streams made by flh_stream_create.  (Never destroyed: threads may outlive
-// the statics.)
+// The streams made by flh_stream_create, and the others that calls have named.  (Never
+// destroyed: threads may outlive the statics.)
 namespace flh {
 namespace {
 struct StreamTurns {
     std::shared_mutex m;
     std::unordered_map<void *, std::shared_ptr<StreamTurn::State>> by_stream;
+    std::shared_ptr<StreamTurn::State> spare = std::make_shared<StreamTurn::State>();   // where memory is short
 };
 StreamTurns & turns() {
     static StreamTurns * t = new StreamTurns();
@@ -314,20 +317,32 @@ StreamTurns & turns() {
 }
 }  // namespace
 
+// Streams that were made elsewhere come and go unseen: past this many entries those that no
+// call holds are dropped (a later call makes a new one).
+constexpr size_t FOREIGN_MAX = 1024;
+
 StreamTurn::StreamTurn(void * stream, bool whole) : whole_(whole) {
+    StreamTurns & t = turns();
     {
-        StreamTurns & t = turns();
         std::shared_lock<std::shared_mutex> l(t.m);
         const auto it = t.by_stream.find(stream);
         if (it != t.by_stream.end()) st_ = it->second;
     }
-    if (!st_) return;
+    if (!st_) try {
+        auto made = std::make_shared<State>();
+        std::unique_lock<std::shared_mutex> l(t.m);
+        if (t.by_stream.size() >= FOREIGN_MAX)
+            for (auto it = t.by_stream.begin(); it != t.by_stream.end();)
+                it = it->second->device < 0 && it->second.use_count() == 1 ? t.by_stream.erase(it) : std::next(it);
+        st_ = t.by_stream.emplace(stream, std::move(made)).first->second;
+    } catch (const std::bad_alloc &) {
+        st_ = t.spare;
+    }
     std::lock_guard<std::mutex> l(st_->gate);                     // a waiting replay is next: calls that go on overlapping cannot keep it out
     if (whole_) st_->m.lock();
     else st_->m.lock_shared();
 }
 StreamTurn::~StreamTurn() {
-    if (!st_) return;
     if (whole_) st_->m.unlock();
     else st_->m.unlock_shared();
 }
@@ -615,9 +630,9 @@ int flh_graph_launch(void * ge, void * stream) {
     const graph_handle * h = (const graph_handle *)ge;
     if (!h) return set_error(FLH_ERR_ARG, "null graph");
     // A replay is one operation of its stream because its thread has the stream to
-    // itself meanwhile (every entry point that issues work takes part in that).  That
-    // holds for the runtime's launch too: three threads that launched graphs of six nodes
-    // on one stream at once were seen to leave the sums of seven dots behind one
+    // itself meanwhile (every entry point that issues work takes part in that, on any
+    // stream).  The runtime's launch needs that too: three threads that launched graphs of
+    // six nodes on one stream at once were seen to leave the sums of seven dots behind one
     // zeroing instead of four.  A chain is only for a stream made here, on the device in
     // force and not being captured.
     const StreamTurn turn(stream, true);

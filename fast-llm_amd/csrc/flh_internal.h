@@ -17,8 +17,9 @@ namespace flh {
 // issuing on that stream, and later ones wait for it, so no other thread's work
 // falls between its kernels.  The other calls do not exclude each other, and
 // streams never wait for one another (a turn is found by the stream's handle).
-// A stream that was not made by flh_stream_create has none (device() is -1),
-// and nothing to wait for: no replay on it is more than one runtime call.
+// Streams that were not made by flh_stream_create have theirs from the first call on
+// (device() is -1): the runtime's launch of a graph is not one operation to the launches
+// of other threads either.
 class StreamTurn {
 public:
     struct State {
@@ -30,7 +31,7 @@ public:
     ~StreamTurn();
     StreamTurn(const StreamTurn &) = delete;
     StreamTurn & operator=(const StreamTurn &) = delete;
-    int device() const { return st_ ? st_->device : -1; }
+    int device() const { return st_->device; }
 
 private:
     std::shared_ptr<State> st_;

@@ -184,11 +184,10 @@ int flh_event_destroy(void * event);
  * through this library comes before or after all of it.  On a stream of
  * flh_stream_create a short chain of kernels (at most 5, 7 with 0.5 MiB of
  * weights each on average, 16 with 12 MiB) is replayed kernel by kernel (less idle
- * time on the device; 2.6 to 4 us of the caller's time per kernel).  What other code issues
- * there directly (a HIP call on the handle) from another thread at the same time
- * may then fall between two of the kernels, and a replay that fails may have run
- * in part.  On any other stream, and for any other graph, a replay is the
- * runtime's own graph launch. */
+ * time on the device; 2.6 to 4 us of the caller's time per kernel); a replay of it that
+ * fails may have run in part.  On any other stream, and for any other graph, a replay is
+ * the runtime's own graph launch.  What other code issues there directly (a HIP call on the
+ * handle) from another thread at the same time may fall between the kernels of either. */
 int flh_graph_capture_begin(void * stream);
 int flh_graph_capture_end(void * stream, void ** graph_exec);
 int flh_graph_launch(void * graph_exec, void * stream);

@@ -12,9 +12,9 @@
 
 namespace flh {
 
-// Held by an entry point while it issues work on a stream.  A graph's replay
-// holds it whole: it waits for the calls that are
-// issuing on that stream, and later ones wait for it, so no other thread's work
+// Held by an entry point while it issues work on a stream.  A graph's replay, and a call
+// whose launches pass a workspace or a table on, holds it whole: it waits for the calls that
+// are issuing on that stream, and later ones wait for it, so no other thread's work
 // falls between its kernels.  The other calls do not exclude each other, and
 // streams never wait for one another (a turn is found by the stream's handle).
 // Streams that were not made by flh_stream_create have theirs from the first call on

@@ -118,7 +118,7 @@ int flh_kv_plan(const flh_kv_plan_p * p, void * stream) {
                            (const void *)p->slot, (const void *)p->pos, (const void *)p->info})
         if (off(q, 4)) return set_error(FLH_ERR_ARG, "kv plan: arrays must be 4-byte aligned");
     if (int rc = need_device()) return rc;
-    const StreamTurn turn(stream);
+    const StreamTurn turn(stream, true);                          // (two launches, as below)
     return launch_kv_plan(*p, (hipStream_t)stream);
 }
 
@@ -237,7 +237,9 @@ int flh_paged_attn(const flh_kv_cache * c, const flh_attn_p * p, void * stream) 
     }
     if (int rc = need_device()) return rc;
     if (p->n_tok == 0 || p->n_seq == 0) return FLH_OK;
-    const StreamTurn turn(stream);
+    // two launches that belong together: another thread's call in between would take the
+    // workspace, which calls on one stream may share
+    const StreamTurn turn(stream, true);
     return launch_attn(a, p->dtype, c->dtype, (hipStream_t)stream);
 }
 

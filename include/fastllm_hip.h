@@ -472,7 +472,8 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, con
  * request that the caller expects (it chooses the kernel, the results hold for
  * any).  ws: flh_paged_attn_ws_bytes of the same arguments (pointers and lengths
  * are not looked at), 16-byte aligned; its contents need not be kept or
- * cleared, but calls that may run at the same time need one each. */
+ * cleared.  Calls on one stream may share one, whichever threads make them; calls on
+ * several streams, and graphs that may be replayed at the same time, need one each. */
 typedef struct flh_attn_p {
     const void * q; void * out;
     const uint32_t * q_start, * kv_len, * table;

@@ -42,12 +42,31 @@ int check_cache(const flh_kv_cache * c) {
     return FLH_OK;
 }
 
-// bytes of [tok][head][d] rows at these strides, 0 for none
-uint64_t extent(uint32_t n_tok, uint64_t tok, uint32_t n_head, uint64_t head, uint32_t d, uintptr_t el) {
-    return n_tok && n_head ? ((n_tok - 1) * tok + (n_head - 1) * head + d) * el : 0;
-}
-bool overlap(const void * a, uint64_t na, const void * b, uint64_t nb) {
-    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+// [tok][head][d] elements at these strides
+struct Rows {
+    const void * p;
+    uint64_t tok, head;
+    uint32_t d;
+};
+typedef unsigned __int128 u128;
+// Whether two sets of n_tok x n_head rows (of el bytes an element, both counts > 0) share a
+// byte.  Their extents tell, or, where both take equal steps, the places within a
+// step: columns of the same rows, or heads that stand in turn, are apart.  Else: yes.
+bool overlap(const Rows & a, const Rows & b, uint32_t n_tok, uint32_t n_head, uintptr_t el) {
+    const u128 pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    auto row = [&](const Rows & r) { return ((u128)(n_head - 1) * r.head + r.d) * el; };
+    auto all = [&](const Rows & r) { return (u128)(n_tok - 1) * r.tok * el + row(r); };
+    if (pa + all(a) <= pb || pb + all(b) <= pa) return false;
+    // pieces of na and nb bytes, each a multiple of `step` bytes behind the first
+    auto apart = [&](u128 step, u128 na, u128 nb) {
+        if (step == 0 || na > step || nb > step) return false;
+        const u128 at = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;
+        return at >= na && at + nb <= step;
+    };
+    if (a.tok == b.tok && apart((u128)a.tok * el, row(a), row(b))) return false;
+    if (a.head == b.head && a.head && (n_tok == 1 || (a.tok % a.head == 0 && b.tok % b.head == 0)) &&
+        apart((u128)a.head * el, a.d * el, b.d * el)) return false;
+    return true;
 }
 
 int check_rope(const flh_rope_table * r, uint32_t d, const int32_t * pos) {
@@ -61,7 +80,7 @@ int check_turned(const void * x, uint64_t x_tok, uint64_t x_head, const void * y
     const uintptr_t el = elem(dtype);
     if (!x || !y || off(x, el) || off(y, el)) return set_error(FLH_ERR_ARG, "rope: x and y must be non-null and element aligned");
     if (x == y && x_tok == y_tok && x_head == y_head) return FLH_OK;
-    if (overlap(x, extent(n_tok, x_tok, n_head, x_head, d, el), y, extent(n_tok, y_tok, n_head, y_head, d, el)))
+    if (overlap({x, x_tok, x_head, d}, {y, y_tok, y_head, d}, n_tok, n_head, el))
         return set_error(FLH_ERR_ARG, "rope: y overlaps x with other strides or another address");
     return FLH_OK;
 }
@@ -228,8 +247,7 @@ int flh_paged_attn(const flh_kv_cache * c, const flh_attn_p * p, void * stream) 
             return set_error(FLH_ERR_ARG, "attention: q and out must be non-null and element aligned");
         if (!p->q_start || !p->kv_len || off(p->q_start, 4) || off(p->kv_len, 4) || off(p->table, 4) || (!p->table && p->table_stride))
             return set_error(FLH_ERR_ARG, "attention: q_start, kv_len and table must be non-null and 4-byte aligned");
-        if (overlap(p->q, extent(p->n_tok, p->q_tok, p->n_head, p->q_head, c->d_k, el), p->out,
-                    extent(p->n_tok, p->o_tok, p->n_head, p->o_head, c->d_v, el)))
+        if (overlap({p->q, p->q_tok, p->q_head, c->d_k}, {p->out, p->o_tok, p->o_head, c->d_v}, p->n_tok, p->n_head, el))
             return set_error(FLH_ERR_ARG, "attention: out overlaps q");
         const size_t need = attn_ws_bytes(a, p->dtype, c->dtype);
         if (need && (!p->ws || off(p->ws, 16) || p->ws_bytes < need))

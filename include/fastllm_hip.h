@@ -468,7 +468,8 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, con
  * tokens).  dtype of q and out: F32 over either
  * cache (products as accurate as fp32 ones), or the cache's own.  Sums, maxima
  * and the softmax are fp32.  scale: finite, >= 0.  q and out: any element strides,
- * aligned to an element; out must not overlap q.  max_q: the most rows of a
+ * aligned to an element; out must not overlap q (other columns of the same rows, or
+ * beside each head, do not).  max_q: the most rows of a
  * request that the caller expects (it chooses the kernel, the results hold for
  * any).  ws: flh_paged_attn_ws_bytes of the same arguments (pointers and lengths
  * are not looked at), 16-byte aligned; its contents need not be kept or

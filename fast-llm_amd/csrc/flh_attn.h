@@ -335,11 +335,6 @@ template <typename T> __device__ __forceinline__ typename VecOf<T>::v4 ld_tr(uin
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)at));
 }
 
-template <typename T> __device__ __forceinline__ float load_f(const T * p) {
-    T v;
-    __builtin_memcpy(&v, p, sizeof v);
-    return (float)v;
-}
 // four values as AT, at any element alignment
 template <typename AT> __device__ __forceinline__ void store4(AT * p, float a, float b, float c, float d) {
     const typename VecOf<AT>::v4 v = {(AT)a, (AT)b, (AT)c, (AT)d};
@@ -419,7 +414,6 @@ struct AttnPlan {
     uint32_t grid, m, dv, min_units;
     size_t ws;
 };
-enum { ATTN_DIMS = 4 };
 // the smallest compiled (d_k, d_v) that holds both: 0: 64 / 64, 1: 128 / 128, 2: 192 / 128, 3: 256 / 256
 inline int attn_dims(const AttnArgs & a) {
     return a.dk <= 64 && a.dv <= 64 ? 0 : a.dk <= 128 && a.dv <= 128 ? 1 : a.dk <= 192 && a.dv <= 128 ? 2 : 3;

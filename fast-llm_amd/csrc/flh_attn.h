@@ -72,7 +72,9 @@ template <typename T, int NS> __device__ __forceinline__ void split(float x, flo
     }
 }
 // The weights exp2(score - max) are made 2^7 times larger for f16 terms, so that
-// small ones do not become subnormal there; the sum has the same factor.  (A
+// small ones do not become subnormal there; the sum has the same factor.  f16's smallest step,
+// 2^-24, is then 2^-31 of a weight of 1: weights are right to 2^-32 of the row's largest,
+// and n of them that are all far below it to n times that.  (A
 // factor, not 7 more in the exponent: that would cost the largest weights, whose
 // exponent is near 0, their last bits.)
 template <typename T> constexpr float weight_unit() { return __is_same(T, _Float16) ? 0x1p7f : 1.f; }
@@ -513,7 +515,7 @@ __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32
 // Behind the main kernel.  Workgroups (w, y): the parts of w's note are added up in
 // order, four rows a wave; PW waves share the parts of the same rows (a few rows of
 // many parts: latency).  Rows of items with sums that are not finite, and rows that lost all their
-// weight, are done by attn_row instead.  The parts' bytes bound it where there are many (16 us for those of 512
+// weight, are done by attn_row instead.  The parts' bytes bound it where there are many (18 us for those of 512
 // workgroups with 128 rows of 128, up to 134 KB each), else a launch (4 us).
 template <typename AT, typename T, int M, int KT, int DV, int PW, int C>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {

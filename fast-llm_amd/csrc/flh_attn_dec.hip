@@ -1,10 +1,11 @@
 // flh_attn_dec.hip -- attention of few rows per kv head (single tokens, short
 // verify steps): the keys and values of a request are read once, so HBM is
-// what bounds it.  32 / 8 heads of 128: 4 requests of 131072 keys in bf16 take 355 us
-// (6.0 TB/s), 64 requests of up to 8192 keys with fp32 activations over f16 205 us (5.0
-// TB/s, ragged), one request of 4001 keys 14.8 us: two launches, each with a chain of
-// loads (lengths, page numbers, keys).  16 requests of up to 8 tokens in fp32 over bf16, 77 us:
-// there the products of three terms and the splitting bound it.
+// what bounds it.  32 / 8 heads of 128: 4 requests of 131072 keys in bf16 take 358 us
+// (6.0 TB/s; a kernel that only reads 4 GiB reaches 6.1, one of 1 GiB 5.7), 64 requests of up to 8192
+// keys with fp32 activations over f16 203 us (5.05 TB/s; 188 with equal lengths, 5.7 TB/s), one
+// request of 4001 keys 15 us: two launches, each with a chain of loads (lengths, page
+// numbers, keys).  16 requests of up to 8 tokens in fp32 over bf16, 73 us: there the products
+// of three terms and the splitting bound it.
 #include "flh_attn.h"
 #include "flh_status.h"
 

@@ -14,18 +14,24 @@ namespace flh {
 // scores are multiplied while this tile's weights are made (an instruction of each in
 // turn), so that neither unit waits for the other.
 // Roundings: with 16-bit activations a weight is rounded to the cache's type for the product
-// with V (half a step of that type, as much as the rounding of the result), sums stay fp32;
-// fp32 activations and their weights are split into terms that hold all their bits, so only
-// fp32 accumulation rounds.
-// 8192 tokens, causal, 32 / 8 heads of 128: 620 to 640 us in bf16 (860 TFLOP/s; a large library
-// product reaches 1220), of which k_attn_join is 16.  The matrix cores are busy 40% of the
-// time (at about 1.9 GHz under this load), the vector units about as long.  fp32 over f16 (two terms, twice the
-// products) 612 us for 5 ragged chunks (830 TFLOP/s of products).  32 rows a wave and two
+// with V (half a step of that type, as much as the rounding of the result; against the
+// formula in 64 bits results are off by about 1.3 times what one rounding of them costs), while the
+// sum below is of the weights as they were, in fp32.  fp32 activations and their weights are split
+// into two f16 terms, right to 2^-22 of a value, or three bf16 terms, to 2^-24; then only fp32
+// accumulation rounds.
+// 8192 tokens, causal, 32 / 8 heads of 128: 642 us in bf16 (857 TFLOP/s; a large library
+// product reaches 1220), of which k_attn_join is 18.  The matrix cores are busy 42% of the time (at about
+// 1.8 GHz under this load) and the vector instructions take as long: they hardly overlap.  fp32
+// over f16 (two terms, twice the products) 622 us for 5 ragged chunks (816 TFLOP/s of products).  32 rows a wave and two
 // workgroups a CU: the registers hold a wave's sums, queries and two tiles' scores (256); a
 // third workgroup of narrow heads (64) would need 168 registers, spilled, and took 69 us
 // instead of 63 for 8 x 20 heads over 1500 keys.
-// C of the line of work.  8192 tokens of 32 / 8 heads in bf16 take 690 us with 0 (the first
-// workgroup has 32 items and takes a third longer than most), 648 with 3.
+// C of the line of work.  With 0 the first workgroup of a causal prompt has most items and
+// takes a third longer than the others.  us with 0 / 1 / 3 / 6, 32 / 8 heads: 8192 tokens in bf16
+// 738 / 700 / 638 / 636, 2048 104 / 89 / 76 / 75; 4096 of heads of 64 166 / 146 / 130 / 133, 80 218 /
+// 194 / 176 / 178, 192/128 398 / 363 / 298 / 296, 256 604 / 542 / 446 / 425; 5 chunks in fp32 over f16 659 /
+// 649 / 626 / 626, over bf16 797 / 776 / 751 / 753, of heads of 256 1389 / 1332 / 1273 / 1254; 8 x 20 heads
+// of 64 over 1500 keys 58 / 58 / 55 / 58; 64 requests of 40 rows over 500 keys 132 / 136 / 136 / 136.
 constexpr int PRE_ITEM = 3;
 template <int DK, int DV> struct PreShape {
     static constexpr int W = 4;                                       // waves

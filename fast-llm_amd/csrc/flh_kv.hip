@@ -17,7 +17,8 @@ namespace flh {
 // workgroup, so taken and kv_len may be updated in place: nobody else reads
 // them.  Sums are 64-bit (a garbage length costs its own rows only).  A launch and
 // a chain of loads, scans and searches bound it: 64 requests of a token each take
-// 6.7 us, 500 with 64000 rows 11.2 (two launches).  Rows in the same launch cost one
+// 7.0 us, 500 with 64000 rows 11.7 (two launches).  (A thread of 1024
+// has 128 registers: five are spilled.)  Rows in the same launch cost one
 // workgroup 1 us for about 1200 of them, a second launch 4 to 5 us: 2048 rows take 8.8
 // us in one and 12.1 in two, 8192 13.4 and 12.2, 16384 19.9 and 12.1.
 constexpr uint32_t PLAN_T = 1024;
@@ -208,8 +209,8 @@ template <int N, typename T> __device__ __forceinline__ void st_vec(T * p, const
 // angles: a workgroup makes each once, behind the loads of its threads' first
 // units, and every head reads them from LDS.  Bytes bound it: 4999 tokens of 32 + 8 heads
 // of 128 with values in bf16 take 27 us (4.5 TB/s; a large copy reaches 5.1), 1000 tokens
-// of 16 + 16 heads of 192 in fp32 11.0 us (5.0 TB/s), one token 6.9 us, a launch and
-// its chain of loads.  One thread per pair with its own angle took 64.5, 23.6 and 7.3;
+// of 16 + 16 heads of 192 in fp32 11.0 us (5.0 TB/s), one token 7.4 us, a launch and
+// its chain of loads (2.8 us on the device).  One thread per pair with its own angle took 64.5, 23.6 and 7.3;
 // two units in flight instead of one 30.6.
 struct RopeUnits {
     uint32_t pu, u, n, step_h, step_e;     // a head's pair units and all its units, their number, and a step in (head, unit)
@@ -319,8 +320,9 @@ static int rope_n(RopeArgs a, hipStream_t s) {
     ru.u = ru.pu + (rest + 2 * N - 1) / (2 * N);
     ru.n = ru.u * (a.n_head + nk);
     const uint32_t most = (uint32_t)((std::max<uint64_t>(ru.n, nk * a.dv / N) + ROPE_T - 1) / ROPE_T);
-    // few tokens: workgroups share a token's units (one token of 128 + 8 heads of 192: 8.3 us
-    // with a unit a thread, 11.1 in one workgroup; of 32 + 8 heads of 128 the same)
+    // Few tokens: workgroups share a token's units.  us so / with one workgroup a token, 128 + 8
+    // heads of 192 in bf16: 4 tokens 7.1 / 7.7, 64 6.7 / 8.1, 256 8.1 / 9.5, 512 12.7 / 12.8; 32 + 8 heads of 128 in
+    // fp32 7.3 / 7.7, 7.0 / 6.8, 6.7 / 7.1, 6.8 / 7.0; one token 7.3 to 7.5 either way.
     const uint32_t parts = std::max(1u, std::min(most, 512 / a.n_tok));
     ru.step_h = parts * ROPE_T / ru.u;
     ru.step_e = parts * ROPE_T % ru.u;

@@ -442,8 +442,8 @@ int flh_rope(const flh_rope_table * r, uint32_t dtype, const void * x, uint64_t 
  * to its dtype; one launch.  Tokens whose slot is not in the cache (FLH_KV_NONE)
  * write nothing there.  Slots of one call must differ.  r = NULL: nothing is
  * rotated (pos is not read).  q, k and v may be columns of one product's rows
- * (any element strides); q_out as y of flh_rope; the cache must not overlap
- * them. */
+ * (any element strides); q_out as y of flh_rope, and apart from k and v; the cache must not
+ * overlap them. */
 typedef struct flh_rope_kv_p {
     const void * q; void * q_out; const void * k; const void * v;
     const int32_t * pos; const uint32_t * slot;
@@ -465,14 +465,19 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, con
  * -infinity; a q.k past the range of fp32 is infinite); keys not seen have no part in it, whatever the cache
  * holds there.  Keys whose table entry is no page of the cache, or lies
  * behind the table's row, are not seen (kv_len and a table's row: at most 2^30
- * tokens).  dtype of q and out: F32 over either
- * cache (products as accurate as fp32 ones), or the cache's own.  Sums, maxima
- * and the softmax are fp32.  scale: finite, >= 0.  q and out: any element strides,
+ * tokens).  dtype of q and out: F32 over either cache, or the cache's own.  Scores,
+ * maxima, weights and sums are fp32.  Into the products go, with F32, queries and weights in two
+ * f16 terms (right to 2^-22 of a value) or three bf16 terms (2^-24); else weights rounded once to the
+ * cache's type (the sum that they are divided by is of the unrounded ones).  Over an F16 cache a
+ * weight is besides right only to 2^-32 of its row's largest.  scale: finite, >= 0.  q and out: any element strides,
  * aligned to an element; out must not overlap q (other columns of the same rows, or
  * beside each head, do not).  max_q: the most rows of a
  * request that the caller expects (it chooses the kernel, the results hold for
- * any).  ws: flh_paged_attn_ws_bytes of the same arguments (pointers and lengths
- * are not looked at), 16-byte aligned; its contents need not be kept or
+ * any).  Rows that see an infinite or NaN key or value, and those that share a
+ * workgroup with one, are done one by one, which takes the call 30 to 300 times as
+ * long.  ws: flh_paged_attn_ws_bytes of the same arguments (pointers and lengths
+ * are not looked at; by the chosen kernel and the widths, not by the rows: 4 to 70 MB on 256
+ * CUs), 16-byte aligned; its contents need not be kept or
  * cleared.  Calls on one stream may share one, whichever threads make them; calls on
  * several streams, and graphs that may be replayed at the same time, need one each. */
 typedef struct flh_attn_p {

@@ -132,6 +132,7 @@ int flh_kv_plan(const flh_kv_plan_p * p, void * stream) {
         return set_error(FLH_ERR_ARG, "kv plan: null argument");
     if ((uint64_t)p->table_stride * p->page_size > (1ull << 31))
         return set_error(FLH_ERR_UNSUPPORTED, "kv plan: table_stride * page_size must be at most 2^31");
+    if (p->max_tok > (1u << 31)) return set_error(FLH_ERR_UNSUPPORTED, "kv plan: max_tok must be at most 2^31");
     for (const void * q : {(const void *)p->held, (const void *)p->add, (const void *)p->free_pages, (const void *)p->taken_in,
                            (const void *)p->taken, (const void *)p->table, (const void *)p->q_start, (const void *)p->kv_len,
                            (const void *)p->slot, (const void *)p->pos, (const void *)p->info})

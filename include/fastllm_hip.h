@@ -400,7 +400,8 @@ typedef struct flh_kv_cache {
  * entry is FLH_KV_NONE, and *taken > n_free), when its page lies behind
  * the table's row, or when its table entry is no page.  info[0]: rows;
  * info[1]: new tokens without a slot (0: all is well; those cut off at max_tok
- * count).  page_size: a power of two up to 65536.  pos and info may be NULL.
+ * count).  page_size: a power of two up to 65536; max_tok and table_stride * page_size at
+ * most 2^31.  pos and info may be NULL.
  * kv_len may be held and taken may be taken_in (a captured step then advances
  * its requests by itself); nothing else may overlap.  free_pages and table
  * hold the page numbers of a flh_kv_cache. */

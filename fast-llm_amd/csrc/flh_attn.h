@@ -47,7 +47,8 @@ __device__ __forceinline__ f32x16 mma32(VecOf<__bf16>::v8 a, VecOf<__bf16>::v8 b
 }
 
 // 16-bit terms that an fp32 value is split into for the matrix cores: two f16
-// (11 + 11 bits) or three bf16 (8 + 8 + 8); 16-bit activations take one.
+// (11 + 11 bits) or three bf16 (8 + 8 + 8); 16-bit activations take one (their weights two
+// in the kernel for few rows).
 template <typename AT, typename T> constexpr int split_terms() {
     return !__is_same(AT, float) ? 1 : __is_same(T, _Float16) ? 2 : 3;
 }

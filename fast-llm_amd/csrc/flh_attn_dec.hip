@@ -17,6 +17,10 @@ namespace flh {
 // lane holds one row's scores of 8 keys, which are, as they are, the operand of
 // O^T += V^T P^T; V^T comes out of LDS by transposing reads.  The W waves of
 // a workgroup take turns of 32 keys of a tile and join their sums at its end.
+// Weights go into the products with V in two terms (three in fp32 over bf16) with 16-bit
+// activations too: one would cost as much precision as the rounding of the result (4
+// requests of 131072 keys in bf16: off by 0.0023 of the results, 0.0016 so, which is that rounding),
+// and a second product costs 0 to 2.5% here (358 and 360 us; 64 requests of up to 8192 keys 195 and 198).
 template <int DK, int DV> struct DecShape {
     static constexpr int W = DK + DV <= 256 ? 4 : 2;                  // waves
     static constexpr int KT = 32 * W;                                 // keys of a unit
@@ -33,7 +37,7 @@ template <typename AT, typename T, int DK, int DV, int MT>
 __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) {
     typedef DecShape<DK, DV> P;
     typedef typename VecOf<T>::v8 v8;
-    constexpr int W = P::W, KT = P::KT, NST = P::NST, M = 16 * MT, NS = split_terms<AT, T>();
+    constexpr int W = P::W, KT = P::KT, NST = P::NST, M = 16 * MT, NS = split_terms<AT, T>(), NW = NS > 1 ? NS : 2;
     constexpr int NK = DK / 16, NV = DV / 16, ND = NK + NV;           // DMAs of a tile
     extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
     const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, q4 = lane >> 4;
@@ -169,7 +173,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                         for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mma16(kf, qf[t2][mt][d], s[mt][kt]);
                 }
             const bool whole = vm == 0xFFFFFFFFu && k0 >= all_lo && k0 + 32 <= all_hi;
-            v8 pf[NS][MT];
+            v8 pf[NW][MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 float x[8], top = -INFINITY;
@@ -198,10 +202,10 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                 for (int j = 0; j < 8; ++j) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(x[j], c[mt], -base)) * weight_unit<T>();
                     sum += p;
-                    T h[NS];
-                    split<T, NS>(p, h);
+                    T h[NW];
+                    split<T, NW>(p, h);
 #pragma unroll
-                    for (int t2 = 0; t2 < NS; ++t2) pf[t2][mt][j] = h[t2];
+                    for (int t2 = 0; t2 < NW; ++t2) pf[t2][mt][j] = h[t2];
                 }
                 l[mt] += sum;
             }
@@ -215,7 +219,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                     for (int j = 0; j < 4; ++j) vf[4 * kt + j] = r4[j];
                 }
 #pragma unroll
-                for (int t2 = NS - 1; t2 >= 0; --t2)
+                for (int t2 = NW - 1; t2 >= 0; --t2)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) o[mt][d] = mma16(vf, pf[t2][mt], o[mt][d]);
             }

@@ -16,7 +16,8 @@ namespace flh {
 // Roundings: with 16-bit activations a weight is rounded to the cache's type for the product
 // with V (half a step of that type, as much as the rounding of the result; against the
 // formula in 64 bits results are off by about 1.3 times what one rounding of them costs), while the
-// sum below is of the weights as they were, in fp32.  fp32 activations and their weights are split
+// sum below is of the weights as they were, in fp32.  A second term, as for few rows, would take
+// 31% longer (8192 tokens in bf16: 816 us beside 621).  fp32 activations and their weights are split
 // into two f16 terms, right to 2^-22 of a value, or three bf16 terms, to 2^-24; then only fp32
 // accumulation rounds.
 // 8192 tokens, causal, 32 / 8 heads of 128: 642 us in bf16 (857 TFLOP/s; a large library

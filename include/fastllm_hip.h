@@ -468,9 +468,10 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, con
  * behind the table's row, are not seen (kv_len and a table's row: at most 2^30
  * tokens).  dtype of q and out: F32 over either cache, or the cache's own.  Scores,
  * maxima, weights and sums are fp32.  Into the products go, with F32, queries and weights in two
- * f16 terms (right to 2^-22 of a value) or three bf16 terms (2^-24); else weights rounded once to the
- * cache's type (the sum that they are divided by is of the unrounded ones).  Over an F16 cache a
- * weight is besides right only to 2^-32 of its row's largest.  scale: finite, >= 0.  q and out: any element strides,
+ * f16 terms (right to 2^-22 of a value) or three bf16 terms (2^-24); else weights in two terms
+ * (2^-22, bf16 2^-16) where max_q * n_head / n_kv_head <= 32, and rounded once to the cache's type
+ * where it is more (the sum that they are divided by is of the unrounded ones).  Over an F16
+ * cache a weight is besides right only to 2^-32 of its row's largest.  scale: finite, >= 0.  q and out: any element strides,
  * aligned to an element; out must not overlap q (other columns of the same rows, or
  * beside each head, do not).  max_q: the most rows of a
  * request that the caller expects (it chooses the kernel, the results hold for

@@ -426,7 +426,7 @@ AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype);
 int launch_attn_dec(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 
-// One row by one wave, a key a lane, in fp32: for items whose sums are not
+// One row by one wave, a key a lane, in fp32 (scores from sums in 64 bits): for items whose sums are not
 // finite, and rows that have keys but no weight: all their scores are -infinity, or
 // finite ones passed fp32's range when they were multiplied by log2(e).  0 * inf is NaN, so in a matrix product a key
 // that a row does not see (weight 0), or the vanished low term of a split weight, carries an
@@ -447,12 +447,12 @@ template <typename AT, typename T, int M> __device__ __forceinline__ void attn_r
         float t = -INFINITY;
         if (in) {
             const T * k = (const T *)(uintptr_t)row_at(kb, pg, a.k_page, (uint32_t)j & a.pmask, a.k_tok);
-            t = 0.f;
+            double dot = 0;                                           // (q.k may pass what scale q.k does not)
             for (uint32_t i = 0; i < a.dk; i += 8) {
                 const Eight<T> x = load8(k + i);
-                for (int e = 0; e < 8; ++e) t = fmaf((float)q[i + e], (float)x.v[e], t);
+                for (int e = 0; e < 8; ++e) dot = fma((double)(float)q[i + e], (double)(float)x.v[e], dot);
             }
-            t *= a.scale;
+            t = (float)(dot * (double)a.scale);
         }
         float top = t;
         for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));

@@ -463,7 +463,8 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * cache, con
  * reads kv head h / (n_head / n_kv_head).
  *   out[row][head] = sum_j softmax_j(scale q.k_j) v_j   over the keys seen,
  * 0 for a row that sees none (not a number for one that sees keys, all with scores of
- * -infinity; a q.k past the range of fp32 is infinite); keys not seen have no part in it, whatever the cache
+ * -infinity; a score past the range of fp32 is infinite, and a q.k below it, whatever the scale, may
+ * count as -infinity); keys not seen have no part in it, whatever the cache
  * holds there.  Keys whose table entry is no page of the cache, or lies
  * behind the table's row, are not seen (kv_len and a table's row: at most 2^30
  * tokens).  dtype of q and out: F32 over either cache, or the cache's own.  Scores,

@@ -125,3 +125,26 @@ def test_no_page_is_not_no_weight(flh, gpu, act, cdt, n):
     assert (got[:n] == 0).all() and (got[n:n + n - n // 2] == 0).all()
     assert torch.isnan(got[2 * n:3 * n, 0]).all()
     assert torch.isfinite(got[2 * n:3 * n, 4:]).all()
+
+
+@pytest.mark.parametrize("cdt,size", [("F16", 1e37), ("BF16", 1e37), ("F16", 1e-37)])
+@pytest.mark.parametrize("n", [2, 6, 40])
+@pytest.mark.parametrize("keys", [150, 9001])
+def test_rows_done_again_at_any_size(flh, gpu, cdt, size, n, keys):
+    """Rows that are done again beside one that is not a number hold what they would hold
+    alone, also where q.k passes the range of fp32 and scale q.k does not."""
+    c = Case(flh, gpu, "F32", cdt, 4, 2, 64, 64, 16, "head", [(n, keys), (n, n)], 44, scale=0.1 / size)
+    c.q *= size
+    if size > 1:
+        c.cache.view[0].mul_(50.0)                     # q.k of up to about 1e39 and more
+        c.scale = c.p.scale = 0.002 / size
+    for j in (keys - 1, keys - 2):
+        c.cache.view[1][(*token(c, 0, j), 0, 9)] = math.nan
+    push(c)
+    c.run()
+    got = heads_of(c, c.result())[:c.n_tok]
+    out, mag, amp = [t[:c.n_tok] for t in attn_oracle(c.q, c.rows, c.kv_len, c.table, c.cache, c.group, c.scale, True, 0)]
+    lim = attn_bound(out, mag, amp, "F32", 64, keys)
+    nan = torch.isnan(out)
+    assert nan.any() and torch.equal(torch.isnan(got), nan)
+    assert ((got - out).abs() <= lim)[~nan].all()

@@ -23,7 +23,7 @@ namespace flh {
 // 8192 tokens, causal, 32 / 8 heads of 128: 642 us in bf16 (857 TFLOP/s; a large library
 // product reaches 1220), of which k_attn_join is 18.  The matrix cores are busy 42% of the time (at about
 // 1.8 GHz under this load) and the vector instructions take as long: they hardly overlap.  fp32
-// over f16 (two terms, twice the products) 622 us for 5 ragged chunks (816 TFLOP/s of products).  32 rows a wave and two
+// over f16 (two terms, twice the products) 626 us for 5 ragged chunks (812 TFLOP/s of products).  32 rows a wave and two
 // workgroups a CU: the registers hold a wave's sums, queries and two tiles' scores (256); a
 // third workgroup of narrow heads (64) would need 168 registers, spilled, and took 69 us
 // instead of 63 for 8 x 20 heads over 1500 keys.

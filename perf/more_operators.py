@@ -584,7 +584,7 @@ def _own_attn(st):
             table=st["table"].data_ptr(), q_tok=q.stride(0), q_head=q.stride(1), o_tok=o.stride(0), o_head=o.stride(1),
             dtype=flh.Dtype[c["act"].upper()], n_head=c["heads"], n_seq=c["seqs"], n_tok=st["rows"], max_q=st["max_q"],
             table_stride=st["table"].shape[1], scale=c["dk"] ** -0.5, causal=1, window=c["window"])
-        p.ws_bytes = flh.paged_attn_ws_bytes(st["cache"], p)
+        p.ws_bytes = flh.tree_attn_ws_bytes(st["cache"], p)
         st["ws"] = torch.empty(max(p.ws_bytes, 1), dtype=torch.uint8, device=DEV)
         p.ws = st["ws"].data_ptr()
         st["p"] = p

@@ -493,7 +493,7 @@ def _plain_pages(st):
     fresh = torch.where(at < n_free, free[at.clamp(max=n_free - 1)], -1)
     mine = table[src]
     last = mine.gather(1, full[:, None].clamp(max=table.shape[1] - 1))[:, 0]
-    table[dst] = torch.where(j < full[:, None], mine, torch.where((j == full[:, None]) & (rest > 0)[:, None], fresh[:, None], -1))
+    table[dst] = torch.where(j < full[:, None], mine, torch.where((j == full[:, None]) & (rest > 0)[:, None], fresh[:, None], table[dst]))
     pages = mine[j < full[:, None]].long()
     shared.index_add_(0, pages, torch.ones_like(pages, dtype=torch.int32))
     kv_len[dst] = held.int()
@@ -524,7 +524,7 @@ def _plain_pages(st):
     shared.copy_((shared - count).clamp(min=0))
     table.masked_fill_(gone, -1)
     table.copy_(torch.where(own_one[:, None] & (j == after[:, None] - 1), fresh[:, None], table))
-    to = top - back.shape[0] + torch.arange(back.shape[0], device=DEV)
+    to = top - 1 - torch.arange(back.shape[0], device=DEV)                # one after another: the last is taken next
     free[to[to >= 0]] = back[to >= 0].int()
     kv_len.copy_(keep.int())
     st["taken"].copy_((top - back.shape[0]).clamp(min=0).int())
@@ -642,9 +642,9 @@ def _own_pages(st):
                                  **both, **lists(st["last"]))
     s = _stream(flh)
     flh.kv_fork(st["fork"], s)
-    flh.kv_copy(st["caches"], st["copies"][0], st["copies"][1], st["copies"][2], st["copies"].shape[1], s)
+    flh.kv_copy(st["caches"], *[t.data_ptr() for t in st["copies"]], st["copies"].shape[1], s)
     flh.kv_trim(st["trim"], s)
-    flh.kv_copy(st["caches"], st["last"][0], st["last"][1], st["last"][2], st["last"].shape[1], s)
+    flh.kv_copy(st["caches"], *[t.data_ptr() for t in st["last"]], st["last"].shape[1], s)
     return {k: st[v] for k, v in PAGES.items()}
 
 

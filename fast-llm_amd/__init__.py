@@ -187,6 +187,54 @@ class AttnP(C.Structure):
                 ("table_stride", C.c_uint32), ("causal", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float)]
 
 
+class TreePlanP(C.Structure):
+    """flh_tree_plan_p (pointers are device addresses)."""
+    _fields_ = [("q_start", C.c_void_p), ("parent", C.c_void_p), ("kv_len", C.c_void_p), ("mask", C.c_void_p),
+                ("depth", C.c_void_p), ("pos", C.c_void_p), ("n_seq", C.c_uint32), ("n_tok", C.c_uint32),
+                ("mask_stride", C.c_uint32), ("window", C.c_uint32)]
+
+
+class TreeP(C.Structure):
+    """flh_tree_p (pointers are device addresses)."""
+    _fields_ = [("mask", C.c_void_p), ("depth", C.c_void_p), ("mask_stride", C.c_uint32)]
+
+
+class VerifyP(C.Structure):
+    """flh_verify_p (pointers are device addresses, strides in elements); max_child is 1 unless given."""
+    _fields_ = [("target", C.c_void_p), ("draft", C.c_void_p), ("q_start", C.c_void_p), ("token", C.c_void_p),
+                ("parent", C.c_void_p), ("inv_temp", C.c_void_p), ("u_accept", C.c_void_p), ("u_next", C.c_void_p),
+                ("kv_len", C.c_void_p), ("n_path", C.c_void_p), ("path", C.c_void_p), ("next", C.c_void_p), ("logp", C.c_void_p),
+                ("len", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t), ("t_row", C.c_uint64), ("d_row", C.c_uint64),
+                ("dtype", C.c_uint32), ("n_seq", C.c_uint32), ("n_tok", C.c_uint32), ("vocab", C.c_uint32),
+                ("path_stride", C.c_uint32), ("max_child", C.c_uint32)]
+
+    def __init__(self, **kw):
+        super().__init__(**{"max_child": 1, **kw})
+
+
+class KvCompactP(C.Structure):
+    """flh_kv_compact_p (pointers are device addresses)."""
+    _fields_ = [("q_start", C.c_void_p), ("slot", C.c_void_p), ("n_path", C.c_void_p), ("path", C.c_void_p),
+                ("n_seq", C.c_uint32), ("n_tok", C.c_uint32), ("path_stride", C.c_uint32)]
+
+
+class KvForkP(C.Structure):
+    """flh_kv_fork_p (pointers are device addresses)."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("len", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p),
+                ("free_pages", C.c_void_p), ("taken", C.c_void_p), ("shared", C.c_void_p), ("copy_src", C.c_void_p),
+                ("copy_dst", C.c_void_p), ("copy_n", C.c_void_p), ("info", C.c_void_p), ("n_fork", C.c_uint32),
+                ("n_seq", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_free", C.c_uint32),
+                ("table_stride", C.c_uint32)]
+
+
+class KvTrimP(C.Structure):
+    """flh_kv_trim_p (pointers are device addresses)."""
+    _fields_ = [("kv_len", C.c_void_p), ("keep", C.c_void_p), ("held", C.c_void_p), ("table", C.c_void_p),
+                ("free_pages", C.c_void_p), ("taken", C.c_void_p), ("shared", C.c_void_p), ("copy_src", C.c_void_p),
+                ("copy_dst", C.c_void_p), ("copy_n", C.c_void_p), ("info", C.c_void_p), ("n_seq", C.c_uint32),
+                ("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_free", C.c_uint32), ("table_stride", C.c_uint32)]
+
+
 class FlhError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"fastllm_hip error {code}: {msg}")
@@ -251,6 +299,15 @@ _SIGS = {
     "flh_rope_kv_append": (_I, [_P, _P, _P, _P]),
     "flh_paged_attn_ws_bytes": (_SZ, [_P, _P]),
     "flh_paged_attn": (_I, [_P, _P, _P]),
+    "flh_tree_plan": (_I, [_P, _P]),
+    "flh_tree_attn_ws_bytes": (_SZ, [_P, _P]),
+    "flh_tree_attn": (_I, [_P, _P, _P, _P]),
+    "flh_spec_verify_ws_bytes": (_SZ, [_P]),
+    "flh_spec_verify": (_I, [_P, _P]),
+    "flh_kv_compact": (_I, [_P, _U32, _P, _P]),
+    "flh_kv_copy": (_I, [_P, _U32, _P, _P, _P, _U32, _P]),
+    "flh_kv_fork": (_I, [_P, _P]),
+    "flh_kv_trim": (_I, [_P, _P]),
     "flh_fill_normal": (_I, [_P, _SZ, _U64, _F, _F, _F, _F, _P]),
     "flh_quantize": (_I, [_I, _P, _U32, _U32, _P, _P]),
     "flh_quantize_host": (_I, [_I, _P, _U32, _U32, _P]),
@@ -641,6 +698,60 @@ def paged_attn_ws_bytes(cache: KvCache, p: AttnP) -> int:
 def paged_attn(cache: KvCache, p: AttnP, stream: Stream) -> None:
     """Attention of new tokens over the paged cache."""
     check(lib().flh_paged_attn(C.byref(cache.c), C.byref(p), stream.handle))
+
+
+# ------------------------------------------- trees of drafted tokens --
+class KvCaches:
+    """The caches of several layers (KvCache, alike but for k and v)."""
+
+    def __init__(self, caches):
+        self.n = len(caches)
+        self.c = (_KvCacheC * max(self.n, 1))(*[x.c for x in caches])
+
+
+def tree_plan(p: TreePlanP, stream: Stream) -> None:
+    """Ancestor bits, depths and positions of trees of drafted tokens."""
+    check(lib().flh_tree_plan(C.byref(p), stream.handle))
+
+
+def tree_attn_ws_bytes(cache: KvCache, p: AttnP) -> int:
+    """Workspace bytes of tree_attn with these arguments."""
+    return lib().flh_tree_attn_ws_bytes(C.byref(cache.c), C.byref(p))
+
+
+def tree_attn(cache: KvCache, p: AttnP, tree: TreeP, stream: Stream) -> None:
+    """Attention of trees of drafted tokens over the paged cache."""
+    check(lib().flh_tree_attn(C.byref(cache.c), C.byref(p), C.byref(tree), stream.handle))
+
+
+def spec_verify_ws_bytes(p: VerifyP) -> int:
+    """Workspace bytes of spec_verify with these arguments."""
+    return lib().flh_spec_verify_ws_bytes(C.byref(p))
+
+
+def spec_verify(p: VerifyP, stream: Stream) -> None:
+    """Which drafted tokens stand against the target, and the token behind them."""
+    check(lib().flh_spec_verify(C.byref(p), stream.handle))
+
+
+def kv_compact(caches: KvCaches, p: KvCompactP, stream: Stream) -> None:
+    """The accepted paths' keys and values moved into place, in all layers."""
+    check(lib().flh_kv_compact(caches.c, caches.n, C.byref(p), stream.handle))
+
+
+def kv_copy(caches: KvCaches, src, dst, n_tok, n_copy: int, stream: Stream) -> None:
+    """Tokens copied from slots on to slots on, in all layers (device arrays)."""
+    check(lib().flh_kv_copy(caches.c, caches.n, _p(src), _p(dst), _p(n_tok), n_copy, stream.handle))
+
+
+def kv_fork(p: KvForkP, stream: Stream) -> None:
+    """Requests that take over others' tokens: full pages are shared, a partly filled one is to be copied."""
+    check(lib().flh_kv_fork(C.byref(p), stream.handle))
+
+
+def kv_trim(p: KvTrimP, stream: Stream) -> None:
+    """Requests cut back to fewer tokens, or freed; pages that nobody holds any more go back to the free list."""
+    check(lib().flh_kv_trim(C.byref(p), stream.handle))
 
 
 def fill_normal(dst, n: int, seed: int, stream: Stream, mean: float = 0.0, std: float = 1.0,

@@ -111,12 +111,28 @@ struct AttnItem {
     int32_t lo, hi;                     // keys that some row of the strip sees
     uint32_t u0, tiles;                 // first unit of the item, tiles (units: C more)
 };
-// keys [lo, hi) that a token of the item's request sees (any lo; none where hi <= lo or hi <= 0)
-__device__ __forceinline__ int32_t key_hi(const AttnArgs & a, const AttnItem & it, uint32_t tok) {
+// keys [lo, hi) that a token of the item's request sees (any lo; none where hi <= lo or hi <= 0).
+// TR, the tokens are a tree: the cached ones in front of it among them; which of the tree's own keys,
+// p0 and behind, a token sees is in its bits (tree_bits).
+template <bool TR> using ArgsOf = std::conditional_t<TR, AttnTreeArgs, AttnArgs>;
+template <bool TR> __device__ __forceinline__ int32_t key_hi(const ArgsOf<TR> & a, const AttnItem & it, uint32_t tok) {
+    if constexpr (TR) return min(it.cap, it.p0);
     return a.causal ? min(it.cap, it.p0 + (int32_t)tok + 1) : it.cap;
 }
-__device__ __forceinline__ int32_t key_lo(const AttnArgs & a, const AttnItem & it, uint32_t tok) {
+template <bool TR> __device__ __forceinline__ int32_t key_lo(const ArgsOf<TR> & a, const AttnItem & it, uint32_t tok) {
+    // (a token's depth is below the request's tokens, whatever the array says)
+    if constexpr (TR) tok = a.window ? min(a.tree_depth[it.r0 + min(tok, it.n - 1)], it.n - 1) : 0u;
     return a.window ? it.p0 + (int32_t)tok + 1 - (int32_t)min(a.window, 1u << 30) : 0;
+}
+// Bits of the 32 keys from k0 on that a token of the item's request sees in its tree (k0 below
+// 2^30; the words from the token's row of the mask).  Words that are not there are zeros: loads
+// of a clamped place and selects, no branch.
+__device__ __forceinline__ uint32_t tree_bits(const AttnTreeArgs & a, const AttnItem & it, uint32_t tok, int32_t k0) {
+    const uint32_t * row = a.tree_mask + (uint64_t)(it.r0 + min(tok, it.n - 1)) * a.tree_stride;
+    const int32_t b = k0 - it.p0, w = b >> 5, last = (int32_t)a.tree_stride - 1;
+    const uint32_t x = row[min(max(w, 0), last)], y = row[min(max(w + 1, 0), last)];
+    const uint32_t lo = w >= 0 && w <= last ? x : 0u, hi = w >= -1 && w < last ? y : 0u;
+    return __builtin_amdgcn_alignbit(hi, lo, (uint32_t)b & 31u);
 }
 // whether one of the keys [lo, hi) (lo >= 0, hi <= cap) has a page; by a whole wave
 __device__ __forceinline__ bool any_page(const AttnArgs & a, const AttnItem & it, int32_t lo, int32_t hi) {
@@ -129,7 +145,7 @@ __device__ __forceinline__ bool any_page(const AttnArgs & a, const AttnItem & it
 // tiles in front of unit x of an item
 template <int C> __device__ __forceinline__ uint32_t tiles_at(uint32_t x) { return x > C ? x - C : 0u; }
 
-template <int M, int KT, int C> struct AttnWalk {
+template <int M, int KT, int C, bool TR = false> struct AttnWalk {
     // the wave's 64 requests at hand, in LDS (they are looked at once an item)
     struct Chunk {
         uint32_t n[64], r0[64], one[64], excl[64];                    // tokens, first row, units a kv head, units before it
@@ -154,7 +170,10 @@ template <int M, int KT, int C> struct AttnWalk {
     __device__ uint32_t span(uint32_t n_, int32_t p, int32_t c, uint32_t i, int32_t & lo, int32_t & hi) const {
         hi = c;
         lo = 0;
-        if (a.causal) {
+        if constexpr (TR) {
+            // (every strip: the tree's keys lie behind all of the others; a root's window begins first)
+            if (a.window) lo = min((int64_t)hi, max((int64_t)0, (int64_t)p + 1 - a.window));
+        } else if (a.causal) {
             const uint32_t t1 = min(n_ - 1, ((i + 1) * M - 1) / a.group);
             hi = max(0, min((int64_t)c, (int64_t)p + t1 + 1));
             if (a.window) {
@@ -421,10 +440,11 @@ struct AttnPlan {
 inline int attn_dims(const AttnArgs & a) {
     return a.dk <= 64 && a.dv <= 64 ? 0 : a.dk <= 128 && a.dv <= 128 ? 1 : a.dk <= 192 && a.dv <= 128 ? 2 : 3;
 }
-AttnPlan attn_dec_plan(const AttnArgs & a);
-AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype);
-int launch_attn_dec(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
-int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
+AttnPlan attn_dec_plan(const AttnTreeArgs & a);
+AttnPlan attn_pre_plan(const AttnTreeArgs & a, uint32_t dtype);
+// (a.tree_mask: of a tree's tokens)
+int launch_attn_dec(const AttnTreeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
+int launch_attn_pre(const AttnTreeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
 
 // One row by one wave, a key a lane, in fp32 (scores from sums in 64 bits): for items whose sums are not
 // finite, and rows that have keys but no weight: all their scores are -infinity, or
@@ -432,18 +452,20 @@ int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hi
 // that a row does not see (weight 0), or the vanished low term of a split weight, carries an
 // infinite or NaN value into the row.  Here only the keys seen are looked at, and
 // scores stay what they are, so that they are finite wherever scale q.k is.
-template <typename AT, typename T, int M> __device__ __forceinline__ void attn_row(const AttnArgs & a, const AttnItem & it, uint32_t r) {
+template <typename AT, typename T, int M, bool TR> __device__ __forceinline__ void attn_row(const ArgsOf<TR> & a, const AttnItem & it, uint32_t r) {
     const uint32_t lane = threadIdx.x & 63, row = it.strip * M + r, tok = row / a.group, head = it.kvh * a.group + row % a.group;
     const AT * q = (const AT *)a.q + (it.r0 + tok) * a.q_tok + head * a.q_head;
-    const int32_t hi = key_hi(a, it, tok), lo = max(0, key_lo(a, it, tok));
+    const int32_t old = key_hi<TR>(a, it, tok), hi = TR ? it.cap : old, lo = max(0, key_lo<TR>(a, it, tok));
     const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
     const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     bool any = false;                                                 // a key is seen
-    for (int32_t j0 = lo; j0 < hi; j0 += 64) {
+    // (a tree behind the window of a row that is deep in it: its keys are looked at from its first on)
+    for (int32_t j0 = TR ? min(lo, max(old, 0)) : lo; j0 < hi; j0 += 64) {
         const int32_t j = j0 + (int32_t)lane;
         const uint32_t pg = j < hi ? tab[(uint32_t)j >> a.sh] : FLH_KV_NONE;
-        const bool in = pg < a.n_pages;
+        bool in = pg < a.n_pages;
+        if constexpr (TR) in = in & (((j >= lo) & (j < old)) | ((tree_bits(a, it, tok, j) & 1u) != 0));
         float t = -INFINITY;
         if (in) {
             const T * k = (const T *)(uintptr_t)row_at(kb, pg, a.k_page, (uint32_t)j & a.pmask, a.k_tok);
@@ -518,8 +540,8 @@ __device__ __forceinline__ void attn_note(const AttnArgs & a, uint32_t w, uint32
 // many parts: latency).  Rows of items with sums that are not finite, and rows that lost all their
 // weight, are done by attn_row instead.  The parts' bytes bound it where there are many (18 us for those of 512
 // workgroups with 128 rows of 128, up to 134 KB each), else a launch (4 us).
-template <typename AT, typename T, int M, int KT, int DV, int PW, int C>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+template <typename AT, typename T, int M, int KT, int DV, int PW, int C, bool TR>
+__global__ __launch_bounds__(256) void k_attn_join(ArgsOf<TR> a) {
     constexpr int V = DV / 64, R = 4;                                 // values a lane, rows a wave
     __shared__ float red[PW > 1 ? PW : 1][R][PW > 1 ? DV : 1];
     const uint32_t lane = threadIdx.x & 63, w = blockIdx.x;
@@ -616,7 +638,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
             else
                 for (uint32_t left = __builtin_amdgcn_readfirstlane(lost); left; left &= left - 1) {
                     const uint32_t k = __builtin_ctz(left), tok = (it.strip * M + min(rbase + k, rows - 1)) / a.group;
-                    if (any_page(a, it, max(key_lo(a, it, tok), 0), key_hi(a, it, tok))) again |= 1u << k;
+                    if (any_page(a, it, TR ? 0 : max(key_lo<TR>(a, it, tok), 0), TR ? it.cap : key_hi<TR>(a, it, tok))) again |= 1u << k;
                 }
             if constexpr (PW > 1) {
 #pragma unroll
@@ -644,19 +666,19 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
                 if (lane * V < a.dv) __builtin_memcpy((AT *)a.out + tok * a.o_tok + head * a.o_head + lane * V, y, sizeof y);
             }
             for (uint32_t k = PW > 1 ? pw : 0; k < R; k += PW)
-                if ((again >> k & 1) && rbase + k < rows) attn_row<AT, T, M>(a, it, rbase + k);
+                if ((again >> k & 1) && rbase + k < rows) attn_row<AT, T, M, TR>(a, it, rbase + k);
         }
     }
     if (!me.odd || pw) return;
-    __shared__ typename AttnWalk<M, KT, C>::Chunk chunks[4];
-    AttnWalk<M, KT, C> walk(a, chunks[wave]);
+    __shared__ typename AttnWalk<M, KT, C, TR>::Chunk chunks[4];
+    AttnWalk<M, KT, C, TR> walk(a, chunks[wave]);
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     const uint32_t u = attn_border(w, U, Ge), end = attn_border(w + 1, U, Ge);
     for (uint32_t x = u; x < end;) {                                  // items of workgroup w alone
         AttnItem it;
         walk.find(x, it);
         if (it.u0 + C >= u && it.u0 + it.tiles + C <= end)
-            for (uint32_t r = rbase; r < min((uint32_t)M, min(rbase + R, it.n * a.group - it.strip * M)); ++r) attn_row<AT, T, M>(a, it, r);
+            for (uint32_t r = rbase; r < min((uint32_t)M, min(rbase + R, it.n * a.group - it.strip * M)); ++r) attn_row<AT, T, M, TR>(a, it, r);
         x = it.u0 + it.tiles + C;
     }
 }

@@ -33,8 +33,8 @@ template <int DK, int DV> struct DecShape {
 };
 template <int DK, int DV> constexpr int dec_threads = 64 * DecShape<DK, DV>::W;
 
-template <typename AT, typename T, int DK, int DV, int MT>
-__global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) {
+template <typename AT, typename T, int DK, int DV, int MT, bool TR>
+__global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(ArgsOf<TR> a) {
     typedef DecShape<DK, DV> P;
     typedef typename VecOf<T>::v8 v8;
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = 16 * MT, NS = split_terms<AT, T>(), NW = NS > 1 ? NS : 2;
@@ -54,9 +54,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
     const uint32_t k_lane = l16 * (DK * 2) + (q4 ^ swz_k<DK>(l16)) * 16;
     const uint32_t v_row = 4 * q4 + (l16 >> 2);
     const uint32_t v_lane = 32 * DK * 2 + v_row * (DV * 2) + (((l16 >> 1) & 1) ^ swz_v<DV>(v_row)) * 16 + (l16 & 1) * 8;
-    typedef typename AttnWalk<M, KT, 0>::Chunk Chunk;
+    typedef typename AttnWalk<M, KT, 0, TR>::Chunk Chunk;
     static_assert(sizeof(Chunk) == P::WALK, "chunk");
-    AttnWalk<M, KT, 0> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
+    AttnWalk<M, KT, 0, TR> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units), w = blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
@@ -87,8 +87,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
         float c[MT];                                                  // scale * log2(e), by column
         int32_t rhi[MT], rlo[MT];                                     // keys that the column's row sees
         const int32_t tf = (int32_t)(it.strip * M / a.group), tl = (int32_t)min(it.n - 1, (it.strip * M + M - 1) / a.group);
-        const int32_t all_lo = a.window ? it.p0 + tl + 1 - (int32_t)min(a.window, 1u << 30) : 0;
-        const int32_t all_hi = a.causal ? min(it.cap, it.p0 + tf + 1) : it.cap;
+        // (a tree: the deepest token that there may be)
+        const int32_t all_lo = a.window ? it.p0 + (TR ? (int32_t)it.n - 1 : tl) + 1 - (int32_t)min(a.window, 1u << 30) : 0;
+        const int32_t all_hi = TR ? min(it.cap, it.p0) : a.causal ? min(it.cap, it.p0 + tf + 1) : it.cap;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const uint32_t r = it.strip * M + 16 * mt + l16, tok = r / a.group, head = it.kvh * a.group + r % a.group;
@@ -96,8 +97,8 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
             // first of the item instead.
             const bool real = r < rows && a.scale != 0.f;
             const AT * q = (const AT *)a.q + (it.r0 + (r < rows ? tok : 0u)) * a.q_tok + (r < rows ? head : it.kvh * a.group) * a.q_head;
-            rhi[mt] = key_hi(a, it, tok);
-            rlo[mt] = key_lo(a, it, tok);
+            rhi[mt] = key_hi<TR>(a, it, tok);
+            rlo[mt] = key_lo<TR>(a, it, tok);
             c[mt] = a.scale == 0.f ? 1.f : a.scale * 1.4426950408889634f;
             Eight<AT> x[DK / 32];
 #pragma unroll
@@ -180,7 +181,11 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = s[mt][j >> 2][j & 3];
                 if (!whole) {
-                    const uint32_t see = fresh((vm & (uint32_t)bits_of(rlo[mt] - k0, rhi[mt] - k0)) >> (4 * q4));
+                    uint32_t may = (uint32_t)bits_of(rlo[mt] - k0, rhi[mt] - k0);
+                    if constexpr (TR) {
+                        if (k0 + 32 > all_hi) may |= tree_bits(a, it, (it.strip * M + 16 * mt + l16) / a.group, k0);
+                    }
+                    const uint32_t see = fresh((vm & may) >> (4 * q4));
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] = seen(x[j], see, 16 * (j >> 2) + (j & 3));
                 }
@@ -322,7 +327,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
                 }
             } else if (d < a.dv) {
                 const uint32_t tok = it.r0 + row / a.group, head = it.kvh * a.group + row % a.group;
-                if (!(sum > 0.f)) lost = lost || key_hi(a, it, row / a.group) > max(key_lo(a, it, row / a.group), 0);
+                if (!(sum > 0.f)) lost = TR || lost || key_hi<TR>(a, it, row / a.group) > max(key_lo<TR>(a, it, row / a.group), 0);
                 if (sum == 0.f) v = f32x4{0.f, 0.f, 0.f, 0.f};
                 else v /= sum;
                 store4((AT *)a.out + tok * a.o_tok + head * a.o_head + d, v[0], v[1], v[2], v[3]);
@@ -344,26 +349,27 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(AttnArgs a) 
 }
 
 namespace {
-template <typename AT, typename T, int DK, int DV, int MT> int go(const AttnArgs & a, hipStream_t s) {
+template <typename AT, typename T, int DK, int DV, int MT, bool TR> int go(const ArgsOf<TR> & a, hipStream_t s) {
     typedef DecShape<DK, DV> P;
     constexpr int M = 16 * MT;
-    const void * k = (const void *)k_attn_dec<AT, T, DK, DV, MT>;
+    const void * k = (const void *)k_attn_dec<AT, T, DK, DV, MT, TR>;
     if (int rc = lds_fits(k, P::LDS, "k_attn_dec")) return rc;
-    hipLaunchKernelGGL((k_attn_dec<AT, T, DK, DV, MT>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
+    hipLaunchKernelGGL((k_attn_dec<AT, T, DK, DV, MT, TR>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_dec launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4, 0>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4, 0, TR>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
-template <typename AT, typename T, int MT> int dims(const AttnArgs & a, hipStream_t s) {
+template <typename AT, typename T, int MT, bool TR> int dims(const ArgsOf<TR> & a, hipStream_t s) {
     switch (attn_dims(a)) {
-        case 0: return go<AT, T, 64, 64, MT>(a, s);
-        case 1: return go<AT, T, 128, 128, MT>(a, s);
-        case 2: return go<AT, T, 192, 128, MT>(a, s);
-        default: return go<AT, T, 256, 256, MT>(a, s);
+        case 0: return go<AT, T, 64, 64, MT, TR>(a, s);
+        case 1: return go<AT, T, 128, 128, MT, TR>(a, s);
+        case 2: return go<AT, T, 192, 128, MT, TR>(a, s);
+        default: return go<AT, T, 256, 256, MT, TR>(a, s);
     }
 }
-template <typename AT, typename T> int tiles(const AttnArgs & a, hipStream_t s) {
-    return attn_dec_plan(a).m == 16 ? dims<AT, T, 1>(a, s) : dims<AT, T, 2>(a, s);
+template <typename AT, typename T> int tiles(const AttnTreeArgs & a, hipStream_t s) {
+    if (a.tree_mask) return attn_dec_plan(a).m == 16 ? dims<AT, T, 1, true>(a, s) : dims<AT, T, 2, true>(a, s);
+    return attn_dec_plan(a).m == 16 ? dims<AT, T, 1, false>(a, s) : dims<AT, T, 2, false>(a, s);
 }
 template <int DK, int DV> void shape(AttnPlan & p, uint32_t & per_cu) {
     p.dv = DV;
@@ -371,7 +377,7 @@ template <int DK, int DV> void shape(AttnPlan & p, uint32_t & per_cu) {
 }
 }  // namespace
 
-AttnPlan attn_dec_plan(const AttnArgs & a) {
+AttnPlan attn_dec_plan(const AttnTreeArgs & a) {
     AttnPlan p{};
     uint32_t per_cu = 1;
     switch (attn_dims(a)) {
@@ -387,7 +393,7 @@ AttnPlan attn_dec_plan(const AttnArgs & a) {
     return p;
 }
 
-int launch_attn_dec(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s) {
+int launch_attn_dec(const AttnTreeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s) {
     if (dtype == FLH_DT_F32) return cache_dtype == FLH_DT_F16 ? tiles<float, _Float16>(a, s) : tiles<float, __bf16>(a, s);
     return dtype == FLH_DT_F16 ? tiles<_Float16, _Float16>(a, s) : tiles<__bf16, __bf16>(a, s);
 }

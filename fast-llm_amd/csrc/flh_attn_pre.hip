@@ -48,8 +48,8 @@ template <int DK, int DV> constexpr int pre_threads = 64 * PreShape<DK, DV>::W;
 // runs at once, else some workgroups of even shares start when others are done
 constexpr int pre_waves(bool split, int dk, int dv) { return dk + dv <= (split ? 128 : 256) ? 2 : 1; }
 
-template <typename AT, typename T, int DK, int DV>
-__global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>() > 1, DK, DV)) void k_attn_pre(AttnArgs a) {
+template <typename AT, typename T, int DK, int DV, bool TR>
+__global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>() > 1, DK, DV)) void k_attn_pre(ArgsOf<TR> a) {
     typedef PreShape<DK, DV> P;
     typedef typename VecOf<T>::v8 v8;
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = P::M, NS = split_terms<AT, T>();
@@ -78,9 +78,9 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         const uint32_t r = 8 * p + 4 * half + (l16 >> 2), pc = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
         v_lane[p] = KT * DK * 2 + r * (DV * 2) + (pc ^ swz_v<DV>(r)) * 16 + (l16 & 1) * 8;
     }
-    typedef typename AttnWalk<M, KT, PRE_ITEM>::Chunk Chunk;
+    typedef typename AttnWalk<M, KT, PRE_ITEM, TR>::Chunk Chunk;
     static_assert(sizeof(Chunk) == P::WALK, "chunk");
-    AttnWalk<M, KT, PRE_ITEM> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 128 + wave * P::WALK));
+    AttnWalk<M, KT, PRE_ITEM, TR> walk(a, *(Chunk *)(sm + NST * P::STAGE + W * P::TAB + 128 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units);
     // neighbours on the line share keys: they go to one XCD (workgroups are dealt
     // to the 8 XCDs in turn)
@@ -102,11 +102,13 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         const uint32_t head = it.kvh * a.group + row % a.group;
         const int32_t win = (int32_t)min(a.window, 1u << 30);
         // keys that the lane's row sees; that all of the wave's rows see
-        const int32_t rhi = key_hi(a, it, tok), rlo = key_lo(a, it, tok);
+        const int32_t rhi = key_hi<TR>(a, it, tok), rlo = key_lo<TR>(a, it, tok);
         const uint32_t first = it.strip * M + 32 * wave;              // the wave's rows
         const bool here = first < rows;
         const int32_t tf = (int32_t)(first / a.group), tl = (int32_t)min(it.n - 1, (first + 31) / a.group);
-        const int32_t all_lo = win ? it.p0 + tl + 1 - win : 0, all_hi = a.causal ? min(it.cap, it.p0 + tf + 1) : it.cap;
+        // (a tree: the deepest token that there may be)
+        const int32_t all_lo = win ? it.p0 + (TR ? (int32_t)it.n - 1 : tl) + 1 - win : 0;
+        const int32_t all_hi = TR ? min(it.cap, it.p0) : a.causal ? min(it.cap, it.p0 + tf + 1) : it.cap;
 
         const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
         const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
@@ -210,7 +212,11 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         // multiplied meanwhile into nx; `midway` is called on the way
         auto tile = [&](int32_t k0, uint64_t vm, uint32_t at, uint32_t next, f32x16 (&s)[2], f32x16 (&nx)[2], auto && midway) {
             if (!(vm == ~0ull && k0 >= all_lo && k0 + KT <= all_hi)) {
-                const uint64_t see = fresh((vm & bits_of(rlo - k0, rhi - k0)) >> (4 * half));
+                uint64_t may = bits_of(rlo - k0, rhi - k0);
+                if constexpr (TR) {
+                    if (k0 + KT > all_hi) may |= (uint64_t)tree_bits(a, it, tok, k0 + 32) << 32 | tree_bits(a, it, tok, k0);
+                }
+                const uint64_t see = fresh((vm & may) >> (4 * half));
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -396,7 +402,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         // a row that has keys got no weight
         const bool lost = !(l > 0.f) & (row < rows);
         if (__ballot(lost) && whole && any_page(a, it, it.lo, it.hi))
-            odd = odd || (lost & (key_hi(a, it, tok) > max(key_lo(a, it, tok), 0)));
+            odd = odd || (lost & (TR || key_hi<TR>(a, it, tok) > max(key_lo<TR>(a, it, tok), 0)));
         if (row < rows) {
             if (whole) {
                 AT * out = (AT *)a.out + (it.r0 + tok) * a.o_tok + head * a.o_head;
@@ -442,22 +448,25 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
 }
 
 namespace {
-template <typename AT, typename T, int DK, int DV> int go(const AttnArgs & a, hipStream_t s) {
+template <typename AT, typename T, int DK, int DV, bool TR> int go(const ArgsOf<TR> & a, hipStream_t s) {
     typedef PreShape<DK, DV> P;
-    const void * k = (const void *)k_attn_pre<AT, T, DK, DV>;
+    const void * k = (const void *)k_attn_pre<AT, T, DK, DV, TR>;
     if (int rc = lds_fits(k, P::LDS, "k_attn_pre")) return rc;
-    hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
+    hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV, TR>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_pre launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV, 1, PRE_ITEM>), dim3(a.grid, P::M / 16), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV, 1, PRE_ITEM, TR>), dim3(a.grid, P::M / 16), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
-template <typename AT, typename T> int dims(const AttnArgs & a, hipStream_t s) {
+template <typename AT, typename T, bool TR> int dims(const ArgsOf<TR> & a, hipStream_t s) {
     switch (attn_dims(a)) {
-        case 0: return go<AT, T, 64, 64>(a, s);
-        case 1: return go<AT, T, 128, 128>(a, s);
-        case 2: return go<AT, T, 192, 128>(a, s);
-        default: return go<AT, T, 256, 256>(a, s);
+        case 0: return go<AT, T, 64, 64, TR>(a, s);
+        case 1: return go<AT, T, 128, 128, TR>(a, s);
+        case 2: return go<AT, T, 192, 128, TR>(a, s);
+        default: return go<AT, T, 256, 256, TR>(a, s);
     }
+}
+template <typename AT, typename T> int forms(const AttnTreeArgs & a, hipStream_t s) {
+    return a.tree_mask ? dims<AT, T, true>(a, s) : dims<AT, T, false>(a, s);
 }
 template <int DK, int DV> void shape(AttnPlan & p, bool split) {
     static_assert(pre_waves(false, DK, DV) * PreShape<DK, DV>::LDS <= 160 * 1024, "workgroups per CU");
@@ -467,7 +476,7 @@ template <int DK, int DV> void shape(AttnPlan & p, bool split) {
 }
 }  // namespace
 
-AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype) {
+AttnPlan attn_pre_plan(const AttnTreeArgs & a, uint32_t dtype) {
     AttnPlan p{};
     const bool split = dtype == FLH_DT_F32;
     switch (attn_dims(a)) {
@@ -483,9 +492,9 @@ AttnPlan attn_pre_plan(const AttnArgs & a, uint32_t dtype) {
     return p;
 }
 
-int launch_attn_pre(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s) {
-    if (dtype == FLH_DT_F32) return cache_dtype == FLH_DT_F16 ? dims<float, _Float16>(a, s) : dims<float, __bf16>(a, s);
-    return dtype == FLH_DT_F16 ? dims<_Float16, _Float16>(a, s) : dims<__bf16, __bf16>(a, s);
+int launch_attn_pre(const AttnTreeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s) {
+    if (dtype == FLH_DT_F32) return cache_dtype == FLH_DT_F16 ? forms<float, _Float16>(a, s) : forms<float, __bf16>(a, s);
+    return dtype == FLH_DT_F16 ? forms<_Float16, _Float16>(a, s) : forms<__bf16, __bf16>(a, s);
 }
 
 }  // namespace flh

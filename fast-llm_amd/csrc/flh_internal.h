@@ -224,10 +224,27 @@ struct AttnArgs {
     uint32_t grid, min_units;           // the launch's (flh_attn.h)
     float scale;
 };
+// of a tree's tokens: bits of the tree's keys that a row sees (null: no tree, the tokens follow one
+// another), and how deep it is (read with a window).  (Apart, so that the kernels of the others do not have them.)
+struct AttnTreeArgs : AttnArgs {
+    const uint32_t * tree_mask; const uint32_t * tree_depth;
+    uint32_t tree_stride;               // words of a row of tree_mask
+};
+int check_kv_cache(const flh_kv_cache * c);               // (flh_paged.cpp)
 int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s);
 int launch_rope(const RopeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
-size_t attn_ws_bytes(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype);
-int launch_attn(const AttnArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
+size_t attn_ws_bytes(const AttnTreeArgs & a, uint32_t dtype);
+int launch_attn(const AttnTreeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);
+// Trees of drafted tokens (flh_tree.hip).
+int launch_tree_plan(const flh_tree_plan_p & p, hipStream_t s);
+// Their verification (flh_verify.hip) and the pages behind it (flh_pages.hip).
+size_t verify_ws_bytes(const flh_verify_p & p);
+int launch_verify(const flh_verify_p & p, hipStream_t s);
+int launch_kv_fork(const flh_kv_fork_p & p, hipStream_t s);
+int launch_kv_trim(const flh_kv_trim_p & p, hipStream_t s);
+int launch_kv_copy(const flh_kv_cache * c, uint32_t n, const uint32_t * src, const uint32_t * dst, const uint32_t * count,
+                   uint32_t n_copy, hipStream_t s);
+int launch_kv_compact(const flh_kv_cache * c, uint32_t n, const flh_kv_compact_p & p, hipStream_t s);
 int launch_fill_normal(float * dst, size_t n, uint64_t seed, float mean,
                        float stddev, float outlier_frac, float outlier_scale,
                        hipStream_t s);

@@ -23,7 +23,9 @@ bool off(const void * p, uintptr_t align) { return ((uintptr_t)p & (align - 1)) 
 bool pow2_page(uint32_t n) { return n >= 1 && n <= 65536 && (n & (n - 1)) == 0; }
 uintptr_t elem(uint32_t dtype) { return dtype == FLH_DT_F32 ? 4 : 2; }
 
-int check_cache(const flh_kv_cache * c) {
+}  // namespace
+
+int flh::check_kv_cache(const flh_kv_cache * c) {
     if (!c) return set_error(FLH_ERR_ARG, "kv cache: null");
     if (c->dtype != FLH_DT_F16 && c->dtype != FLH_DT_BF16)
         return set_error(FLH_ERR_UNSUPPORTED, "kv cache: dtype must be F16 or BF16");
@@ -41,6 +43,8 @@ int check_cache(const flh_kv_cache * c) {
         return set_error(FLH_ERR_UNSUPPORTED, "kv cache: page and token strides must be below 2^31 elements, head strides below 2^40");
     return FLH_OK;
 }
+
+namespace {
 
 // [tok][head][d] elements at these strides
 struct Rows {
@@ -91,8 +95,8 @@ void set_rope(RopeArgs & a, const flh_rope_table * r) {
     a.halves = r ? r->halves : 0;
 }
 
-int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
-    if (int rc = check_cache(c)) return rc;
+int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnTreeArgs & a) {
+    if (int rc = check_kv_cache(c)) return rc;
     if (!p) return set_error(FLH_ERR_ARG, "attention: null arguments");
     if (p->dtype > FLH_DT_BF16) return set_error(FLH_ERR_ARG, "attention: unknown dtype");
     if (p->dtype != FLH_DT_F32 && p->dtype != c->dtype)
@@ -107,7 +111,7 @@ int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
     // units of work are counted in 32 bits (strips of 16 rows or more, tiles of 64 keys or more and 3 units a strip)
     if ((double)c->n_kv_head * ((double)p->n_tok * group / 16 + 2.0 * p->n_seq) * ((double)keys / 64 + 5) >= 4.0e9)
         return set_error(FLH_ERR_UNSUPPORTED, "attention: too much work for one call (rows times table length)");
-    a = AttnArgs{};
+    a = AttnTreeArgs{};
     a.q = p->q; a.out = p->out; a.q_start = p->q_start; a.kv_len = p->kv_len; a.table = p->table; a.ws = p->ws;
     a.k = c->k; a.v = c->v;
     a.q_tok = p->q_tok; a.q_head = p->q_head; a.o_tok = p->o_tok; a.o_head = p->o_head;
@@ -118,6 +122,29 @@ int attn_args(const flh_kv_cache * c, const flh_attn_p * p, AttnArgs & a) {
     a.n_seq = p->n_seq; a.n_tok = p->n_tok; a.max_q = p->max_q; a.table_stride = p->table_stride;
     a.causal = p->causal != 0; a.window = p->window; a.pmask = c->page_size - 1; a.scale = p->scale;
     return FLH_OK;
+}
+
+// the rest of a call: pointers, workspace, launches
+int attn_run(const flh_kv_cache * c, const flh_attn_p * p, const AttnTreeArgs & a, void * stream) {
+    if (p->n_tok && p->n_seq) {
+        const uintptr_t el = elem(p->dtype);
+        if (!p->q || !p->out || off(p->q, el) || off(p->out, el))
+            return set_error(FLH_ERR_ARG, "attention: q and out must be non-null and element aligned");
+        if (!p->q_start || !p->kv_len || off(p->q_start, 4) || off(p->kv_len, 4) || off(p->table, 4) || (!p->table && p->table_stride))
+            return set_error(FLH_ERR_ARG, "attention: q_start, kv_len and table must be non-null and 4-byte aligned");
+        if (overlap({p->q, p->q_tok, p->q_head, c->d_k}, {p->out, p->o_tok, p->o_head, c->d_v}, p->n_tok, p->n_head, el))
+            return set_error(FLH_ERR_ARG, "attention: out overlaps q");
+        const size_t need = attn_ws_bytes(a, p->dtype);
+        if (need && (!p->ws || off(p->ws, 16) || p->ws_bytes < need))
+            return set_error(FLH_ERR_ARG, a.tree_stride ? "attention: ws must be 16-byte aligned and of flh_tree_attn_ws_bytes"
+                                                        : "attention: ws must be 16-byte aligned and of flh_paged_attn_ws_bytes");
+    }
+    if (int rc = need_device()) return rc;
+    if (p->n_tok == 0 || p->n_seq == 0) return FLH_OK;
+    // two launches that belong together: another thread's call in between would take the
+    // workspace, which calls on one stream may share
+    const StreamTurn turn(stream, true);
+    return launch_attn(a, p->dtype, c->dtype, (hipStream_t)stream);
 }
 
 }  // namespace
@@ -204,7 +231,7 @@ int flh_rope(const flh_rope_table * r, uint32_t dtype, const void * x, uint64_t 
 }
 
 int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * c, const flh_rope_kv_p * p, void * stream) {
-    if (int rc = check_cache(c)) return rc;
+    if (int rc = check_kv_cache(c)) return rc;
     if (!p) return set_error(FLH_ERR_ARG, "rope append: null arguments");
     if (p->dtype > FLH_DT_BF16) return set_error(FLH_ERR_ARG, "rope append: unknown dtype");
     if (p->n_head > 65535) return set_error(FLH_ERR_ARG, "rope append: n_head must be at most 65535");
@@ -234,32 +261,37 @@ int flh_rope_kv_append(const flh_rope_table * r, const flh_kv_cache * c, const f
 }
 
 size_t flh_paged_attn_ws_bytes(const flh_kv_cache * c, const flh_attn_p * p) {
-    AttnArgs a;
+    AttnTreeArgs a;
     if (attn_args(c, p, a)) return 0;
-    return attn_ws_bytes(a, p->dtype, c->dtype);
+    return attn_ws_bytes(a, p->dtype);
 }
 
 int flh_paged_attn(const flh_kv_cache * c, const flh_attn_p * p, void * stream) {
-    AttnArgs a;
+    AttnTreeArgs a;
     if (int rc = attn_args(c, p, a)) return rc;
+    return attn_run(c, p, a, stream);
+}
+
+size_t flh_tree_attn_ws_bytes(const flh_kv_cache * c, const flh_attn_p * p) {
+    AttnTreeArgs a;
+    if (attn_args(c, p, a)) return 0;
+    a.tree_stride = 1;
+    return attn_ws_bytes(a, p->dtype);
+}
+
+int flh_tree_attn(const flh_kv_cache * c, const flh_attn_p * p, const flh_tree_p * t, void * stream) {
+    AttnTreeArgs a;
+    if (int rc = attn_args(c, p, a)) return rc;
+    if (!t) return set_error(FLH_ERR_ARG, "tree attention: null arguments");
+    if (!p->causal) return set_error(FLH_ERR_ARG, "tree attention: causal must be set");
+    if (t->mask_stride == 0 || t->mask_stride > 32768) return set_error(FLH_ERR_ARG, "tree attention: mask_stride must be in 1 .. 32768");
     if (p->n_tok && p->n_seq) {
-        const uintptr_t el = elem(p->dtype);
-        if (!p->q || !p->out || off(p->q, el) || off(p->out, el))
-            return set_error(FLH_ERR_ARG, "attention: q and out must be non-null and element aligned");
-        if (!p->q_start || !p->kv_len || off(p->q_start, 4) || off(p->kv_len, 4) || off(p->table, 4) || (!p->table && p->table_stride))
-            return set_error(FLH_ERR_ARG, "attention: q_start, kv_len and table must be non-null and 4-byte aligned");
-        if (overlap({p->q, p->q_tok, p->q_head, c->d_k}, {p->out, p->o_tok, p->o_head, c->d_v}, p->n_tok, p->n_head, el))
-            return set_error(FLH_ERR_ARG, "attention: out overlaps q");
-        const size_t need = attn_ws_bytes(a, p->dtype, c->dtype);
-        if (need && (!p->ws || off(p->ws, 16) || p->ws_bytes < need))
-            return set_error(FLH_ERR_ARG, "attention: ws must be 16-byte aligned and of flh_paged_attn_ws_bytes");
+        if (!t->mask || off(t->mask, 4)) return set_error(FLH_ERR_ARG, "tree attention: mask must be non-null and 4-byte aligned");
+        if ((p->window && !t->depth) || off(t->depth, 4))
+            return set_error(FLH_ERR_ARG, "tree attention: a window needs depth, 4-byte aligned");
     }
-    if (int rc = need_device()) return rc;
-    if (p->n_tok == 0 || p->n_seq == 0) return FLH_OK;
-    // two launches that belong together: another thread's call in between would take the
-    // workspace, which calls on one stream may share
-    const StreamTurn turn(stream, true);
-    return launch_attn(a, p->dtype, c->dtype, (hipStream_t)stream);
+    a.tree_mask = t->mask; a.tree_depth = t->depth; a.tree_stride = t->mask_stride;
+    return attn_run(c, p, a, stream);
 }
 
 }  // extern "C"

@@ -494,6 +494,131 @@ typedef struct flh_attn_p {
 size_t flh_paged_attn_ws_bytes(const flh_kv_cache * cache, const flh_attn_p * p);
 int flh_paged_attn(const flh_kv_cache * cache, const flh_attn_p * p, void * stream);
 
+/* ------------------------------------------- trees of drafted tokens -- */
+/* A step that verifies drafts which branch: flh_kv_plan (slots by row), flh_tree_plan, then the layers
+ * (flh_rope_kv_append with its pos, flh_tree_attn), the vocabulary's product, flh_spec_verify,
+ * flh_kv_compact and flh_kv_trim; nothing comes back to the host in between.  The reference
+ * verifies runs of drafted tokens one sequence at a time, greedily, on the host
+ * (tools/decode_main.cpp:332-370); these are this backend's own form.
+ *
+ * A request's rows are a tree: row 0 is its last token (whose keys and values are new, too), the
+ * others drafted ones behind it. */
+
+/* parent[r]: the row that row r of a request hangs on, by its index in the request, below its own; anything
+ * else: row r is a root.  depth[r]: rows above it; bit b of its mask_stride words of mask: row b of the
+ * request is r itself or above it (rows b >= 32 * mask_stride have no bit), with window > 0 only those
+ * less than window above it; pos[r] (may be NULL, then kv_len too): kv_len[s] - rows of the
+ * request + depth[r].  Rows n_tok and behind, and rows of no request, are left as they are.
+ * mask_stride: 1 .. 32768.  Outputs must not overlap anything. */
+typedef struct flh_tree_plan_p {
+    const uint32_t * q_start; const int32_t * parent; const uint32_t * kv_len;
+    uint32_t * mask, * depth; int32_t * pos;
+    uint32_t n_seq, n_tok, mask_stride, window;
+} flh_tree_plan_p;
+int flh_tree_plan(const flh_tree_plan_p * p, void * stream);
+
+/* flh_paged_attn for a tree's rows (causal must be set): row i of a request's n sees the keys
+ * j < kv_len - n (with window > 0 those with j > kv_len - n + depth[row] - window) and key kv_len - n + b for
+ * each bit b of its words of mask (any bits, also of rows behind it; the window is not applied to them).
+ * A row that sees no key gives 0.  depth (NULL without a window) counts as at most n - 1.
+ * Everything else, ws too, is as flh_paged_attn's, but that weights go into the products in two
+ * terms up to 64 rows a kv head (max_q * n_head / n_kv_head) instead of 32. */
+typedef struct flh_tree_p {
+    const uint32_t * mask, * depth;
+    uint32_t mask_stride;
+} flh_tree_p;
+size_t flh_tree_attn_ws_bytes(const flh_kv_cache * cache, const flh_attn_p * p);
+int flh_tree_attn(const flh_kv_cache * cache, const flh_attn_p * p, const flh_tree_p * t, void * stream);
+
+/* Which rows of each request's tree stand, and the token behind them.  target: logits of row r at
+ * target + r * t_row (vocab of them, any stride, aligned to an element).  draft (NULL: tokens drafted
+ * without a distribution): logits, in the same way, that the children of row r were drawn from, each by itself; rows
+ * without children are not read.  token[r]: the drafted token (a request's row 0 has none); one that is not below vocab does not
+ * stand.  parent as in flh_tree_plan (NULL: each row hangs on the one before); of a row's children the first max_child (1 .. 64) are
+ * looked at, of a request's rows the first 256.
+ * p = softmax(inv_temp[s] * target) and q of the draft (inv_temp NULL: 1; infinity: greedy, p is 1 at
+ * the first of the largest, whatever the draft; what is not >= 0 counts as 0).  A logit that is no number counts as -infinity, infinity as
+ * the largest float.  From row 0 on, a row's children are tested in order: the first one stands if
+ * u_accept * q(x) < p(x), and each that does not stand leaves max(p - q, 0), over its sum, as p for the next
+ * (without a draft: p without its token).  The path goes on at the first that stands; where none does, or there is
+ * none, next is the first token whose sum of what is left of p, up to and with it, passes u_next[s] times the
+ * whole (nothing left: of p).  Then the tokens of the path and next together are distributed as p alone would
+ * have them, u_accept and u_next being uniform in [0, 1).  All of it in 64 bits.
+ *   n_path[s]: rows of the path, row 0 with it (0 for a request without rows); path[s * path_stride + j]: its
+ * rows, by their index in the request, ascending; FLH_KV_NONE behind them.  A path ends at path_stride rows, as if the last one
+ * had no children.  next[s]: the token (FLH_KV_NONE where the target allows none, or there is no row).
+ * logp (or NULL): entry j of a request, the logarithm of p (of the row, as it was) at the token behind the path's row j: that of row
+ * j + 1, at last next; 0 behind.  len (or NULL, then kv_len may be): kv_len[s] - rows + n_path[s], what the
+ * request holds then.  ws: flh_spec_verify_ws_bytes of the same arguments, 16-byte aligned, as
+ * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; n_tok times the vocabulary's
+ * chunks of 4096 below 2^31. */
+typedef struct flh_verify_p {
+    const void * target, * draft;
+    const uint32_t * q_start, * token; const int32_t * parent;
+    const float * inv_temp, * u_accept, * u_next; const uint32_t * kv_len;
+    uint32_t * n_path, * path, * next; float * logp; uint32_t * len;
+    void * ws; size_t ws_bytes;
+    uint64_t t_row, d_row;
+    uint32_t dtype, n_seq, n_tok, vocab, path_stride, max_child;
+} flh_verify_p;
+size_t flh_spec_verify_ws_bytes(const flh_verify_p * p);
+int flh_spec_verify(const flh_verify_p * p, void * stream);
+
+/* ------------------------------------------------- pages between steps -- */
+/* caches: a host array of n_cache layers' caches, alike but for k and v (one launch for up
+ * to 64 of them). */
+
+/* The rows of a path into place: in every layer, token path[s * path_stride + j] of request s (j < n_path[s]; by
+ * row, slot as flh_kv_plan gave it) is moved to the slot of its row j, so that the path's tokens follow one another
+ * behind the cached ones.  path ascends with path[j] >= j, as flh_spec_verify's does (an entry that is no row
+ * of the request, or has no slot, is left out).  n_tok: entries of slot. */
+typedef struct flh_kv_compact_p {
+    const uint32_t * q_start, * slot, * n_path, * path;
+    uint32_t n_seq, n_tok, path_stride;
+} flh_kv_compact_p;
+int flh_kv_compact(const flh_kv_cache * caches, uint32_t n_cache, const flh_kv_compact_p * p, void * stream);
+
+/* n_copy copies in every layer: n_tok[i] tokens from slot src[i] on to slot dst[i] on, as far
+ * as both pages reach; a slot that is not in the cache (FLH_KV_NONE): none.  No slot that is written may be
+ * another copy's, or this one's, source or target. */
+int flh_kv_copy(const flh_kv_cache * caches, uint32_t n_cache, const uint32_t * src, const uint32_t * dst, const uint32_t * n_tok,
+                uint32_t n_copy, void * stream);
+
+/* Requests that share pages.  shared[page]: how many hold it besides the first (0: it is one request's, or
+ * free), n_pages entries.  The free list is flh_kv_plan's: free_pages[*taken ..] are free.
+ *
+ * flh_kv_fork: request dst[i] (a row of table that holds nothing) takes over the first len[i] (NULL: all) tokens of
+ * request src[i], at most what it holds and its row of the table reaches.  Full pages are shared; for a partly
+ * filled last one dst gets a page off the free list and copy i of the
+ * lists (copy_src, copy_dst: slots, copy_n: tokens; FLH_KV_NONE, FLH_KV_NONE, 0 where there is none), which
+ * flh_kv_copy has to run before dst is read or src's page written again.  kv_len[dst[i]] is set.  Where the list ran out
+ * the entry is FLH_KV_NONE (those tokens are not seen), *taken > n_free, and info[1] (info may be NULL) counts it;
+ * info[0]: copies.  An entry that is no page is FLH_KV_NONE in dst, too.  dst differ from each other and from every src; a
+ * pair of which one is not below n_seq, or that is one and the same, is left out.
+ *
+ * flh_kv_trim: request s holds min(kv_len[s], keep[s]) tokens afterwards (held[s]; may be kv_len).  Pages
+ * behind them are left: their table entries are FLH_KV_NONE, and those that nobody holds any more go back to
+ * the free list, in the order of the requests' and pages that left them last, the last one to be taken next (*taken
+ * goes down; a list of n_free entries takes back what was taken off it).  A last page that is partly filled and shared is left to the others: the
+ * request gets one off the list, and a copy in the lists (as above; run it before the next flh_kv_plan, n_seq entries), so that it may append.  shared NULL: nothing
+ * is shared, and the lists are not written.  info[0]: pages put back; info[1]: pages that the list has no
+ * room for, and copies that found no page (the entry is FLH_KV_NONE).  n_seq * table_stride below 2^31 - 1.
+ * Entries of table that are no page are left out.  Nothing may overlap but held and kv_len. */
+typedef struct flh_kv_fork_p {
+    const uint32_t * src, * dst, * len;
+    uint32_t * kv_len, * table; const uint32_t * free_pages; uint32_t * taken, * shared;
+    uint32_t * copy_src, * copy_dst, * copy_n, * info;
+    uint32_t n_fork, n_seq, n_pages, page_size, n_free, table_stride;
+} flh_kv_fork_p;
+int flh_kv_fork(const flh_kv_fork_p * p, void * stream);
+typedef struct flh_kv_trim_p {
+    const uint32_t * kv_len, * keep;
+    uint32_t * held, * table, * free_pages, * taken, * shared;
+    uint32_t * copy_src, * copy_dst, * copy_n, * info;
+    uint32_t n_seq, n_pages, page_size, n_free, table_stride;
+} flh_kv_trim_p;
+int flh_kv_trim(const flh_kv_trim_p * p, void * stream);
+
 /* ---------------------------------------------------------------- GGUF -- */
 /* GGUF v2/v3 reader (replaces fastllm::Gguf, src/model/gguf.h:28-79,
  * src/model/gguf.cpp:133-303).  The file is mmapped read-only; metadata and

@@ -32,7 +32,7 @@ int check_verify(const flh_verify_p * p) {
     if (p->path_stride == 0) return set_error(FLH_ERR_ARG, "verify: path_stride must be at least 1");
     if (p->max_child == 0 || p->max_child > 64) return set_error(FLH_ERR_ARG, "verify: max_child must be in 1 .. 64");
     const uint64_t chunks = (p->vocab + 4095) / 4096;
-    if (p->n_tok * chunks >= (1ull << 31) || p->n_seq * chunks >= (1ull << 31))
+    if (2 * p->n_tok * chunks >= (1ull << 31) || p->n_seq * chunks >= (1ull << 31))
         return set_error(FLH_ERR_UNSUPPORTED, "verify: too many rows for one call");
     return FLH_OK;
 }

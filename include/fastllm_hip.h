@@ -551,7 +551,7 @@ int flh_tree_attn(const flh_kv_cache * cache, const flh_attn_p * p, const flh_tr
  * j + 1, at last next; 0 behind.  len (or NULL, then kv_len may be): kv_len[s] - rows + n_path[s], what the
  * request holds then.  ws: flh_spec_verify_ws_bytes of the same arguments, 16-byte aligned, as
  * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; n_tok times the vocabulary's
- * chunks of 4096 below 2^31. */
+ * chunks of 4096 below 2^30. */
 typedef struct flh_verify_p {
     const void * target, * draft;
     const uint32_t * q_start, * token; const int32_t * parent;

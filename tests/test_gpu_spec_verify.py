@@ -282,3 +282,20 @@ def test_two_streams_and_no_extras(flh, gpu):
         np.testing.assert_array_equal(x, y)
     s1.close()
     s2.close()
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_logits_of_any_size(flh, gpu, draft):
+    """Rows whose largest logit is so large that its neighbour floats are far below it, temperatures that make
+    a step of a logit decide, or hardly any; all of them against the same formula."""
+    v = Verify(flh, gpu, [6] * 12, 5000, "F32", draft, seed=30, peak=2.0)
+    scale = [1e-30, 1e-3, 1.0, 1e3, 1e6, 1e9, 1e15, 1e30, 3e37, 1e3, 1e-3, 1e-30]
+    temp = [1e30, 1e3, 1.0, 1e-3, 1e-6, 1e-9, 1e-15, 1e-30, 3e-38, 3.0, 1e-3, 1.0]
+    for s in range(12):
+        r = slice(int(v.start[s]), int(v.start[s]) + 6)
+        v.target[r] = (v.target[r].double() * scale[s] + (scale[s] * 50 if s % 2 else 0)).float()
+        if draft:
+            v.draft[r] = (v.draft[r].double() * scale[s] + (scale[s] * 50 if s % 2 else 0)).float()
+        v.inv_temp[s] = temp[s]
+    v.push().run()
+    v.check()

@@ -544,7 +544,11 @@ template <typename AT, typename T, int M, int KT, int DV, int PW, int C, bool TR
 __global__ __launch_bounds__(256) void k_attn_join(ArgsOf<TR> a) {
     constexpr int V = DV / 64, R = 4;                                 // values a lane, rows a wave
     __shared__ float red[PW > 1 ? PW : 1][R][PW > 1 ? DV : 1];
-    const uint32_t lane = threadIdx.x & 63, w = blockIdx.x;
+    // Workgroups are dealt to the 8 XCDs in turn, and items that begin every 16, 32, .. workgroups would all be one XCD's,
+    // whose share of the parts' bytes bounds it then (8 tokens over 4001 keys: 14 us, 6 so): within 8 neighbours w turns with
+    // the bits above and with y.
+    const uint32_t lane = threadIdx.x & 63, g8 = blockIdx.x >> 3;
+    const uint32_t w = a.grid % 8 ? blockIdx.x : g8 << 3 | ((blockIdx.x + (g8 ^ g8 >> 3 ^ g8 >> 6) + blockIdx.y) & 7);
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const AttnNote * notes = attn_notes<M, DV>(a);
     // workgroups that the main kernel had no work for left no note: their number

@@ -31,12 +31,17 @@ template <int DK, int DV> struct DecShape {
     static constexpr int WALK = 6 * 256;                              // AttnWalk::Chunk
     static constexpr size_t LDS = (size_t)W * (WAVE + WALK) + 1088;            // and maxima, sums, flags
 };
+// C of the line of work, for trees.  Items of short requests cost their begin and end: us with 0 / 2 / 4 / 6, trees of 8 tokens,
+// 32 / 8 heads of 128 in bf16: 64 requests of 20 to 1000 keys 93 / 64 / 55 / 55, 32 of 32 to 8192 169 / 145 / 134 / 135, 32 of 4096
+// 106 / 107 / 107 / 106, 4 of 32768 111 / 114 / 113 / 115.  (Runs of drafted tokens keep the sums they have: 0.)
+constexpr int dec_item(bool tree) { return tree ? 4 : 0; }
 template <int DK, int DV> constexpr int dec_threads = 64 * DecShape<DK, DV>::W;
 
 template <typename AT, typename T, int DK, int DV, int MT, bool TR>
 __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(ArgsOf<TR> a) {
     typedef DecShape<DK, DV> P;
     typedef typename VecOf<T>::v8 v8;
+    constexpr int C = dec_item(TR);
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = 16 * MT, NS = split_terms<AT, T>(), NW = NS > 1 ? NS : 2;
     constexpr int NK = DK / 16, NV = DV / 16, ND = NK + NV;           // DMAs of a tile
     extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
@@ -54,9 +59,9 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(ArgsOf<TR> a
     const uint32_t k_lane = l16 * (DK * 2) + (q4 ^ swz_k<DK>(l16)) * 16;
     const uint32_t v_row = 4 * q4 + (l16 >> 2);
     const uint32_t v_lane = 32 * DK * 2 + v_row * (DV * 2) + (((l16 >> 1) & 1) ^ swz_v<DV>(v_row)) * 16 + (l16 & 1) * 8;
-    typedef typename AttnWalk<M, KT, 0, TR>::Chunk Chunk;
+    typedef typename AttnWalk<M, KT, C, TR>::Chunk Chunk;
     static_assert(sizeof(Chunk) == P::WALK, "chunk");
-    AttnWalk<M, KT, 0, TR> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
+    AttnWalk<M, KT, C, TR> walk(a, *(Chunk *)(sm + W * P::WAVE + 1088 + wave * P::WALK));
     const uint32_t U = walk.total(), Ge = attn_wgs(U, a.grid, a.min_units), w = blockIdx.x;
     if (w >= Ge) return;
     uint32_t u = attn_border(w, U, Ge);
@@ -66,10 +71,11 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(ArgsOf<TR> a
     while (u < end) {
         AttnItem it;
         walk.find(u, it);
-        const uint32_t skip = u - it.u0, nt = min(it.tiles - skip, end - u);
+        const uint32_t skip = tiles_at<C>(u - it.u0), nt = C ? tiles_at<C>(min(it.tiles + C, end - it.u0)) - skip : min(it.tiles - skip, end - u);
         const int32_t key0 = (int32_t)((it.lo / KT + skip) * KT + 32 * wave);   // this wave's first key
         const bool begins = skip == 0, ends = skip + nt == it.tiles;
-        if (u == first_u && wave == 0) attn_note<M, DV, 0>(a, w, U, Ge, it, skip);
+        if (u == first_u && wave == 0) attn_note<M, DV, C>(a, w, U, Ge, it, skip);
+        if (C && nt == 0) break;                                      // (the workgroup ends among the item's empty units)
         const uint32_t rows = it.n * a.group;
 
         const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
@@ -334,7 +340,7 @@ __global__ __launch_bounds__((dec_threads<DK, DV>)) void k_attn_dec(ArgsOf<TR> a
             }
         }
         if (__ballot(lost)) odd = odd || any_page(a, it, it.lo, it.hi);
-        u += nt;
+        u = C ? it.u0 + C + skip + nt : u + nt;
         __syncthreads();                                              // the next item's stages
     }
     sm_odd[wave] = __ballot(odd) != 0;
@@ -356,7 +362,7 @@ template <typename AT, typename T, int DK, int DV, int MT, bool TR> int go(const
     if (int rc = lds_fits(k, P::LDS, "k_attn_dec")) return rc;
     hipLaunchKernelGGL((k_attn_dec<AT, T, DK, DV, MT, TR>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_dec launch")) return rc;
-    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4, 0, TR>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<AT, T, M, P::KT, DV, 4, dec_item(TR), TR>), dim3(a.grid, M / 4), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
 }
 template <typename AT, typename T, int MT, bool TR> int dims(const ArgsOf<TR> & a, hipStream_t s) {
@@ -368,7 +374,7 @@ template <typename AT, typename T, int MT, bool TR> int dims(const ArgsOf<TR> & 
     }
 }
 template <typename AT, typename T> int tiles(const AttnTreeArgs & a, hipStream_t s) {
-    if (a.tree_mask) return attn_dec_plan(a).m == 16 ? dims<AT, T, 1, true>(a, s) : dims<AT, T, 2, true>(a, s);
+    if (a.tree_stride) return attn_dec_plan(a).m == 16 ? dims<AT, T, 1, true>(a, s) : dims<AT, T, 2, true>(a, s);
     return attn_dec_plan(a).m == 16 ? dims<AT, T, 1, false>(a, s) : dims<AT, T, 2, false>(a, s);
 }
 template <int DK, int DV> void shape(AttnPlan & p, uint32_t & per_cu) {

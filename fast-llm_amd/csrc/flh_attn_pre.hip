@@ -34,25 +34,28 @@ namespace flh {
 // 649 / 626 / 626, over bf16 797 / 776 / 751 / 753, of heads of 256 1389 / 1332 / 1273 / 1254; 8 x 20 heads
 // of 64 over 1500 keys 58 / 58 / 55 / 58; 64 requests of 40 rows over 500 keys 132 / 136 / 136 / 136.
 constexpr int PRE_ITEM = 3;
-template <int DK, int DV> struct PreShape {
-    static constexpr int W = 4;                                       // waves
+template <int DK, int DV, int WAVES> struct PreShape {
+    static constexpr int W = WAVES;
     static constexpr int M = 32 * W, KT = 64, NST = 2;
     static constexpr int STAGE = KT * (DK + DV) * 2;
-    // a wave's page numbers of 4 tiles, 16 keys each; row addresses of 8 tiles' keys, K and V
-    static constexpr int TAB = 256 + 2 * 1024;
+    // A wave finds the rows of KW keys of GT tiles together, AHEAD such groups before they are read: a group's rows are
+    // found in its second round, from page numbers asked for in its first, and K is asked for two rounds before its own.
+    static constexpr int GT = W, KW = 64 / W, AHEAD = GT < 4 ? 2 : 1;
+    // a wave's page numbers of AHEAD groups; row addresses of two groups' keys, K and V
+    static constexpr int PAGES = 256 * AHEAD, TAB = PAGES + 2 * 1024;
     static constexpr int WALK = 6 * 256;                              // AttnWalk::Chunk
     static constexpr size_t LDS = (size_t)NST * STAGE + W * (TAB + WALK) + 128;
 };
-template <int DK, int DV> constexpr int pre_threads = 64 * PreShape<DK, DV>::W;
 // waves per SIMD that the registers are cut for, and so workgroups per CU: the grid is what
 // runs at once, else some workgroups of even shares start when others are done
 constexpr int pre_waves(bool split, int dk, int dv) { return dk + dv <= (split ? 128 : 256) ? 2 : 1; }
 
-template <typename AT, typename T, int DK, int DV, bool TR>
-__global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>() > 1, DK, DV)) void k_attn_pre(ArgsOf<TR> a) {
-    typedef PreShape<DK, DV> P;
+template <typename AT, typename T, int DK, int DV, bool TR, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, pre_waves(split_terms<AT, T>() > 1, DK, DV)) void k_attn_pre(ArgsOf<TR> a) {
+    typedef PreShape<DK, DV, WAVES> P;
     typedef typename VecOf<T>::v8 v8;
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = P::M, NS = split_terms<AT, T>();
+    constexpr int GT = P::GT, KW = P::KW, AHEAD = P::AHEAD;
     constexpr int NK = DK / 8 / W, NV = DV / 8 / W;                   // DMAs of a tile, this wave's
     constexpr int DB = DV / 32;
     // Where the registers allow it: two tiles a turn of the loop, so that no scores are copied,
@@ -66,7 +69,7 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
     uint8_t * tabs = sm + NST * P::STAGE + wave * P::TAB;
     const uint32_t tab_at = sm_at + NST * P::STAGE + wave * P::TAB;
     uint32_t * sm_odd = (uint32_t *)(sm + NST * P::STAGE + W * P::TAB);   // [W]
-    // keys of 8 tiles that have a page and that a row of the strip sees: a bit each
+    // keys of two groups' tiles that have a page and that a row of the strip sees: a bit each
     uint64_t * sm_live = (uint64_t *)(sm_odd + 16);
 
     // the lane's addresses in a stage: K rows l32 (+ 32 b), pieces half (+ 2 d); V
@@ -112,14 +115,15 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
 
         const uint64_t zero = (uint64_t)(uintptr_t)g_attn_zero;
         const uint32_t * tab = a.table + (uint64_t)it.seq * a.table_stride;
-        // The rows of four tiles are found together, 16 keys of each by the wave that brings
-        // them (lane l: key l % 16 of tile 4 g + l / 16).
-        auto key_of = [&](uint32_t g) { return key0 + (int32_t)((4 * g + (lane >> 4)) * KT + 16 * wave + l16); };
+        // The rows of a group of GT tiles are found together, KW keys of each by the wave that brings
+        // them (lane l: key l % KW of tile GT g + l / KW).
+        auto key_of = [&](uint32_t g) { return key0 + (int32_t)((GT * g + lane / KW) * KT + KW * wave + lane % KW); };
         auto issue_tab = [&](uint32_t g) {                            // page numbers
             const uint32_t pg = (uint32_t)min(key_of(g), max(it.cap - 1, 0)) >> a.sh;
-            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at);
+            dma4(it.cap > 0 ? (uint64_t)(uintptr_t)(tab + pg) : zero, tab_at + (AHEAD > 1 ? (g & 1) * 256 : 0));
         };
-        issue_tab(0);                                                 // (they arrive with the queries)
+        issue_tab(0);
+        if constexpr (AHEAD > 1) issue_tab(1);                                                 // (they arrive with the queries)
 
         // ---- queries: column l32, elements 16 s + 8 half ..
         v8 qf[NS][DK / 16];
@@ -168,24 +172,25 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
         const uint64_t kb = (uint64_t)(uintptr_t)a.k + it.kvh * a.k_head, vb = (uint64_t)(uintptr_t)a.v + it.kvh * a.v_head;
         auto find_rows = [&](uint32_t g) {                            // from them, row addresses and live keys
             const int32_t key = key_of(g);
-            const uint32_t own = *(const uint32_t *)(tabs + 4 * lane), tok = (uint32_t)key & a.pmask;
+            const uint32_t own = *(const uint32_t *)(tabs + (AHEAD > 1 ? (g & 1) * 256 : 0) + 4 * lane), tok = (uint32_t)key & a.pmask;
             const bool in = (key >= it.lo) & (key < it.hi) & (own < a.n_pages);
-            uint64_t * rows_of = (uint64_t *)(tabs + 256) + 64 * (g & 1) + lane;
+            uint64_t * rows_of = (uint64_t *)(tabs + P::PAGES) + 64 * (g & 1) + lane;
             const uint64_t kr = fresh(row_at(kb, own, a.k_page, tok, a.k_tok)), vr = fresh(row_at(vb, own, a.v_page, tok, a.v_tok));
             rows_of[0] = in ? kr : zero;
             rows_of[128] = in ? vr : zero;
-            // (the 16 lanes of a tile write the same)
-            ((uint16_t *)(sm_live + 4 * (g & 1) + (lane >> 4)))[wave] = (uint16_t)(__ballot(in) >> (lane & 48));
+            // (the lanes of a tile write the same)
+            typedef std::conditional_t<KW == 16, uint16_t, uint32_t> Keys;
+            ((Keys *)(sm_live + GT * (g & 1) + lane / KW))[wave] = (Keys)(__ballot(in) >> (lane & ~(KW - 1)));
         };
         auto live = [&](uint32_t t) -> uint64_t {                     // of tile t
-            const uint64_t v = sm_live[t & 7];
+            const uint64_t v = sm_live[t & (2 * GT - 1)];
             return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
         };
         // this wave's part of tile t's rows
         DmaRows<DK, false, NK> dk;
         DmaRows<DV, true, NV> dv;
-        auto read_k = [&](uint32_t t) { dk.read(tab_at + 256 + 128 * (t & 7), fresh(lane)); };
-        auto read_v = [&](uint32_t t) { dv.read(tab_at + 1280 + 128 * (t & 7), fresh(lane)); };
+        auto read_k = [&](uint32_t t) { dk.read(tab_at + P::PAGES + 8 * KW * (t & (2 * GT - 1)), fresh(lane)); };
+        auto read_v = [&](uint32_t t) { dv.read(tab_at + P::PAGES + 1024 + 8 * KW * (t & (2 * GT - 1)), fresh(lane)); };
         auto issue_k = [&](uint32_t t) { dk.issue(fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE + 1024 * NK * wave); };
         auto issue_v = [&](uint32_t t) { dv.issue(fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2 + 1024 * NV * wave); };
 
@@ -352,10 +357,11 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
             // K runs a tile ahead of V: stage t & 1 has K of tile t, then of t + 2, while V
             // of tile t is still needed.  Every wave brings its part at the begin of a round,
             // behind the barrier that tells that the round before is over, and waits
-            // for it at the begin of the next.  Rows of the next four tiles are found in
-            // round 1 of four, from page numbers asked for in round 0.
+            // for it at the begin of the next.  Rows of a group of tiles are found in
+            // a group's round 1, from page numbers asked for in its round 0.
             wait_vm<0>();
             find_rows(0);
+            if constexpr (AHEAD > 1) find_rows(1);
             read_k(0);
             read_v(0);
             issue_k(0);
@@ -373,8 +379,8 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (t + 2 < nt) issue_k(t + 2);
                 if (t + 1 < nt) issue_v(t + 1);
-                if ((t & 3) == 0 && t + 4 < nt) issue_tab(t / 4 + 1);
-                auto midway = [&]() { if ((t & 3) == 1 && t + 3 < nt) find_rows(t / 4 + 1); };
+                if (t % GT == 0 && t + AHEAD * GT < nt) issue_tab(t / GT + AHEAD);
+                auto midway = [&]() { if (t % GT == 1 && t - 1 + AHEAD * GT < nt) find_rows(t / GT + AHEAD); };
                 if (here) tile(key0 + (int32_t)(t * KT), now, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE, s, nx, midway);
                 else midway();
             };
@@ -448,11 +454,11 @@ __global__ __launch_bounds__((pre_threads<DK, DV>), pre_waves(split_terms<AT, T>
 }
 
 namespace {
-template <typename AT, typename T, int DK, int DV, bool TR> int go(const ArgsOf<TR> & a, hipStream_t s) {
-    typedef PreShape<DK, DV> P;
-    const void * k = (const void *)k_attn_pre<AT, T, DK, DV, TR>;
+template <typename AT, typename T, int DK, int DV, bool TR, int W = 4> int go(const ArgsOf<TR> & a, hipStream_t s) {
+    typedef PreShape<DK, DV, W> P;
+    const void * k = (const void *)k_attn_pre<AT, T, DK, DV, TR, W>;
     if (int rc = lds_fits(k, P::LDS, "k_attn_pre")) return rc;
-    hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV, TR>), dim3(a.grid), dim3(64 * P::W), P::LDS, s, a);
+    hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV, TR, W>), dim3(a.grid), dim3(64 * W), P::LDS, s, a);
     if (int rc = hip_check(hipGetLastError(), "k_attn_pre launch")) return rc;
     hipLaunchKernelGGL((k_attn_join<AT, T, P::M, P::KT, DV, 1, PRE_ITEM, TR>), dim3(a.grid, P::M / 16), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "k_attn_join launch");
@@ -465,13 +471,20 @@ template <typename AT, typename T, bool TR> int dims(const ArgsOf<TR> & a, hipSt
         default: return go<AT, T, 256, 256, TR>(a, s);
     }
 }
+// Trees of up to 64 rows a kv head in fp32, whose form has one wave a SIMD: strips of 64 rows, two waves, two workgroups on a
+// CU (half of the waves of a strip of 128 have no rows).  us with 128 / 64, 32 requests of 32 to 8192 keys, 32 / 8 heads of 128, over
+// f16: 9 tokens 203 / 168, 16 189 / 166, 1 to 16 178 / 148, but 20 212 / 265 (two strips), 25 228 / 279, 1 to 25 184 / 175; over bf16
+// 210 / 162, 217 / 181, 211 / 157, 247 / 293, 277 / 318, 219 / 194.  4 of 16 tokens over 65536 301 / 252 and 348 / 290.
+bool half(const AttnTreeArgs & a, bool split) { return a.tree_stride && split && attn_dims(a) < 2 && (uint64_t)a.max_q * a.group <= 64; }
 template <typename AT, typename T> int forms(const AttnTreeArgs & a, hipStream_t s) {
-    return a.tree_mask ? dims<AT, T, true>(a, s) : dims<AT, T, false>(a, s);
+    if constexpr (split_terms<AT, T>() > 1)
+        if (half(a, true)) return attn_dims(a) == 0 ? go<AT, T, 64, 64, true, 2>(a, s) : go<AT, T, 128, 128, true, 2>(a, s);
+    return a.tree_stride ? dims<AT, T, true>(a, s) : dims<AT, T, false>(a, s);
 }
 template <int DK, int DV> void shape(AttnPlan & p, bool split) {
-    static_assert(pre_waves(false, DK, DV) * PreShape<DK, DV>::LDS <= 160 * 1024, "workgroups per CU");
+    static_assert(pre_waves(false, DK, DV) * PreShape<DK, DV, 4>::LDS <= 160 * 1024, "workgroups per CU");
     p.dv = DV;
-    p.m = PreShape<DK, DV>::M;
+    p.m = PreShape<DK, DV, 4>::M;
     p.grid = (uint32_t)(num_cus() * pre_waves(split, DK, DV));
 }
 }  // namespace
@@ -484,6 +497,11 @@ AttnPlan attn_pre_plan(const AttnTreeArgs & a, uint32_t dtype) {
         case 1: shape<128, 128>(p, split); break;
         case 2: shape<192, 128>(p, split); break;
         default: shape<256, 256>(p, split); break;
+    }
+    if (half(a, split)) {
+        static_assert(3 * PreShape<64, 64, 2>::LDS <= 160 * 1024 && 2 * PreShape<128, 128, 2>::LDS <= 160 * 1024, "workgroups per CU");
+        p.m = PreShape<128, 128, 2>::M;
+        p.grid = (uint32_t)num_cus() * (attn_dims(a) == 0 ? 3 : 2);
     }
     // (64 tokens over 4096 keys: 48 us with 1 or 2, 38 with 4: fewer parts to join; over 512 keys
     // 23 us with 2, 24 with 4)

@@ -521,8 +521,7 @@ int flh_tree_plan(const flh_tree_plan_p * p, void * stream);
  * j < kv_len - n (with window > 0 those with j > kv_len - n + depth[row] - window) and key kv_len - n + b for
  * each bit b of its words of mask (any bits, also of rows behind it; the window is not applied to them).
  * A row that sees no key gives 0.  depth (NULL without a window) counts as at most n - 1.
- * Everything else, ws too, is as flh_paged_attn's, but that weights go into the products in two
- * terms up to 64 rows a kv head (max_q * n_head / n_kv_head) instead of 32. */
+ * Everything else is as flh_paged_attn's. */
 typedef struct flh_tree_p {
     const uint32_t * mask, * depth;
     uint32_t mask_stride;

@@ -105,129 +105,147 @@ int launch_kv_fork(const flh_kv_fork_p & p, hipStream_t s) {
 // One workgroup walks the requests 1024 at a time, and the pages that they leave flat, four a
 // thread and turn.  A page is put back by the last holder that leaves it, in the order of requests and pages,
 // not of time: all count themselves off first (below 0: nobody holds it any more), then the
-// place of the last one in order is found by a minimum in the page's own count, then it is put
-// back and the count is 0 again.  Without counts every page left is put back.
+// place of the last one in order is found by a minimum in the page's own count, which that one makes 0 again
+// when it puts the page back.  Without counts every page left is put back.  Rounds of loads and of
+// atomics bound it; up to 4096 pages of up to 1024 requests, what a step leaves, are found once and stay in registers (8 forks
+// of 126 pages each 10.2 us, 18.0 found again in each round; 64 requests of 3 pages 7.0, 13.4).  Many more take a
+// microsecond for about 90 pages (8192 pages 94 us), 700 without counts.
 struct TrimOf {
     uint32_t before, after, part;       // pages held, pages kept, tokens in a last one that is partly filled
 };
-__device__ __forceinline__ TrimOf trim_of(const flh_kv_trim_p & p, uint32_t s, uint32_t sh, uint32_t & keep) {
-    const uint64_t ps = 1ull << sh, held = p.kv_len[s];
-    keep = min(p.kv_len[s], p.keep[s]);
+__device__ __forceinline__ TrimOf trim_of(const flh_kv_trim_p & p, uint32_t held, uint32_t keep, uint32_t sh) {
+    const uint64_t ps = 1ull << sh, all = ((uint64_t)keep + ps - 1) >> sh;
     TrimOf t;
-    t.before = (uint32_t)min((held + ps - 1) >> sh, (uint64_t)p.table_stride);
-    const uint64_t all = ((uint64_t)keep + ps - 1) >> sh;
+    t.before = (uint32_t)min(((uint64_t)held + ps - 1) >> sh, (uint64_t)p.table_stride);
     t.after = (uint32_t)min(all, (uint64_t)p.table_stride);
     t.part = all <= p.table_stride ? keep & (uint32_t)(ps - 1) : 0;
     return t;
 }
 
 __global__ __launch_bounds__(PG_T) void k_kv_trim(flh_kv_trim_p p, uint32_t sh) {
-    __shared__ uint32_t ws[PG_T / 64], l_at[PG_T], l_from[PG_T];
-    __shared__ uint8_t l_own[PG_T];
+    constexpr uint32_t N = 4;
+    __shared__ uint32_t ws[PG_T / 64], l_at[PG_T], l_from[PG_T], l_own[PG_T];
     const uint32_t tid = threadIdx.x;
-    uint32_t taken = min(*p.taken, p.n_free), lost = 0;
-    // ---- a last page that others hold too: a fresh one in its place (before anybody leaves a page)
-    if (p.shared)
-        for (uint32_t s0 = 0; s0 < p.n_seq; s0 += PG_T) {
-            const uint32_t s = s0 + tid;
-            uint32_t keep, last = FLH_KV_NONE, fresh = FLH_KV_NONE;
-            TrimOf t{0, 0, 0};
-            if (s < p.n_seq) t = trim_of(p, s, sh, keep);
+    const bool once = p.n_seq <= PG_T;
+    uint32_t taken = min(*p.taken, p.n_free), lost = 0, sum = 0;
+    // A batch of requests: where their pages are on the line of all that are left (l_at), from which table entry on; l_own: a
+    // last page that others hold too, which is left, too, and has a fresh one in its place (before anybody leaves a page)
+    auto batch = [&](uint32_t s0, bool first) {
+        const uint32_t s = s0 + tid;
+        uint32_t own = FLH_KV_NONE;
+        TrimOf t{0, 0, 0};
+        if (s < p.n_seq) {
+            const uint32_t held = p.kv_len[s];
+            t = trim_of(p, held, min(held, p.keep[s]), sh);
+        }
+        if (p.shared && first) {
             uint32_t * at = p.table + (uint64_t)s * p.table_stride + (t.after - 1);
+            uint32_t last = FLH_KV_NONE, fresh = FLH_KV_NONE;
             if (t.part) last = *at;
-            const uint32_t need = last < p.n_pages && p.shared[last] != 0;
-            uint32_t sum;
+            const bool need = last < p.n_pages && p.shared[last] != 0;
             const uint32_t i = taken + scan_before(need, ws, &sum);
             if (need && i < p.n_free) fresh = p.free_pages[i];
             const bool got = fresh < p.n_pages;
             if (s < p.n_seq) {
-                p.copy_src[s] = need ? last << sh : FLH_KV_NONE;
+                p.copy_src[s] = need ? last << sh : FLH_KV_NONE;  // (without a page to go to: until the end)
                 p.copy_dst[s] = got ? fresh << sh : FLH_KV_NONE;
                 p.copy_n[s] = got ? t.part : 0;
                 if (need) *at = got ? fresh : FLH_KV_NONE;
             }
+            if (need) own = last;
             lost += __syncthreads_count(need && !got);
             taken = min(p.n_free, taken + sum);
+        } else if (p.shared && s < p.n_seq) {
+            own = p.copy_src[s];
+            if (own != FLH_KV_NONE) own >>= sh;
         }
-    __syncthreads();
-    // ---- the pages that are left: begin(i, page) for each, i its place in the order of all
+        const uint32_t at = scan_before(t.before - t.after + (own != FLH_KV_NONE), ws, &sum);
+        l_at[tid] = at;
+        l_from[tid] = t.after;
+        l_own[tid] = own;
+        __syncthreads();
+    };
+    // entry i of the batch's line: the page, and its place in the table (null: none)
+    auto entry = [&](uint32_t s0, uint32_t i, uint32_t & e, uint32_t *& in) {
+        e = FLH_KV_NONE;
+        in = nullptr;
+        if (i >= sum) return;
+        uint32_t lo = 0, n = min(PG_T, p.n_seq - s0);
+        while (n > 1) {
+            const uint32_t h = n >> 1;
+            if (l_at[lo + h] <= i) { lo += h; n -= h; }
+            else n = h;
+        }
+        const uint32_t j = i - l_at[lo], own = l_own[lo];
+        if (own != FLH_KV_NONE && j == 0) e = own;
+        else {
+            in = p.table + (uint64_t)(s0 + lo) * p.table_stride + l_from[lo] + j - (own != FLH_KV_NONE);
+            e = *in;
+        }
+    };
+    uint32_t e[N];
+    uint32_t * in[N];
+    bool kept = false;
+    // with(i, page, place) for every page that is left, i its place in the order of all; all threads together
     auto each = [&](auto && with) {
-        uint32_t base = 0;
-        for (uint32_t s0 = 0; s0 < p.n_seq; s0 += PG_T) {
-            const uint32_t s = s0 + tid, nb = min(PG_T, p.n_seq - s0);
-            uint32_t keep, own = 0;
-            TrimOf t{0, 0, 0};
-            if (s < p.n_seq) {
-                t = trim_of(p, s, sh, keep);
-                own = p.shared && p.copy_src[s] != FLH_KV_NONE;   // (its last page is left, too)
-            }
-            uint32_t sum;
-            const uint32_t at = scan_before(t.before - t.after + own, ws, &sum);
-            l_at[tid] = at;
-            l_from[tid] = t.after;
-            l_own[tid] = (uint8_t)own;
-            __syncthreads();
-            constexpr uint32_t N = 4;
-            for (uint32_t i0 = 0; i0 < sum; i0 += N * PG_T) {
-                uint32_t e[N];
-                uint32_t * in[N];
+        if (kept) {
 #pragma unroll
-                for (uint32_t k = 0; k < N; ++k) {
-                    const uint32_t i = i0 + k * PG_T + tid;
-                    e[k] = FLH_KV_NONE;
-                    in[k] = nullptr;
-                    if (i >= sum) continue;
-                    uint32_t lo = 0, n = nb;
-                    while (n > 1) {
-                        const uint32_t h = n >> 1;
-                        if (l_at[lo + h] <= i) { lo += h; n -= h; }
-                        else n = h;
-                    }
-                    const uint32_t j = i - l_at[lo];
-                    if (l_own[lo] && j == 0) e[k] = p.copy_src[s0 + lo] >> sh;
-                    else {
-                        in[k] = p.table + (uint64_t)(s0 + lo) * p.table_stride + l_from[lo] + j - l_own[lo];
-                        e[k] = *in[k];
-                    }
+            for (uint32_t k = 0; k < N; ++k)
+                if (k * PG_T < sum) with(k * PG_T + tid, e[k], in[k]);
+        } else {
+            uint32_t base = 0;
+            for (uint32_t s0 = 0; s0 < p.n_seq; s0 += PG_T) {
+                if (!once) batch(s0, false);
+                for (uint32_t i0 = 0; i0 < sum; i0 += N * PG_T) {
+#pragma unroll
+                    for (uint32_t k = 0; k < N; ++k) entry(s0, i0 + k * PG_T + tid, e[k], in[k]);
+#pragma unroll
+                    for (uint32_t k = 0; k < N; ++k)
+                        if (i0 + k * PG_T < sum) with(base + i0 + k * PG_T + tid, e[k], in[k]);
                 }
-#pragma unroll
-                for (uint32_t k = 0; k < N; ++k) with(base + i0 + k * PG_T + tid, e[k], in[k]);
+                base += sum;
+                __syncthreads();                                  // the tables in LDS are the next batch's
             }
-            base += sum;
-            __syncthreads();                                      // the tables in LDS are the next batch's
         }
         __threadfence_block();
         __syncthreads();
     };
+    for (uint32_t s0 = 0; s0 < p.n_seq; s0 += PG_T)
+        if (once || p.shared) {
+            batch(s0, true);
+            __syncthreads();
+        }
+    if (once && sum <= N * PG_T) {
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) entry(0, k * PG_T + tid, e[k], in[k]);
+        kept = true;
+    }
+    int32_t * count = (int32_t *)p.shared;
     if (p.shared) {
-        int32_t * count = (int32_t *)p.shared;
-        each([&](uint32_t, uint32_t e, uint32_t *) { if (e < p.n_pages) atomicSub(count + e, 1); });
-        // (a page that is left more often than it was held: as if as often)
-        each([&](uint32_t, uint32_t e, uint32_t *) { if (e < p.n_pages) atomicMax(count + e, -1); });
-        each([&](uint32_t i, uint32_t e, uint32_t *) {
-            if (e < p.n_pages && __hip_atomic_load(count + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < 0)
-                atomicMin(count + e, -2 - (int32_t)i);
+        each([&](uint32_t, uint32_t x, uint32_t *) { if (x < p.n_pages) atomicSub(count + x, 1); });
+        // (-2 - the last one's place is below the count, also of a page that was left more often than it was held: places
+        // are as many)
+        each([&](uint32_t i, uint32_t x, uint32_t *) {
+            if (x < p.n_pages && __hip_atomic_load(count + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < 0)
+                atomicMin(count + x, -2 - (int32_t)i);
         });
     }
     // ---- put back, one after another: the last one is taken next
     uint32_t back = 0;
-    each([&](uint32_t i, uint32_t e, uint32_t * in) {
-        bool mine = e < p.n_pages;
+    each([&](uint32_t i, uint32_t x, uint32_t * at) {
+        bool mine = x < p.n_pages;
         if (p.shared && mine) {
-            int32_t * c = (int32_t *)p.shared + e;
-            mine = __hip_atomic_load(c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == -2 - (int32_t)i;
-            if (mine) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            mine = __hip_atomic_load(count + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == -2 - (int32_t)i;
+            if (mine) __hip_atomic_store(count + x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        uint32_t sum;
-        const uint32_t at = back + scan_before(mine, ws, &sum);
-        if (mine && at < taken) p.free_pages[taken - 1 - at] = e;
-        if (in) *in = FLH_KV_NONE;
-        back += sum;
+        uint32_t all;
+        const uint32_t to = back + scan_before(mine, ws, &all);
+        if (mine && to < taken) p.free_pages[taken - 1 - to] = x;
+        if (at) *at = FLH_KV_NONE;
+        back += all;
     });
     for (uint32_t s = tid; s < p.n_seq; s += PG_T) {
-        uint32_t keep;
-        (void)trim_of(p, s, sh, keep);
-        p.held[s] = keep;
+        p.held[s] = min(p.kv_len[s], p.keep[s]);
         if (p.shared && p.copy_dst[s] == FLH_KV_NONE) p.copy_src[s] = FLH_KV_NONE;
     }
     if (tid == 0) {

@@ -269,7 +269,7 @@ __device__ __forceinline__ uint32_t children(const flh_verify_p & p, uint32_t r0
 // ------------------------------------------------------------- the rows' sums --
 // Workgroup (row, side, chunk) of the target or of the draft (rows with children), two waves.  Instructions bound it:
 // 20 an element, and 330 a wave for whose row it is and for putting the sums together, so a thread has 32 elements (with 16
-// it takes 28 us for 32 requests of 2 to 6 rows of 128256, and WITH_E32).  Longer shares, the next chunk's logits on their way
+// they take 28 us for 32 requests of 2 to 6 rows of 128256 with a draft, so 25).  Longer shares, the next chunk's logits on their way
 // meanwhile, leave the last workgroups alone for longer than they save.  The target's logits are asked for before it is
 // known whose they are.
 constexpr int SUM_W = 2;
@@ -503,15 +503,22 @@ template <typename T> __global__ __launch_bounds__(VER_T) void k_verify_next(Ver
     w.tok[tid] = tok;
     // (a draft's row without children: anything, and not used)
     const bool drafts = p.draft && !greedy;
-    for (uint32_t i0 = 0; i0 < (drafts ? 2 * n : n); i0 += VER_T / 4) {
-        const uint32_t x = i0 + tid / 4;
-        const bool d = x >= n && drafts;
-        const uint32_t i = min(d ? x - n : x, n - 1);
-        const VerRow r = merge_row<4>((d ? a.dp : a.tp) + (uint64_t)(r0 + i) * a.nc, a.nc, wt);
-        (d ? w.dm : w.tm)[i] = r.m;
-        (d ? w.dz : w.tz)[i] = r.z;
-        if (!d) w.at[i] = r.at;
-    }
+    const uint32_t merges = drafts ? 2 * n : n;
+    auto merge = [&](auto lanes) {                                    // a row's parts by so many lanes
+        constexpr uint32_t G = decltype(lanes)::value;
+        for (uint32_t i0 = 0; i0 < merges; i0 += VER_T / G) {
+            if (i0 + (tid & ~63u) / G >= merges) break;               // (no row for this wave)
+            const uint32_t x = i0 + tid / G;
+            const bool d = x >= n && drafts;
+            const uint32_t i = min(d ? x - n : x, n - 1);
+            const VerRow r = merge_row<G>((d ? a.dp : a.tp) + (uint64_t)(r0 + i) * a.nc, a.nc, wt);
+            (d ? w.dm : w.tm)[i] = r.m;
+            (d ? w.dz : w.tz)[i] = r.z;
+            if (!d) w.at[i] = r.at;
+        }
+    };
+    if (merges <= VER_T / 16) merge(std::integral_constant<int, 16>());
+    else merge(std::integral_constant<int, 4>());
     __syncthreads();
     uint32_t rank = 0;
     if (p.parent && up != NO_ROW)

@@ -31,8 +31,8 @@ int check_verify(const flh_verify_p * p) {
     if (p->vocab == 0 || p->vocab > (1u << 22)) return set_error(FLH_ERR_UNSUPPORTED, "verify: vocab must be in 1 .. 2^22");
     if (p->path_stride == 0) return set_error(FLH_ERR_ARG, "verify: path_stride must be at least 1");
     if (p->max_child == 0 || p->max_child > 64) return set_error(FLH_ERR_ARG, "verify: max_child must be in 1 .. 64");
-    const uint64_t chunks = (p->vocab + 4095) / 4096;
-    if (2 * p->n_tok * chunks >= (1ull << 31) || p->n_seq * chunks >= (1ull << 31))
+    const uint64_t chunks = (p->vocab + 4095) / 4096;             // (a grid's threads are counted in 32 bits)
+    if (p->n_tok * chunks >= (1u << 24) || p->n_seq * chunks >= (1u << 24))
         return set_error(FLH_ERR_UNSUPPORTED, "verify: too many rows for one call");
     return FLH_OK;
 }
@@ -63,6 +63,7 @@ extern "C" {
 int flh_tree_plan(const flh_tree_plan_p * p, void * stream) {
     if (!p) return set_error(FLH_ERR_ARG, "tree plan: null arguments");
     if (p->mask_stride == 0 || p->mask_stride > 32768) return set_error(FLH_ERR_ARG, "tree plan: mask_stride must be in 1 .. 32768");
+    if (p->n_tok > (1u << 30)) return set_error(FLH_ERR_UNSUPPORTED, "tree plan: n_tok must be at most 2^30");
     if (p->n_tok && p->n_seq && (any_null({p->q_start, p->parent, p->mask, p->depth}) || (p->pos && !p->kv_len)))
         return set_error(FLH_ERR_ARG, "tree plan: null argument");
     if (any_off({p->q_start, p->parent, p->kv_len, p->mask, p->depth, p->pos}))
@@ -122,7 +123,7 @@ int flh_kv_copy(const flh_kv_cache * caches, uint32_t n_cache, const uint32_t * 
 int flh_kv_fork(const flh_kv_fork_p * p, void * stream) {
     if (!p) return set_error(FLH_ERR_ARG, "kv fork: null arguments");
     if (int rc = check_pages(p->n_pages, p->page_size)) return rc;
-    if (p->n_fork > (1u << 30)) return set_error(FLH_ERR_UNSUPPORTED, "kv fork: n_fork must be at most 2^30");
+    if (p->n_fork > (1u << 21)) return set_error(FLH_ERR_UNSUPPORTED, "kv fork: n_fork must be at most 2^21");
     if (p->n_fork && (any_null({p->src, p->dst, p->kv_len, p->table, p->taken, p->shared, p->copy_src, p->copy_dst, p->copy_n}) ||
                       (p->n_free && !p->free_pages) || p->table_stride == 0))
         return set_error(FLH_ERR_ARG, "kv fork: null argument");

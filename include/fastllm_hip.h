@@ -509,7 +509,7 @@ int flh_paged_attn(const flh_kv_cache * cache, const flh_attn_p * p, void * stre
  * request is r itself or above it (rows b >= 32 * mask_stride have no bit), with window > 0 only those
  * less than window above it; pos[r] (may be NULL, then kv_len too): kv_len[s] - rows of the
  * request + depth[r].  Rows n_tok and behind, and rows of no request, are left as they are.
- * mask_stride: 1 .. 32768.  Outputs must not overlap anything. */
+ * mask_stride: 1 .. 32768; n_tok: at most 2^30.  Outputs must not overlap anything. */
 typedef struct flh_tree_plan_p {
     const uint32_t * q_start; const int32_t * parent; const uint32_t * kv_len;
     uint32_t * mask, * depth; int32_t * pos;
@@ -549,8 +549,8 @@ int flh_tree_attn(const flh_kv_cache * cache, const flh_attn_p * p, const flh_tr
  * logp (or NULL): entry j of a request, the logarithm of p (of the row, as it was) at the token behind the path's row j: that of row
  * j + 1, at last next; 0 behind.  len (or NULL, then kv_len may be): kv_len[s] - rows + n_path[s], what the
  * request holds then.  ws: flh_spec_verify_ws_bytes of the same arguments, 16-byte aligned, as
- * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; n_tok times the vocabulary's
- * chunks of 4096 below 2^30. */
+ * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; n_tok and n_seq, times the
+ * vocabulary's chunks of 4096, below 2^24. */
 typedef struct flh_verify_p {
     const void * target, * draft;
     const uint32_t * q_start, * token; const int32_t * parent;
@@ -593,7 +593,7 @@ int flh_kv_copy(const flh_kv_cache * caches, uint32_t n_cache, const uint32_t * 
  * flh_kv_copy has to run before dst is read or src's page written again.  kv_len[dst[i]] is set.  Where the list ran out
  * the entry is FLH_KV_NONE (those tokens are not seen), *taken > n_free, and info[1] (info may be NULL) counts it;
  * info[0]: copies.  An entry that is no page is FLH_KV_NONE in dst, too.  dst differ from each other and from every src; a
- * pair of which one is not below n_seq, or that is one and the same, is left out.
+ * pair of which one is not below n_seq, or that is one and the same, is left out.  n_fork: at most 2^21.
  *
  * flh_kv_trim: request s holds min(kv_len[s], keep[s]) tokens afterwards (held[s]; may be kv_len).  Pages
  * behind them are left: their table entries are FLH_KV_NONE, and those that nobody holds any more go back to

@@ -393,3 +393,65 @@ def test_offsets_past_32_bits(flh, gpu):
     for at in (5, last - page):
         np.testing.assert_array_equal(buf.download(np.uint8, row, gpu, offset=at * row), want)
     buf.close()
+
+
+def test_more_requests_and_copies_than_a_grid_has(flh, gpu):
+    """70000 requests of two rows, of which the second one stands where the first was dropped, and as many copies."""
+    n, page = 70000, 16
+    pages = 2 * n // page + 1
+    buf = flh.DeviceBuffer(pages * page * 64)
+    rows = np.arange(pages * page, dtype=np.uint32)
+    data = np.repeat(rows[:, None], 16, 1)                    # a token: 16 bytes of keys, 48 of values
+    buf.upload(data, gpu)
+    cache = flh.KvCache(buf.ptr, buf.ptr + 16, flh.Dtype.F16, pages, page, 1, 8, 24, (page * 32, 32, 8), (page * 32, 32, 8))
+    start = (2 * np.arange(n + 1)).astype(np.uint32)
+    b = [up(flh, gpu, x) for x in (start, np.arange(2 * n, dtype=np.uint32), np.full(n, 1, np.uint32), np.ones(n, np.uint32))]
+    flh.kv_compact(flh.KvCaches([cache]), flh.KvCompactP(q_start=b[0].ptr, slot=b[1].ptr, n_path=b[2].ptr, path=b[3].ptr, n_seq=n,
+                                                         n_tok=2 * n, path_stride=1), gpu)
+    want = rows.copy()
+    want[0:2 * n:2] = rows[1:2 * n:2]
+    got = buf.download(np.uint32, data.size, gpu).reshape(data.shape)
+    assert (got == want[:, None]).all()
+    c = [up(flh, gpu, x) for x in (start[:n], start[:n] + np.uint32(1), np.ones(n, np.uint32))]
+    buf.upload(data, gpu)
+    flh.kv_copy(flh.KvCaches([cache]), c[0], c[1], c[2], n, gpu)
+    want = rows.copy()
+    want[1:2 * n:2] = rows[0:2 * n:2]
+    got = buf.download(np.uint32, data.size, gpu).reshape(data.shape)
+    assert (got == want[:, None]).all()
+
+
+def test_captured(flh, gpu):
+    """Fork, copy and trim as graphs of one kernel each, and as one, replayed: the requests go back and forth."""
+    b = Book(flh, gpu, 16, 4, 8, 40, 11)
+    b.take(0, 75)
+    p = b.push(4)
+    ls = Layers(flh, gpu, 3, "F16", 40, 16, 2, 64, 64, "head", 0, 5)
+    a = [up(flh, gpu, np.array(x, np.uint32)) for x in ([0, 0], [1, 2], [0xFFFFFFFF, 0, 0, 0])]
+    first = b.read()
+    steps = [lambda: flh.kv_fork(flh.KvForkP(src=a[0].ptr, dst=a[1].ptr, n_fork=2, **p), gpu),
+             lambda: flh.kv_copy(ls.all, b.lists[0], b.lists[1], b.lists[2], 2, gpu),
+             lambda: flh.kv_trim(flh.KvTrimP(keep=a[2].ptr, held=p["kv_len"], **p), gpu)]
+    graphs = []
+    for group in ([steps[0]], [steps[1]], [steps[2]], steps):
+        with flh.Graph.capture(gpu) as g:
+            for f in group:
+                f()
+        graphs.append(g)
+    for turn in range(4):
+        if turn % 2:
+            graphs[3].launch()
+        else:
+            graphs[0].launch()
+            mid = b.read()
+            assert mid["held"].tolist() == [75, 75, 75, 0] and mid["info"] == [2, 0] and mid["taken"] == 7
+            assert (mid["shared"][first["table"][0, :4]] == 2).all() and mid["num"][:2].tolist() == [11, 11]
+            graphs[1].launch()
+            ls.check([(int(mid["src"][i]) + t, int(mid["dst"][i]) + t) for i in range(2) for t in range(11)])
+            graphs[2].launch()
+        got = b.read()
+        assert got["taken"] == 5 and got["held"].tolist() == [75, 0, 0, 0] and got["info"] == [2, 0]
+        np.testing.assert_array_equal(got["table"], first["table"])
+        assert (got["shared"] == 0).all() and sorted(got["free"][5:].tolist()) == sorted(first["free"][5:].tolist())
+    for g in graphs:
+        g.close()

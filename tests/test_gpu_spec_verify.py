@@ -299,3 +299,15 @@ def test_logits_of_any_size(flh, gpu, draft):
         v.inv_temp[s] = temp[s]
     v.push().run()
     v.check()
+
+
+@pytest.mark.parametrize("n_seq", [62, 63, 64, 65, 128, 700])
+def test_numbers_of_requests(flh, gpu, n_seq):
+    """A row's request is found 64 at a time: around that, with requests of no rows among them."""
+    rng = np.random.default_rng(n_seq)
+    n = rng.integers(0, 7, n_seq).tolist()
+    n[0], n[-1] = (0, 3) if n_seq % 2 else (4, 0)
+    for draft in (False, True):
+        v = Verify(flh, gpu, n, 60, "F32", draft, 2, seed=n_seq, lead=n_seq % 3, peak=2.0).push()
+        v.run()
+        v.check()

@@ -53,6 +53,13 @@ def test_tree_plan_refusals(flh, word, kw):
     refused(flh, flh.ERR_ARG, word, flh.tree_plan, tree_plan(flh, **kw), S)
 
 
+def test_sizes_that_are_too_large(flh):
+    refused(flh, flh.ERR_UNSUPPORTED, "n_tok", flh.tree_plan, tree_plan(flh, n_tok=(1 << 30) + 1), S)
+    refused(flh, flh.ERR_UNSUPPORTED, "n_fork", flh.kv_fork, fork(flh, n_fork=(1 << 21) + 1), S)
+    for kw in (dict(n_tok=1 << 24, vocab=1), dict(n_seq=1 << 24, vocab=1), dict(n_tok=1 << 19, vocab=128256), dict(n_tok=0xFFFFFFFF, vocab=5)):
+        refused(flh, flh.ERR_UNSUPPORTED, "rows", flh.spec_verify, verify(flh, **kw), S)
+
+
 @pytest.mark.parametrize("word,kw,akw", [
     ("mask", dict(mask=None), {}), ("mask", dict(mask=P + 2), {}), ("mask_stride", dict(mask_stride=0), {}),
     ("mask_stride", dict(mask_stride=40000), {}), ("depth", dict(depth=None), dict(window=5)), ("depth", dict(depth=P + 1), {}),

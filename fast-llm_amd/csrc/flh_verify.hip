@@ -420,7 +420,8 @@ __device__ __forceinline__ VerLeft left_of(const VerRow & t, const VerRow & d, d
 }
 
 // n_i, i = `round`, of the rows with more than i children: workgroup (row, chunk).  Its waves put the row's sums
-// together, one each, while the logits are on their way.
+// together, one each, while the logits are on their way.  16 requests of 7 to 21 rows, 50257 tokens in bf16: 14 us, of
+// which the instructions of two exponentials an element are about 4 and three rounds of loads the rest.
 template <typename T> __global__ __launch_bounds__(VER_T) void k_verify_rest(VerArgs a, uint32_t round) {
     __shared__ double sm[4], sm_z[2], sm_t;
     __shared__ float sm_m[2];
@@ -450,7 +451,9 @@ template <typename T> __global__ __launch_bounds__(VER_T) void k_verify_rest(Ver
 
 // -------------------------------------------------------- the walk and the draw --
 // A thread a row: its parent, its token and what its test needs are asked for at once, before the
-// rows' sums are put together (16 lanes a row), so the walk is three rounds of loads long.
+// rows' sums are put together (16 lanes a row), so the walk is three rounds of loads long.  With a draft every
+// workgroup of a request (one a chunk) walks by itself, then sums what is left of its chunk of the row at the path's end; the last
+// one to finish draws: 17 to 19 us for 32 requests of 128256 tokens, 8 to 10 for one without a draft.  Rounds of loads bound it.
 struct VerWalk {
     double tz[VER_ROWS], dz[VER_ROWS], pc[VER_ROWS];                  // sums of rows; p of rows' tokens
     double t[VER_ROWS], n[VER_ROWS];                                  // what rows' tests are against

@@ -549,7 +549,8 @@ int flh_tree_attn(const flh_kv_cache * cache, const flh_attn_p * p, const flh_tr
  * logp (or NULL): entry j of a request, the logarithm of p (of the row, as it was) at the token behind the path's row j: that of row
  * j + 1, at last next; 0 behind.  len (or NULL, then kv_len may be): kv_len[s] - rows + n_path[s], what the
  * request holds then.  ws: flh_spec_verify_ws_bytes of the same arguments, 16-byte aligned, as
- * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; n_tok and n_seq, times the
+ * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; all n_tok rows of target, and
+ * of draft, have to be there, also those of no request; n_tok and n_seq, times the
  * vocabulary's chunks of 4096, below 2^24. */
 typedef struct flh_verify_p {
     const void * target, * draft;

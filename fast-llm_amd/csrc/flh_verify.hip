@@ -586,7 +586,9 @@ template <typename T> __global__ __launch_bounds__(VER_T) void k_verify_next(Ver
             w.path[len++] = (uint8_t)cur;
         }
         w.len = len;
-        w.k = w.best[cur] == NO_ROW;                                  // (a path cut off ends as at a row without children)
+        // (A path cut off ends as at a row without children, whether one of them would have stood or not: drawn from what
+        // is left where none would, the token would not be distributed as p.)
+        w.k = len < p.path_stride;
         n_again = 0;
     }
     __syncthreads();

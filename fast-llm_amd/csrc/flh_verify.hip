@@ -485,7 +485,7 @@ template <typename T> __global__ __launch_bounds__(VER_T) void k_verify_next(Ver
         if (tid == 0) {
             p.n_path[s] = 0;
             p.next[s] = FLH_KV_NONE;
-            if (p.len) p.len[s] = p.kv_len[s];
+            if (p.len) p.len[s] = p.kv_len[s] - rows;                 // (rows that n_tok cuts off have no keys)
         }
         return;
     }

@@ -19,6 +19,7 @@
 #include "flh_internal.h"
 #include "flh_status.h"
 #include <float.h>
+#include <type_traits>
 
 namespace flh {
 
@@ -110,7 +111,16 @@ struct VerExp {
         pow2<N>(f, t, e);
     }
 };
-// A logit: what is no number counts as -infinity, infinity as the largest number: the median of three, which is their
+// A logit as it is in memory.  One that is no number is a quiet one behind this: of a signalling one the instructions below
+// make a quiet one first and then the other operand, which would be the largest number.  The conversion from f16
+// quiets by itself; the compiler would leave a multiplication by 1 out.
+template <typename T> __device__ __forceinline__ float number(T x) {
+    if constexpr (std::is_same_v<T, _Float16>) return (float)x;
+    float y;
+    asm("v_max_f32 %0, %1, %1" : "=v"(y) : "v"((float)x));
+    return y;
+}
+// What is no number counts as -infinity, infinity as the largest number: the median of three, which is their
 // smallest where one is no number.  (In asm: the compiler takes the median with -infinity for a minimum of two, which
 // makes the largest number of what is none.)
 __device__ __forceinline__ float logit(float x, float low = -INFINITY) {
@@ -118,10 +128,11 @@ __device__ __forceinline__ float logit(float x, float low = -INFINITY) {
     asm("v_med3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "v"(low), "s"(FLT_MAX));
     return y;
 }
-// the largest of three that is a number (in asm: the compiler would look for signalling ones first)
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// the largest of three that is a number (in asm: the compiler would look for signalling ones first), or, MUST, no number where one is none
+template <bool MUST = false> __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+    if constexpr (MUST) asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+    else asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
     return y;
 }
 // Sums, maxima and minima over groups of G lanes, the same in each of them (all lanes of the wave are on), without
@@ -190,7 +201,7 @@ template <typename T, bool IN_ORDER, int W = 4> struct Chunk {
     // the logits (RAW: as they are), and which token element e is
     template <bool RAW = false> __device__ __forceinline__ void get(uint32_t c, uint32_t v, float (&x)[E]) const {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = RAW ? (float)t[e / N].v[e % N] : logit((float)t[e / N].v[e % N]);
+        for (int e = 0; e < E; ++e) x[e] = RAW ? (float)t[e / N].v[e % N] : logit(number(t[e / N].v[e % N]));
         if ((c + 1) * VER_CH <= v) return;                            // (uniform)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -300,7 +311,14 @@ template <typename T> __global__ __launch_bounds__(64 * SUM_W) void k_verify_sum
     chunk.template get<true>(c, p.vocab, x);
     VerPart o{0, -INFINITY, NO_ROW};
 #pragma unroll
-    for (int i = 0; i < C::E; i += 2) o.m = max3(o.m, x[i], x[i + 1]);
+    for (int i = 0; i < C::E; i += 2) o.m = max3<true>(o.m, x[i], x[i + 1]);
+    if (__ballot(isnan(o.m))) {                                       // (hardly ever: 43 us for 32 chains instead of 44 with `number` for all)
+        o.m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < C::E; ++i) x[i] = number(x[i]);
+#pragma unroll
+        for (int i = 0; i < C::E; i += 2) o.m = max3(o.m, x[i], x[i + 1]);
+    }
     o.m = group_max(fminf(o.m, FLT_MAX));
     if (greedy) {
 #pragma unroll
@@ -529,7 +547,7 @@ template <typename T> __global__ __launch_bounds__(VER_T) void k_verify_next(Ver
     const bool tested = up != NO_ROW && rank < p.max_child;
     w.rank[tid] = tested ? (uint8_t)rank : 255;
     // ---- p of the rows' tokens
-    const float xl = logit((float)xt), yl = logit((float)yt);
+    const float xl = logit(number(xt)), yl = logit(number(yt));
     double e = 0, pc = 0;
     if (drafted) {
         e = greedy ? 0.0 : VerExp(w.tm[up], it).of(xl);

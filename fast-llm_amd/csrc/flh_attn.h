@@ -546,9 +546,11 @@ __global__ __launch_bounds__(256) void k_attn_join(ArgsOf<TR> a) {
     __shared__ float red[PW > 1 ? PW : 1][R][PW > 1 ? DV : 1];
     // Workgroups are dealt to the 8 XCDs in turn, and items that begin every 16, 32, .. workgroups would all be one XCD's,
     // whose share of the parts' bytes bounds it then (8 tokens over 4001 keys: 14 us, 6 so): within 8 neighbours w turns with
-    // the bits above and with y.
+    // the bits above and with y.  Where one wave has all the rows (a single token of 4 heads), its bytes are few and its
+    // own XCD's L2 has its note: one token over 4001 keys takes 13.9 us with w as it is and 14.5 turned, 2 tokens, 8 rows, 15.7 and 14.7.
     const uint32_t lane = threadIdx.x & 63, g8 = blockIdx.x >> 3;
-    const uint32_t w = a.grid % 8 ? blockIdx.x : g8 << 3 | ((blockIdx.x + (g8 ^ g8 >> 3 ^ g8 >> 6) + blockIdx.y) & 7);
+    const bool turn = a.grid % 8 == 0 && (uint64_t)a.max_q * a.group > R;
+    const uint32_t w = turn ? g8 << 3 | ((blockIdx.x + (g8 ^ g8 >> 3 ^ g8 >> 6) + blockIdx.y) & 7) : blockIdx.x;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const AttnNote * notes = attn_notes<M, DV>(a);
     // workgroups that the main kernel had no work for left no note: their number

@@ -36,6 +36,7 @@ template <int DK, int DV> struct DecShape {
 // 32 / 8 heads of 128 in bf16: 64 requests of 20 to 1000 keys 93 / 64 / 55 / 55, 32 of 32 to 8192 169 / 145 / 134 / 135, 32 of 4096
 // 106 / 107 / 107 / 106, 4 of 32768 111 / 114 / 113 / 115.  (Runs of drafted tokens keep the sums they have: 0.)
 constexpr int dec_item(bool tree) { return tree ? 4 : 0; }
+static_assert(dec_item(true) <= ATTN_ITEM && dec_item(false) <= ATTN_ITEM, "the host's count of units");
 template <int DK, int DV> constexpr int dec_threads = 64 * DecShape<DK, DV>::W;
 
 template <typename AT, typename T, int DK, int DV, int MT, bool TR>

@@ -34,6 +34,7 @@ namespace flh {
 // 649 / 626 / 626, over bf16 797 / 776 / 751 / 753, of heads of 256 1389 / 1332 / 1273 / 1254; 8 x 20 heads
 // of 64 over 1500 keys 58 / 58 / 55 / 58; 64 requests of 40 rows over 500 keys 132 / 136 / 136 / 136.
 constexpr int PRE_ITEM = 3;
+static_assert(PRE_ITEM <= ATTN_ITEM, "the host's count of units");
 // STAGES of the ring: with two, V of a tile comes in the round before it and K in the one before that; with three, where
 // a CU's LDS holds them, both a round earlier (5 ragged chunks in fp32 over f16 603 us, 619 with two; 32 trees of 25 tokens
 // over up to 8192 keys 211, 218; of heads of 192 215, 229).

@@ -230,6 +230,8 @@ struct AttnTreeArgs : AttnArgs {
     const uint32_t * tree_mask; const uint32_t * tree_depth;
     uint32_t tree_stride;               // words of a row of tree_mask
 };
+// the most units that a strip of attention's rows counts for beside its tiles of 64 keys or more (flh_attn_dec.hip, flh_attn_pre.hip)
+constexpr int ATTN_ITEM = 4;
 int check_kv_cache(const flh_kv_cache * c);               // (flh_paged.cpp)
 int launch_kv_plan(const flh_kv_plan_p & p, hipStream_t s);
 int launch_rope(const RopeArgs & a, uint32_t dtype, uint32_t cache_dtype, hipStream_t s);

@@ -493,14 +493,27 @@ template <typename AT, typename T, bool TR> int dims(const ArgsOf<TR> & a, hipSt
 }
 // Trees in fp32, whose form has one wave a SIMD: strips of 64 rows, two waves, two workgroups on a CU, where no request has
 // more rows a kv head, or most have no more (half of the waves of a strip of 128 would have no rows).  us with 128 / 64, 32
-// requests of 32 to 8192 keys, 32 / 8 heads of 128, over f16: 9 tokens 173 / 137, 16 179 / 150, 1 to 16 172 / 135, 1 to 25
-// 178 / 163, but 20 194 / 250 (two strips), 25 211 / 259; over bf16 208 / 152, 212 / 164, 209 / 145, 214 / 176, 226 / 270,
-// 251 / 292.  4 of 16 tokens over 65536 279 / 224 and 342 / 256.  So requests of one strip gain what three fifths as many
-// of two lose; rows of 56 on average, up to 128, have no more of these.
+// requests of 32 to 8192 keys, 32 / 8 heads, over f16 (over bf16); rows on average, as a share of the most:
+//   tokens               heads of 128              heads of 64
+//   9              1     176 / 138 (213 / 151)      93 / 80 (109 / 92)     one strip of 64 each
+//   1 to 20        .53   179 / 144 (213 / 157)
+//   1 to 25        .52   181 / 156 (217 / 173)      94 / 91 (111 / 105)    a third have two
+//   1 to 32        .52   195 / 180 (237 / 204)
+//   27, 1, 1, 1    .28   181 / 146 (218 / 161)      96 / 88 (114 / 101)
+//   27, 1          .52   196 / 186 (231 / 210)     104 / 111 (123 / 129)   half have two
+//   17, 1          .53   178 / 170 (219 / 195)      95 / 106
+//   17, 17, 1      .69   183 / 193 (216 / 217)                             two thirds
+//   17, 17, 17, 1  .76   180 / 198 (220 / 221)
+//   25             1     216 / 261                 119 / 152               all
+// Over 65536 keys 4 of 16 tokens take 279 / 224 and 342 / 256.  So half of the requests may have two strips with heads of 128, which
+// the average tells where they are spread out: up to 9/16 of the most.  With heads of 64 that gains too little: one strip
+// each, by max_q.  n_tok is the rows that there may be: where a captured step has room for more than it has
+// rows, the average says too much and strips stay at 128.
 bool may_half(const AttnTreeArgs & a, bool split) { return a.tree_stride && split && attn_dims(a) < 2; }
 bool half(const AttnTreeArgs & a, bool split) {
     const uint64_t most = (uint64_t)a.max_q * a.group;
-    return may_half(a, split) && (most <= 64 || (most <= 128 && (uint64_t)a.n_tok * a.group <= 56ull * a.n_seq));
+    return may_half(a, split) &&
+           (most <= 64 || (attn_dims(a) == 1 && most <= 128 && 16ull * a.n_tok * a.group <= 9 * most * a.n_seq));
 }
 template <typename AT, typename T> int forms(const AttnTreeArgs & a, hipStream_t s) {
     if constexpr (split_terms<AT, T>() > 1)

@@ -281,8 +281,9 @@ __device__ __forceinline__ uint32_t children(const flh_verify_p & p, uint32_t r0
 // Workgroup (row, side, chunk) of the target or of the draft (rows with children), two waves.  Instructions bound it:
 // 20 an element, and 330 a wave for whose row it is and for putting the sums together, so a thread has 32 elements (with 16
 // they take 28 us for 32 requests of 2 to 6 rows of 128256 with a draft, so 25).  Longer shares, the next chunk's logits on their way
-// meanwhile, leave the last workgroups alone for longer than they save.  The target's logits are asked for before it is
-// known whose they are.
+// meanwhile, leave the last workgroups alone for longer than they save.  The target's logits are asked for before it is known
+// whose they are, but only of rows that some request may have: of a captured step with room for four times as many rows the
+// others would be most of the bytes (32 chains 69 us, 48 so; without spare rows 42.5 and 43).
 constexpr int SUM_W = 2;
 template <typename T> __global__ __launch_bounds__(64 * SUM_W) void k_verify_sums(VerArgs a) {
     typedef Chunk<T, false, SUM_W> C;
@@ -296,7 +297,10 @@ template <typename T> __global__ __launch_bounds__(64 * SUM_W) void k_verify_sum
     if (blockIdx.x == 0 && p.draft)
         for (uint32_t i = threadIdx.x; i < p.n_seq; i += 64 * SUM_W) a.done[i] = 0;
     C chunk;
-    if (!draft) chunk.load((const T *)p.target + row * p.t_row, c, p.vocab);
+    if (!draft) {
+        if (row >= p.q_start[p.n_seq]) return;                        // (uniform)
+        chunk.load((const T *)p.target + row * p.t_row, c, p.vocab);
+    }
     VerReq q;
     const bool some = request_of(p, row, q);
     if (draft) {

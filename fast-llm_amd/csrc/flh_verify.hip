@@ -13,7 +13,7 @@
 //
 // Launches: sums of every row's chunks; n_i (only with several children a row); the walk and the
 // draw.  A random number may lie next to the border of two of 10^5 tokens, so weights, sums and
-// borders are in 64 bits: with the exponential below an element costs 18 instructions of a
+// borders are in 64 bits: with the exponential below an element costs 17 instructions of a
 // SIMD, about as much time as its bytes in fp32.
 #include "flh_common.h"
 #include "flh_internal.h"
@@ -279,7 +279,7 @@ __device__ __forceinline__ uint32_t children(const flh_verify_p & p, uint32_t r0
 
 // ------------------------------------------------------------- the rows' sums --
 // Workgroup (row, side, chunk) of the target or of the draft (rows with children), two waves.  Instructions bound it:
-// 20 an element, and 330 a wave for whose row it is and for putting the sums together, so a thread has 32 elements (with 16
+// 17 an element, 15 of them in 64 bits, and 110 a wave for whose row it is and for putting the sums together, so a thread has 32 elements (with 16
 // they take 28 us for 32 requests of 2 to 6 rows of 128256 with a draft, so 25).  Longer shares, the next chunk's logits on their way
 // meanwhile, leave the last workgroups alone for longer than they save.  The target's logits are asked for before it is known
 // whose they are, but only of rows that some request may have: of a captured step with room for four times as many rows the

@@ -509,7 +509,8 @@ int flh_paged_attn(const flh_kv_cache * cache, const flh_attn_p * p, void * stre
  * request is r itself or above it (rows b >= 32 * mask_stride have no bit), with window > 0 only those
  * less than window above it; pos[r] (may be NULL, then kv_len too): kv_len[s] - rows of the
  * request + depth[r].  Rows n_tok and behind, and rows of no request, are left as they are.
- * mask_stride: 1 .. 32768; n_tok: at most 2^30.  Outputs must not overlap anything. */
+ * mask_stride: 1 .. 32768; n_tok: at most 2^30.  Each row's line is walked up, for each
+ * word: the time grows with the trees' depth.  Outputs must not overlap anything. */
 typedef struct flh_tree_plan_p {
     const uint32_t * q_start; const int32_t * parent; const uint32_t * kv_len;
     uint32_t * mask, * depth; int32_t * pos;
@@ -539,16 +540,19 @@ int flh_tree_attn(const flh_kv_cache * cache, const flh_attn_p * p, const flh_tr
  * the first of the largest, whatever the draft; what is not >= 0 counts as 0).  A logit that is no number counts as -infinity, infinity as
  * the largest float.  From row 0 on, a row's children are tested in order: the first one stands if
  * u_accept * q(x) < p(x), and each that does not stand leaves max(p - q, 0), over its sum, as p for the next
- * (without a draft: p without its token).  The path goes on at the first that stands; where none does, or there is
- * none, next is the first token whose sum of what is left of p, up to and with it, passes u_next[s] times the
+ * (without a draft: p without its token; where that is nothing at all, none of the next stands).  The path goes on at
+ * the first that stands; where none does, or there is none, next is the first token whose sum of what is left of p, up to and with it, passes u_next[s] times the
  * whole (nothing left: of p).  Then the tokens of the path and next together are distributed as p alone would
- * have them, u_accept and u_next being uniform in [0, 1).  All of it in 64 bits.
+ * have them, u_accept and u_next being uniform in [0, 1).  Weights, sums and borders are in 64 bits: a weight is right to
+ * 2^-45 of itself and 0 below 2^-1000 of its row's largest (one below 2^-600 counts as about that in the row's sum); without a draft
+ * what fallen tokens leave is 1 less their p, right to 2^-52 of the whole.
  *   n_path[s]: rows of the path, row 0 with it (0 for a request without rows); path[s * path_stride + j]: its
  * rows, by their index in the request, ascending; FLH_KV_NONE behind them.  A path ends at path_stride rows, as if the last one
- * had no children.  next[s]: the token (FLH_KV_NONE where the target allows none, or there is no row).
+ * had no children (whether one would have stood or not).  next[s]: the token (FLH_KV_NONE where the target allows
+ * none, or there is no row).
  * logp (or NULL): entry j of a request, the logarithm of p (of the row, as it was) at the token behind the path's row j: that of row
  * j + 1, at last next; 0 behind.  len (or NULL, then kv_len may be): kv_len[s] - rows + n_path[s], what the
- * request holds then.  ws: flh_spec_verify_ws_bytes of the same arguments, 16-byte aligned, as
+ * request holds then (all of its rows, also those that n_tok cuts off).  ws: flh_spec_verify_ws_bytes of the same arguments, 16-byte aligned, as
  * flh_paged_attn's.  Outputs must not overlap anything, but len may be kv_len.  vocab: 1 .. 2^22; all n_tok rows of target, and
  * of draft, have to be there, also those of no request; n_tok and n_seq, times the
  * vocabulary's chunks of 4096, below 2^24. */

@@ -63,7 +63,9 @@ extern "C" {
 int flh_tree_plan(const flh_tree_plan_p * p, void * stream) {
     if (!p) return set_error(FLH_ERR_ARG, "tree plan: null arguments");
     if (p->mask_stride == 0 || p->mask_stride > 32768) return set_error(FLH_ERR_ARG, "tree plan: mask_stride must be in 1 .. 32768");
-    if (p->n_tok > (1u << 30)) return set_error(FLH_ERR_UNSUPPORTED, "tree plan: n_tok must be at most 2^30");
+    // (a chain of all rows is walked up by each of them for each word: at this size for some seconds)
+    if (p->n_tok > (1u << 22) || (uint64_t)p->n_tok * p->n_tok * p->mask_stride > (1ull << 44))
+        return set_error(FLH_ERR_UNSUPPORTED, "tree plan: n_tok * n_tok * mask_stride must be at most 2^44");
     if (p->n_tok && p->n_seq && (any_null({p->q_start, p->parent, p->mask, p->depth}) || (p->pos && !p->kv_len)))
         return set_error(FLH_ERR_ARG, "tree plan: null argument");
     if (any_off({p->q_start, p->parent, p->kv_len, p->mask, p->depth, p->pos}))

@@ -509,8 +509,8 @@ int flh_paged_attn(const flh_kv_cache * cache, const flh_attn_p * p, void * stre
  * request is r itself or above it (rows b >= 32 * mask_stride have no bit), with window > 0 only those
  * less than window above it; pos[r] (may be NULL, then kv_len too): kv_len[s] - rows of the
  * request + depth[r].  Rows n_tok and behind, and rows of no request, are left as they are.
- * mask_stride: 1 .. 32768; n_tok: at most 2^30.  Each row's line is walked up, for each
- * word: the time grows with the trees' depth.  Outputs must not overlap anything. */
+ * mask_stride: 1 .. 32768.  Each row's line is walked up, for each word, so the time grows with the trees' depth:
+ * n_tok * n_tok * mask_stride is at most 2^44 (2^22 rows with a word each).  Outputs must not overlap anything. */
 typedef struct flh_tree_plan_p {
     const uint32_t * q_start; const int32_t * parent; const uint32_t * kv_len;
     uint32_t * mask, * depth; int32_t * pos;

@@ -1,8 +1,8 @@
-"""Attention counts its units of work in 32 bits: calls whose units could pass that are refused, those that cannot are not."""
+"""Sizes that could pass what the kernels count, or take too long, are refused; those that cannot are not."""
 import pytest
 
 from test_paged_args import S, attn, cache, refused
-from test_spec_args import tree
+from test_spec_args import tree, tree_plan
 
 
 @pytest.mark.parametrize("tree_form", [False, True])
@@ -22,3 +22,14 @@ def test_units(flh, keys, n_seq, n_tok, tree_form):
     more = {**a, "n_seq": 2 * n_seq}
     assert 8 * (n_tok / 16 + 2 * n_seq) * (keys / 64 + 1 + 4) > 4.0e9
     refused(flh, flh.ERR_UNSUPPORTED, "too much work", call, attn(flh, **more, out=1 << 50))
+
+
+@pytest.mark.parametrize("n_tok,stride,ok", [(1 << 22, 1, True), ((1 << 22) + 1, 1, False), (0xFFFFFFFF, 1, False), (1 << 20, 16, True),
+                                             (1 << 20, 17, False), (80_000, 2500, True), (100_000, 32768, False), (1 << 14, 32768, True)])
+def test_plans_end(flh, n_tok, stride, ok):
+    """A plan whose walks, if all rows were one line, would not end for minutes is refused: squares of rows times words."""
+    p = tree_plan(flh, n_tok=n_tok, mask_stride=stride, q_start=None)
+    if ok:                                                    # (the next check refuses it: nothing is launched)
+        refused(flh, flh.ERR_ARG, "null", flh.tree_plan, p, S)
+    else:
+        refused(flh, flh.ERR_UNSUPPORTED, "n_tok", flh.tree_plan, p, S)
